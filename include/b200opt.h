@@ -429,6 +429,142 @@ B200OPT_API int b200opt_adam_mixed_static(size_t n, float alpha, void *weights,
                                           float l2_lambda, uint32_t *flags_out,
                                           void *stream);
 
+/* ------------------------------------------- language-model operators
+ *
+ * The operators of a language model's training step whose parameters' gradients
+ * the optimizer step reads: embedding lookup, layer norm, and the softmax cross
+ * entropy over the vocabulary with the classifier's product, each with its
+ * gradient.  The reference has none of them; its nearest relatives are the
+ * classifier and loss-gradient kernels (src/cuda/cuda_kernels.cu:33-65,388-420).
+ *
+ * Common to all of them:
+ *   - Caller-owned memory of the CURRENT device, asynchronous on `stream` (a
+ *     cudaStream_t), no allocation, no host synchronise, no state kept between
+ *     calls: they may be captured into a graph and replayed.
+ *   - Matrices are row-major with a row stride in ELEMENTS (>= the row length);
+ *     elements of a row are contiguous.  Outputs must not overlap inputs.
+ *     Bytes between a row's end and the next row's start are never written.
+ *   - dtype is B200OPT_HALF or B200OPT_FLOAT, the groups the optimizer has.
+ *     Sums, statistics and products are held in fp32; an fp16 result is rounded
+ *     once, to nearest.
+ *   - Index arrays (ids, targets) are int32 or int64: index_bytes is 4 or 8.
+ *     An index outside [0, vocab) is valid input: a padding id looks up a row
+ *     of zeros and has no gradient, an ignored target has loss 0 and no
+ *     gradient.
+ *   - Results are deterministic: no floating-point atomics, a fixed order of
+ *     every sum for given sizes.
+ *   - `workspace` is device memory of at least the size that the operator's
+ *     _workspace function gives for the same sizes, 256-byte aligned, free to be
+ *     reused once the call's work on `stream` is done.  Calls that may run at
+ *     the same time (two streams, two graphs) need a workspace each.  Its
+ *     contents need no initialisation.
+ *   - `accumulate` != 0 adds the parameter's gradient to what its buffer holds
+ *     (micro-batches, a table shared by embedding and classifier) instead of
+ *     overwriting the buffer.
+ *   - B200OPT_EINVAL: a missing or misaligned pointer, a stride below the row
+ *     length, a dtype or index size out of range, a workspace too small;
+ *     B200OPT_ETOOBIG: a size over B200OPT_LM_MAX; nothing is launched then.
+ *     A failed launch gives B200OPT_ECUDA.
+ */
+#define B200OPT_LM_MAX ((size_t)0x7fffff00) /* tokens, rows, vocab, dim */
+
+/* out[t] = scale * weight[ids[t]], t < tokens; weight is [vocab][dim]. */
+B200OPT_API int b200opt_embedding_fwd(int dtype, size_t tokens, size_t vocab,
+                       size_t dim, const void *ids, int index_bytes,
+                       const void *weight, size_t weight_stride, float scale,
+                       void *out, size_t out_stride, void *stream);
+
+/*
+ * grad_weight[v] = scale * sum over the tokens t with ids[t] == v, in
+ * ascending t, of grad_out[t].  All vocab rows are written (rows that no token
+ * names become zero), so that grad_weight can be a tensor of the flat gradient
+ * buffer; with `accumulate` the sum is added to the rows that tokens name and
+ * the others are not touched.
+ */
+B200OPT_API int b200opt_embedding_bwd_workspace(size_t tokens, size_t vocab,
+                       size_t dim, size_t *bytes);
+B200OPT_API int b200opt_embedding_bwd(int dtype, size_t tokens, size_t vocab,
+                       size_t dim, const void *ids, int index_bytes,
+                       const void *grad_out, size_t grad_out_stride, float scale,
+                       void *grad_weight, size_t grad_weight_stride,
+                       int accumulate, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+/*
+ * Layer norm over the last dimension: y = (x - mean) * rstd * gamma + beta with
+ * rstd = 1/sqrt(variance + eps), the variance taken around the mean.  gamma and
+ * beta are vectors of dtype param_dtype; either may be NULL (1 and 0).  mean and
+ * rstd (fp32, one per row) may be NULL when no gradient will be asked for.
+ * param_dtype B200OPT_HALF needs dtype B200OPT_HALF.
+ */
+B200OPT_API int b200opt_layernorm_fwd(int dtype, int param_dtype, size_t rows,
+                       size_t dim, const void *x, size_t x_stride,
+                       const void *gamma, const void *beta, float eps, void *y,
+                       size_t y_stride, float *mean, float *rstd, void *stream);
+
+/*
+ * Its gradient.  With xh = (x - mean) * rstd and d = grad_y * gamma:
+ *   grad_x     = rstd * (d - mean_row(d) - xh * mean_row(d * xh))
+ *   grad_gamma = sum over rows of grad_y * xh,  grad_beta = sum of grad_y
+ * grad_x, grad_gamma and grad_beta may each be NULL; the last two have dtype
+ * param_dtype and obey `accumulate`.
+ */
+B200OPT_API int b200opt_layernorm_bwd_workspace(size_t rows, size_t dim,
+                       size_t *bytes);
+B200OPT_API int b200opt_layernorm_bwd(int dtype, int param_dtype, size_t rows,
+                       size_t dim, const void *grad_y, size_t grad_y_stride,
+                       const void *x, size_t x_stride, const void *gamma,
+                       const float *mean, const float *rstd, void *grad_x,
+                       size_t grad_x_stride, void *grad_gamma, void *grad_beta,
+                       int accumulate, void *workspace, size_t workspace_bytes,
+                       void *stream);
+
+/*
+ * Softmax cross entropy over the vocabulary together with the classifier's
+ * product, fp16: logits z = hidden weight^T with hidden [tokens][dim] and weight
+ * [vocab][dim], lse[t] = log sum_v exp z[t][v], loss[t] = lse[t] - z[t][target].
+ * The logits are formed in pieces of the vocabulary in fp32 and never stored.
+ *   loss, lse  fp32, one per token (an ignored token has loss 0, its lse is
+ *              written as well)
+ *   stats      two floats: the sum of the losses and the number of tokens that
+ *              were not ignored; may be NULL
+ * dim, the strides and the matrices' addresses are multiples of 8 elements (16
+ * bytes), which every tensor of the flat layout satisfies when dim does.
+ */
+B200OPT_API int b200opt_vocab_loss_fwd_workspace(size_t tokens, size_t vocab,
+                       size_t dim, size_t *bytes);
+B200OPT_API int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim,
+                       const void *hidden, size_t hidden_stride,
+                       const void *weight, size_t weight_stride,
+                       const void *targets, int index_bytes, float *loss,
+                       float *lse, float *stats, void *workspace,
+                       size_t workspace_bytes, void *stream);
+
+/*
+ * Its gradient: with p = exp(z - lse) and
+ *   f = grad_scale * (loss_scale ? *loss_scale : 1) / (stats ? max(stats[1], 1) : 1)
+ *   grad_hidden = f * (p - onehot) weight,  grad_weight = f * (p - onehot)^T hidden
+ * over the tokens that are not ignored (the others have a zero row in
+ * grad_hidden).  lse and stats are the forward pass's; stats NULL asks for the
+ * gradient of the sum of the losses instead of their mean.  loss_scale is a
+ * device address, for instance the one of b200opt_device_scale_ptr.
+ * grad_hidden and grad_weight may each be NULL; grad_weight obeys `accumulate`.
+ * The logits are recomputed piece by piece; p - onehot, at most 1 in magnitude,
+ * is rounded to fp16 after a multiplication by 2^15 (which keeps every
+ * probability over 2e-9 at full fp16 precision), for the tensor cores.
+ */
+B200OPT_API int b200opt_vocab_loss_bwd_workspace(size_t tokens, size_t vocab,
+                       size_t dim, size_t *bytes);
+B200OPT_API int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim,
+                       const void *hidden, size_t hidden_stride,
+                       const void *weight, size_t weight_stride,
+                       const void *targets, int index_bytes, const float *lse,
+                       const float *stats, float grad_scale,
+                       const float *loss_scale, void *grad_hidden,
+                       size_t grad_hidden_stride, void *grad_weight,
+                       size_t grad_weight_stride, int accumulate,
+                       void *workspace, size_t workspace_bytes, void *stream);
+
 /* ------------------------------------------------------- state and options */
 
 /* Iteration counter (AdamMixed::m_iter, src/cuda/cuda_optimizer.cpp:41). */

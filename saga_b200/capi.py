@@ -11,6 +11,7 @@ LIB_PATH = os.path.join(_HERE, "libb200opt.so")
 
 OK, EINVAL, ECUDA, ENOMEM, ETIMEOUT, ESTATE, EUNSUPPORTED, ETOOBIG = 0, -1, -2, -3, -4, -5, -6, -7
 STATIC_MAX_ELEMS = 1 << 30
+LM_MAX = 0x7fffff00
 HALF, FLOAT = 0, 1
 POLICY_REFERENCE, POLICY_INTERVAL = 0, 1
 PATH_AUTO, PATH_PEER, PATH_NCCL, PATH_NVLS = 0, 1, 2, 3
@@ -66,6 +67,21 @@ SIGNATURES = {
     "b200opt_adam_mixed": (_i, [_sz, _f, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _vp, _vp]),
     "b200opt_adam_float": (_i, [_sz, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _vp, _vp]),
     "b200opt_adam_mixed_static": (_i, [_sz, _f, _vp, _vp, _vp, _vp, _vp, _f, _f, _f, _f, _vp, _vp]),
+    "b200opt_embedding_fwd": (_i, [_i, _sz, _sz, _sz, _vp, _i, _vp, _sz, _f, _vp, _sz, _vp]),
+    "b200opt_embedding_bwd_workspace": (_i, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "b200opt_embedding_bwd": (_i, [_i, _sz, _sz, _sz, _vp, _i, _vp, _sz, _f, _vp, _sz, _i, _vp,
+                                   _sz, _vp]),
+    "b200opt_layernorm_fwd": (_i, [_i, _i, _sz, _sz, _vp, _sz, _vp, _vp, _f, _vp, _sz, _vp, _vp,
+                                   _vp]),
+    "b200opt_layernorm_bwd_workspace": (_i, [_sz, _sz, C.POINTER(_sz)]),
+    "b200opt_layernorm_bwd": (_i, [_i, _i, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _vp, _vp, _vp, _sz,
+                                   _vp, _vp, _i, _vp, _sz, _vp]),
+    "b200opt_vocab_loss_fwd_workspace": (_i, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "b200opt_vocab_loss_fwd": (_i, [_sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _i, _vp, _vp, _vp,
+                                    _vp, _sz, _vp]),
+    "b200opt_vocab_loss_bwd_workspace": (_i, [_sz, _sz, _sz, C.POINTER(_sz)]),
+    "b200opt_vocab_loss_bwd": (_i, [_sz, _sz, _sz, _vp, _sz, _vp, _sz, _vp, _i, _vp, _vp, _f, _vp,
+                                    _vp, _sz, _vp, _sz, _i, _vp, _sz, _vp]),
     "b200opt_get_iter": (_i, [_vp, C.POINTER(_i)]),
     "b200opt_set_iter": (_i, [_vp, _i]),
     "b200opt_export_state": (_i, [_vp, _i, _i, _vp, _sz, C.POINTER(_sz)]),

@@ -1,0 +1,84 @@
+// Shared by the language-model operators (embedding, layer norm, vocabulary
+// loss): argument checks of their C entries, element conversions, reductions.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstddef>
+#include <cstdint>
+
+#include "../../include/b200opt.h"
+
+namespace b200 {
+
+inline bool lm_dtype(int dtype) { return dtype == B200OPT_HALF || dtype == B200OPT_FLOAT; }
+inline size_t lm_size(int dtype) { return dtype == B200OPT_HALF ? 2 : 4; }
+inline bool lm_aligned(const void *p, size_t a) { return ((uintptr_t)p & (a - 1)) == 0; }
+inline bool lm_index(int bytes) { return bytes == 4 || bytes == 8; }
+inline size_t lm_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
+
+// A matrix argument: present (when it has elements), aligned to its element,
+// stride not below the row length, and no address beyond 63 bits.
+inline bool lm_matrix(const void *p, size_t rows, size_t cols, size_t stride, size_t elem)
+{
+    if(!rows || !cols)
+        return true;
+    if(!p || !lm_aligned(p, elem) || stride < cols)
+        return false;
+    return stride <= ((size_t)1 << 62) / elem / rows;
+}
+
+// The launches of a call so far, and any error an earlier asynchronous failure
+// left behind: both are reported, neither crosses the C boundary otherwise.
+inline int lm_launched()
+{
+    return cudaGetLastError() == cudaSuccess ? B200OPT_OK : B200OPT_ECUDA;
+}
+
+// The number of SMs of the current device.
+inline bool lm_sms(int *sms)
+{
+    int dev = 0;
+    return cudaGetDevice(&dev) == cudaSuccess &&
+           cudaDeviceGetAttribute(sms, cudaDevAttrMultiProcessorCount, dev) == cudaSuccess;
+}
+
+__device__ __forceinline__ float lm_load(const __half *p) { return __half2float(*p); }
+__device__ __forceinline__ float lm_load(const float *p) { return *p; }
+__device__ __forceinline__ void lm_store(__half *p, float v) { *p = __float2half_rn(v); }
+__device__ __forceinline__ void lm_store(float *p, float v) { *p = v; }
+
+// Element i of an index array, or -1 when it lies outside [0, vocab).
+__device__ __forceinline__ int lm_index_at(const void *ids, int wide, size_t i, size_t vocab)
+{
+    const long long v = wide ? static_cast<const long long *>(ids)[i]
+                             : (long long)static_cast<const int *>(ids)[i];
+    return v >= 0 && v < (long long)vocab ? (int)v : -1;
+}
+
+__device__ __forceinline__ float warp_sum(float v)
+{
+#pragma unroll
+    for(int o = 16; o; o >>= 1)
+        v += __shfl_xor_sync(0xffffffffu, v, o);
+    return v;
+}
+
+// Sum over the block, the same value in every thread; `red` holds one float per
+// warp.  Two barriers: the caller may reuse `red` at once.
+__device__ __forceinline__ float block_sum(float v, float *red)
+{
+    const int warps = blockDim.x >> 5;
+    v = warp_sum(v);
+    if((threadIdx.x & 31) == 0)
+        red[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float s = 0.0f;
+    for(int w = 0; w < warps; w++)
+        s += red[w];
+    __syncthreads();
+    return s;
+}
+
+}  // namespace b200

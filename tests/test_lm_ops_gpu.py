@@ -1,0 +1,630 @@
+"""The language-model operators on a GPU against their definitions in 64 bits.
+
+Tolerances are error bounds, element by element.  u = 2^-24 is half a step of
+fp32.  A sum of n terms that no addend passes more than h additions of is off by
+at most h u times the sum of the magnitudes; h <= n always, and the bounds below
+use h = n where n is small and the length of the longest chain otherwise.
+Results in fp16 are off by half a step, 2^-11 of their size (2^-25 below the
+normal range).  SLACK covers the products of such terms and the few steps of exp,
+log, division and square root that a bound does not name one by one.
+"""
+import ctypes as C
+
+import pytest
+import torch
+
+from saga_b200 import AdamGroup, FlatLayout, capi, layers
+
+pytestmark = pytest.mark.gpu
+
+U = 2.0 ** -24
+SLACK = 1.05
+DEV = "cuda:0"
+
+
+def gen(seed):
+    g = torch.Generator(device=DEV)
+    g.manual_seed(seed)
+    return g
+
+
+def normal(g, *shape, std=1.0, mean=0.0, dtype=torch.float16):
+    return torch.empty(*shape, device=DEV).normal_(mean, std, generator=g).to(dtype)
+
+
+def integers(g, n, low, high, dtype=torch.int64):
+    return torch.randint(low, high, (n,), generator=g, device=DEV).to(dtype)
+
+
+def half_step(exact, dtype):
+    """What the last rounding may be off by."""
+    if dtype == torch.float16:
+        return exact.abs() * 2.0 ** -11 + 2.0 ** -25
+    return exact.abs() * U + 2.0 ** -149
+
+
+def close(got, exact, tol):
+    assert got.shape == exact.shape
+    off = (got.double() - exact).abs()
+    bad = ~(off <= tol * SLACK)
+    assert not bad.any(), (int(bad.sum()), float(off[bad].max()), float((off / (tol + 1e-300)).max()))
+
+
+def strided(t, stride, shift=0):
+    """A copy of the matrix with another row stride, `shift` elements off its allocation's start,
+    between guard values; and a check that nothing around its rows was written."""
+    rows, cols = t.shape
+    buf = torch.full((shift + rows * stride + 16,), 77.0, device=DEV, dtype=t.dtype)
+    view = torch.as_strided(buf, (rows, cols), (stride, 1), shift)
+    view.copy_(t)
+
+    def untouched():
+        keep = view.clone()
+        view.fill_(77.0)
+        ok = bool((buf == 77.0).all())
+        view.copy_(keep)
+        return ok
+    return view, untouched
+
+
+# ----------------------------------------------------------------- embedding
+
+EMB_SIZES = [  # tokens, vocab, dim
+    (1, 1, 1), (1, 1000, 64), (7, 3, 5), (64, 1000, 333), (1000, 17, 40), (1025, 5003, 96),
+    (300, 300, 1032), (2049, 1, 24), (33, 70001, 8), (20011, 211, 16)]
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens,vocab,dim", EMB_SIZES)
+def test_embedding_forward(tokens, vocab, dim, dtype):
+    g = gen(tokens + vocab)
+    w = normal(g, vocab, dim, dtype=dtype)
+    ids = integers(g, tokens, -1, vocab + 1, torch.int32 if tokens % 2 else torch.int64)
+    out, clean = strided(torch.zeros(tokens, dim, device=DEV, dtype=dtype), dim + 3, 1)
+    layers.embedding_forward(ids, w, scale=1.7, out=out)
+    ok = (ids >= 0) & (ids < vocab)
+    scale = float(torch.tensor(1.7, dtype=torch.float32))
+    exact = w[torch.where(ok, ids, 0).long()].double() * scale * ok[:, None]
+    close(out, exact, exact.abs() * U + half_step(exact, dtype))
+    assert (out[~ok] == 0).all() and clean()
+    same = layers.embedding_forward(ids, w, scale=1.7)
+    assert torch.equal(same, out)
+
+
+def embedding_exact(ids, dy, vocab, scale):
+    ok = (ids >= 0) & (ids < vocab)
+    at = torch.where(ok, ids, 0).long()
+    scale = float(torch.tensor(scale, dtype=torch.float32))
+    d = dy.double() * ok[:, None]
+    zero = torch.zeros(vocab, dy.shape[1], device=DEV, dtype=torch.float64)
+    n = torch.zeros(vocab, device=DEV, dtype=torch.float64).index_add_(0, at, ok.double())
+    exact = zero.index_add(0, at, d) * scale
+    size = zero.index_add(0, at, d.abs()) * abs(scale)
+    return exact, size * ((n + 1) * U)[:, None], n      # at most n additions, one product
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
+@pytest.mark.parametrize("tokens,vocab,dim", EMB_SIZES)
+def test_embedding_backward(tokens, vocab, dim, dtype):
+    g = gen(2 * tokens + vocab)
+    dy, _ = strided(normal(g, tokens, dim, dtype=dtype), dim + 1, 1)
+    ids = integers(g, tokens, -1, vocab + 1, torch.int64 if tokens % 2 else torch.int32)
+    ids[tokens // 2:] = ids[tokens // 2].clone()              # one token has at least half of all places
+    exact, tol, n = embedding_exact(ids, dy, vocab, 0.75)
+    dw, clean = strided(torch.full((vocab, dim), float("nan"), device=DEV, dtype=dtype), dim + 2, 3)
+    layers.embedding_backward(ids, dy, vocab, scale=0.75, grad_weight=dw)
+    close(dw, exact, tol + half_step(exact, dtype))
+    assert (dw[n == 0] == 0).all() and clean()
+    again = layers.embedding_backward(ids, dy, vocab, scale=0.75)
+    assert torch.equal(again, dw)                     # the same bits, whatever ran when
+    # accumulating: rows without a token are not touched, not even a NaN
+    base = normal(g, vocab, dim, dtype=dtype)
+    base[n == 0] = float("nan")
+    got = layers.embedding_backward(ids, dy, vocab, scale=0.75, grad_weight=base.clone(), accumulate=True)
+    assert torch.equal(got[n == 0].isnan(), base[n == 0].isnan())
+    total = exact + base.double()
+    close(got[n > 0], total[n > 0], (tol + total.abs() * U + half_step(total, dtype))[n > 0])
+
+
+@pytest.mark.parametrize("pattern", ["none", "all the same", "sorted", "reversed", "two"])
+@pytest.mark.parametrize("tokens", [31, 32, 33, 4096, 16384, 16385, 40000])
+def test_embedding_backward_orders(tokens, pattern):
+    """Orders of ids that leave a sort or a split of a long run nothing to hide behind."""
+    g, vocab, dim = gen(tokens), 30011, 24
+    dy = normal(g, tokens, dim)
+    ids = {"none": lambda: torch.full((tokens,), -100, device=DEV),
+           "all the same": lambda: torch.full((tokens,), vocab - 1, device=DEV),
+           "sorted": lambda: integers(g, tokens, 0, vocab).sort().values,
+           "reversed": lambda: integers(g, tokens, 0, vocab).sort(descending=True).values,
+           "two": lambda: torch.where(integers(g, tokens, 0, 2) > 0, 29999, 3)}[pattern]()
+    exact, tol, n = embedding_exact(ids, dy, vocab, 1.0)
+    close(layers.embedding_backward(ids, dy, vocab), exact, tol + half_step(exact, dy.dtype))
+
+
+def test_embedding_non_finite_values_stay_in_their_rows():
+    ids = torch.tensor([5, 6, 5, 9], device=DEV)
+    dy = torch.ones(4, 40, device=DEV)
+    dy[1], dy[3, 7] = float("nan"), float("inf")
+    dw = layers.embedding_backward(ids, dy, 12)
+    assert dw[6].isnan().all() and dw[9, 7] == float("inf")
+    assert (dw[5] == 2).all() and (dw[9, :7] == 1).all() and dw[[0, 1, 2, 3, 4, 7, 8, 10, 11]].abs().sum() == 0
+
+
+# ---------------------------------------------------------------- layer norm
+
+LN_SIZES = [  # rows, dim
+    (1, 1), (1, 2), (3, 7), (64, 512), (5, 1001), (33, 1024), (9, 4096), (2, 8193), (300, 40),
+    (1030, 264), (4, 16384), (3, 40001), (2000, 8)]
+KINDS = [(torch.float16, torch.float16), (torch.float16, torch.float32), (torch.float32, torch.float32)]
+
+
+def chain(n):
+    """Longest chain of additions over n terms of a row: 32 lanes or more, then a tree."""
+    return min(n, n / 32 + 16)
+
+
+def layernorm_exact(x, gamma, beta, eps):
+    d = x.shape[1]
+    xd = x.double()
+    mean = xd.mean(1, keepdim=True)
+    c = xd - mean
+    var = c.square().mean(1, keepdim=True)
+    rstd = 1.0 / torch.sqrt(var + eps)
+    h = chain(d) + 2
+    e_mean = h * U * xd.abs().mean(1, keepdim=True)
+    # each centred value is off by e_mean and one rounding of the difference
+    e_c = e_mean + U * c.abs()
+    e_var = (2 * c.abs() * e_c + e_c.square()).mean(1, keepdim=True) + (h + 2) * U * var
+    e_rstd = rstd * (0.5 * e_var / (var + eps) + 4 * U)
+    g = gamma.double() if gamma is not None else torch.ones(d, device=DEV, dtype=torch.float64)
+    b = beta.double() if beta is not None else torch.zeros(d, device=DEV, dtype=torch.float64)
+    y = c * rstd * g + b
+    e_y = g.abs() * (e_c * rstd + c.abs() * e_rstd) + 3 * U * (c * rstd * g).abs() + U * y.abs()
+    return y, mean[:, 0], rstd[:, 0], e_y, e_mean[:, 0], e_rstd[:, 0]
+
+
+@pytest.mark.parametrize("dtype,params", KINDS)
+@pytest.mark.parametrize("rows,dim", LN_SIZES)
+def test_layernorm_forward(rows, dim, dtype, params):
+    g = gen(rows + dim)
+    x = normal(g, rows, dim, mean=3.0, std=0.5, dtype=dtype)
+    x[0] = 1.25                                                  # a row without variance
+    gamma, beta = normal(g, dim, dtype=params), normal(g, dim, dtype=params)
+    for shift, ga, be in ((0, gamma, beta), (1, gamma, None), (8, None, beta), (0, None, None)):
+        xs, _ = strided(x, dim + shift, shift)
+        out, clean = strided(torch.zeros_like(x), dim + 2 * shift, shift)
+        eps = float(torch.tensor(1e-5))
+        y, mean, rstd, e_y, e_m, e_r = layernorm_exact(x, ga, be, eps)
+        got, gm, gr = layers.layernorm_forward(xs, ga, be, eps=1e-5, out=out)
+        close(got, y, e_y + half_step(y, dtype))
+        close(gm, mean, e_m + half_step(mean, torch.float32))
+        close(gr, rstd, e_r + half_step(rstd, torch.float32))
+        assert clean()
+
+
+@pytest.mark.parametrize("dtype,params", KINDS)
+@pytest.mark.parametrize("rows,dim", LN_SIZES)
+def test_layernorm_backward(rows, dim, dtype, params):
+    g = gen(3 * rows + dim)
+    x = normal(g, rows, dim, mean=0.5, dtype=dtype)
+    gamma = normal(g, dim, mean=1.0, std=0.2, dtype=params)
+    dy = normal(g, rows, dim, std=0.3, dtype=dtype)
+    xd = x.double()
+    mean = xd.mean(1).float()
+    rstd = (1.0 / torch.sqrt((xd - xd.mean(1, keepdim=True)).square().mean(1) + 1e-5)).float()
+    for shift, ga in ((0, gamma), (1, gamma), (8, None)):
+        kind = params if ga is not None else torch.float32
+        gd = ga.double() if ga is not None else torch.ones(dim, device=DEV, dtype=torch.float64)
+        rs = rstd.double()[:, None]
+        xh = (xd - mean.double()[:, None]) * rs
+        e_xh = 2 * U * xh.abs() + U * rs * xd.abs()
+        d = dy.double() * gd
+        a, b = d.mean(1, keepdim=True), (d * xh).mean(1, keepdim=True)
+        h = chain(dim) + 4
+        e_a = h * U * d.abs().mean(1, keepdim=True)
+        e_b = h * U * (d * xh).abs().mean(1, keepdim=True) + (d.abs() * e_xh).mean(1, keepdim=True)
+        dx = rs * (d - a - xh * b)
+        e_dx = rs * (4 * U * (d.abs() + a.abs() + (xh * b).abs()) + e_a + xh.abs() * e_b + e_xh * b.abs())
+        dg, db = (dy.double() * xh).sum(0), dy.double().sum(0)
+        # all rows in one chain would be the longest order; a block's share and a tree is shorter
+        e_dg = (rows + 3) * U * (dy.double() * xh).abs().sum(0) + (dy.double().abs() * e_xh).sum(0)
+        e_db = (rows + 1) * U * dy.double().abs().sum(0)
+        xs, _ = strided(x, dim + shift, shift)
+        ys, _ = strided(dy, dim + 2 * shift, shift)
+        out, clean = strided(torch.zeros_like(x), dim + shift, shift)
+        gx, gg, gb = layers.layernorm_backward(ys, xs, ga, mean, rstd, grad_x=out)
+        close(gx, dx, e_dx + half_step(dx, dtype))
+        close(gg, dg, e_dg + half_step(dg, kind))
+        close(gb, db, e_db + half_step(db, kind))
+        assert clean()
+        same = layers.layernorm_backward(ys, xs, ga, mean, rstd)
+        assert all(torch.equal(p, q) for p, q in zip(same, (gx, gg, gb)))
+        bg, bb = normal(g, dim, dtype=kind), normal(g, dim, dtype=kind)
+        _, ag, ab = layers.layernorm_backward(ys, xs, ga, mean, rstd, grad_gamma=bg.clone(),
+                                              grad_beta=bb.clone(), accumulate=True)
+        close(ag, dg + bg.double(), e_dg + U * (dg.abs() + bg.double().abs()) + half_step(dg + bg.double(), kind))
+        close(ab, db + bb.double(), e_db + U * (db.abs() + bb.double().abs()) + half_step(db + bb.double(), kind))
+
+
+def test_layernorm_large_mean_and_non_finite_rows():
+    g = gen(5)
+    x = normal(g, 6, 777, mean=4096.0, std=1.0, dtype=torch.float32)
+    y, mean, rstd, e_y, e_m, e_r = layernorm_exact(x, None, None, float(torch.tensor(1e-5)))
+    x[2, 5], x[4, 0] = float("inf"), float("nan")
+    got, gm, gr = layers.layernorm_forward(x)
+    keep = [0, 1, 3, 5]
+    close(got[keep], y[keep], (e_y + half_step(y, torch.float32))[keep])
+    assert got[2].isnan().any() and got[4].isnan().all()
+
+
+def test_layernorm_no_rows_gives_zero_parameter_gradients():
+    x = torch.zeros(0, 96, device=DEV)
+    s = torch.zeros(0, device=DEV)
+    gamma = torch.ones(96, device=DEV)
+    full = lambda: torch.full((96,), 3.0, device=DEV)
+    _, dg, db = layers.layernorm_backward(x, x, gamma, s, s, grad_gamma=full(), grad_beta=full())
+    assert (dg == 0).all() and (db == 0).all()
+    _, dg, db = layers.layernorm_backward(x, x, gamma, s, s, grad_gamma=full(), grad_beta=full(), accumulate=True)
+    assert (dg == 3).all() and (db == 3).all()
+
+
+def test_layernorm_gradient_against_differences():
+    """<dL/dx, w> against (L(x + e w) - L(x - e w)) / 2e with L = sum(c * y), fp32 forward pass.
+    L is off by the rounding of y, at most sum|c| |y| 8 u; the difference by e^2/6 |L'''|, taken
+    as e^2 times the sum of magnitudes."""
+    g = gen(8)
+    x = normal(g, 16, 200, dtype=torch.float32)
+    gamma, c = normal(g, 200, dtype=torch.float32), normal(g, 16, 200, dtype=torch.float32)
+    w = torch.sign(normal(g, 16, 200, dtype=torch.float32))
+    _, mean, rstd = layers.layernorm_forward(x, gamma)
+    dx, _, _ = layers.layernorm_backward(c, x, gamma, mean, rstd)
+    e = 2.0 ** -7
+    ys = [layers.layernorm_forward(x + s * e * w, gamma)[0].double() for s in (1, -1)]
+    diff = ((ys[0] - ys[1]) * c.double()).sum() / (2 * e)
+    size = (c.double() * ys[0]).abs().sum()
+    assert abs(float((dx.double() * w.double()).sum() - diff)) <= float(size * (8 * U / e + e * e))
+
+
+# ----------------------------------------------------------- vocabulary loss
+
+VL_SIZES = [  # tokens, vocab, dim
+    (1, 1, 8), (1, 1000, 64), (3, 7, 64), (64, 1000, 256), (127, 255, 72), (128, 256, 128),
+    (129, 257, 136), (300, 5003, 264), (1000, 333, 1032), (2, 20011, 2048), (513, 1025, 520)]
+
+
+def head_exact(x, w, y, factor, mean=True):
+    """Loss, gradients and what each may be off by."""
+    xd, wd = x.double(), w.double()
+    vocab, dim = w.shape
+    ok = (y >= 0) & (y < vocab)
+    at = torch.where(ok, y, 0).long()
+    z = xd @ wd.t()
+    # products of fp16 are exact in fp32; a tensor core may cut instead of round: 2u an addition
+    e_z = 2 * dim * U * (xd.abs() @ wd.abs().t())
+    lse = torch.logsumexp(z, 1)
+    e_lse = e_z.amax(1) + (chain(vocab) + 16) * U + 2 * U * lse.abs() + 4 * U * z.abs().amax(1)
+    zt = z.gather(1, at[:, None])[:, 0]
+    loss = torch.where(ok, lse - zt, 0.0)
+    e_loss = torch.where(ok, e_lse + e_z.amax(1) + U * loss.abs(), 0.0)
+    n = ok.double().sum()
+    stats = torch.stack([loss.sum(), n])
+    e_stats = torch.stack([e_loss.sum() + chain(len(y)) * U * loss.sum() + len(y) * U * loss.mean(), 0 * n])
+    f = factor / n.clamp(min=1.0) if mean else torch.tensor(factor, device=DEV, dtype=torch.float64)
+    p = torch.exp(z - lse[:, None]) * ok[:, None]
+    one = torch.zeros_like(p).scatter_(1, at[:, None], ok.double()[:, None])
+    dz = p - one
+    e_exp = (e_z + e_lse[:, None] + 4 * U * (1 + (z - lse[:, None]).abs()))
+    # fp16 of 2^15 dz: half a step, 2^-25 / 2^15 below the normal range
+    e_dz = (p * e_exp + (2.0 ** -11 + U) * dz.abs() + 2.0 ** -40) * ok[:, None]
+    dx, dw = f * dz @ wd, f * dz.t() @ xd
+    tokens = len(y)
+    e_dx = f * (e_dz @ wd.abs() + 2 * vocab * U * (dz.abs() @ wd.abs())) + 4 * U * dx.abs()
+    e_dw = f * (e_dz.t() @ xd.abs() + 2 * tokens * U * (dz.abs().t() @ xd.abs())) + 4 * U * dw.abs()
+    return dict(loss=loss, lse=lse, stats=stats, dx=dx, dw=dw, e_loss=e_loss, e_lse=e_lse,
+                e_stats=e_stats, e_dx=e_dx, e_dw=e_dw, ok=ok)
+
+
+def head_inputs(tokens, vocab, dim, seed=0, ignored=0.25):
+    g = gen(tokens + vocab + dim + seed)
+    x = normal(g, tokens, dim)
+    w = normal(g, vocab, dim, std=dim ** -0.5 * 1.5)
+    y = integers(g, tokens, 0, vocab)
+    if ignored:
+        y[torch.rand(tokens, generator=g, device=DEV) < ignored] = -100
+        y[tokens // 3] = vocab
+    return x, w, y
+
+
+def check_head(x, w, y, got_f, got_b, factor, mean=True, base=None):
+    r = head_exact(x, w, y, factor, mean)
+    loss, lse, stats = got_f
+    close(lse, r["lse"], r["e_lse"] + half_step(r["lse"], torch.float32))
+    close(loss, r["loss"], r["e_loss"] + half_step(r["loss"], torch.float32))
+    close(stats, r["stats"], r["e_stats"] + half_step(r["stats"], torch.float32))
+    assert (loss[~r["ok"]] == 0).all()
+    if got_b is None:
+        return
+    dx, dw = got_b
+    close(dx, r["dx"], r["e_dx"] + half_step(r["dx"], torch.float16))
+    if base is None:
+        close(dw, r["dw"], r["e_dw"] + half_step(r["dw"], torch.float16))
+    else:
+        total = r["dw"] + base.double()
+        close(dw, total, r["e_dw"] + U * total.abs() + half_step(total, torch.float16))
+    assert (dx[~r["ok"]] == 0).all()
+
+
+@pytest.mark.parametrize("tokens,vocab,dim", VL_SIZES)
+def test_vocab_loss(tokens, vocab, dim):
+    x, w, y = head_inputs(tokens, vocab, dim)
+    scale = torch.full((1,), 64.0, device=DEV)
+    f = layers.vocab_loss_forward(x, w, y)
+    b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=0.5, loss_scale=scale)
+    check_head(x, w, y, f, b, 32.0)
+    f2 = layers.vocab_loss_forward(x, w, y)
+    b2 = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=0.5, loss_scale=scale)
+    assert all(torch.equal(p, q) for p, q in zip(f + b, f2 + b2))
+
+
+@pytest.mark.parametrize("tokens,vocab,dim", [(65, 300, 72), (260, 130, 200), (5, 1001, 64)])
+def test_vocab_loss_strides_sum_accumulate_int32(tokens, vocab, dim):
+    x, w, y = head_inputs(tokens, vocab, dim, seed=3)
+    xs, _ = strided(x, dim + 8, 8)
+    ws, _ = strided(w, dim + 24, 16)
+    base = normal(gen(1), vocab, dim)
+    dw, clean_w = strided(base, dim + 8, 8)
+    dx, clean_x = strided(torch.full_like(x, float("nan")), dim + 16, 8)
+    f = layers.vocab_loss_forward(xs, ws, y.int())
+    b = layers.vocab_loss_backward(xs, ws, y.int(), f[1], grad_scale=0.25, grad_hidden=dx,
+                                   grad_weight=dw, accumulate=True)
+    check_head(x, w, y, f, b, 0.25, mean=False, base=base)
+    assert clean_x() and clean_w()
+
+
+def test_vocab_loss_several_pieces_of_the_vocabulary():
+    x, w, y = head_inputs(8200, 20000, 64)
+    f = layers.vocab_loss_forward(x, w, y)
+    b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=4096.0)
+    check_head(x, w, y, f, b, 4096.0)
+
+
+@pytest.mark.parametrize("std", [0.0, 30.0])
+def test_vocab_loss_flat_and_peaked_distributions(std):
+    g = gen(17)
+    x, w = normal(g, 70, 64), normal(g, 900, 64, std=std)
+    y = integers(g, 70, 0, 900)
+    f = layers.vocab_loss_forward(x, w, y)
+    b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=8.0)
+    check_head(x, w, y, f, b, 8.0)
+
+
+def test_vocab_loss_all_ignored():
+    x, w, y = head_inputs(40, 100, 64)
+    y[:] = -1
+    f = layers.vocab_loss_forward(x, w, y)
+    b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=1024.0)
+    assert (f[0] == 0).all() and f[2].tolist() == [0.0, 0.0]
+    assert (b[0] == 0).all() and (b[1] == 0).all()
+
+
+def test_vocab_loss_no_tokens():
+    x, w, y = torch.zeros(0, 64, device=DEV).half(), normal(gen(2), 100, 64), torch.zeros(0, device=DEV).long()
+    f = layers.vocab_loss_forward(x, w, y)
+    assert f[2].tolist() == [0.0, 0.0]
+    dx, dw = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2])
+    assert dx.shape == (0, 64) and (dw == 0).all()
+    base = normal(gen(3), 100, 64)
+    _, dw = layers.vocab_loss_backward(x, w, y, f[1], grad_weight=base.clone(), accumulate=True)
+    assert torch.equal(dw, base)
+
+
+def test_vocab_loss_non_finite_tokens_stay_in_their_rows():
+    """A NaN token spoils its own loss and the table's gradient, which the optimizer's flags then
+    report, but no other token's loss or gradient; an ignored NaN token spoils nothing."""
+    x, w, y = head_inputs(300, 500, 64, ignored=0)
+    clean = layers.vocab_loss_forward(x, w, y)
+    x2 = x.clone()
+    x2[7], x2[200, 3] = float("nan"), float("inf")
+    f = layers.vocab_loss_forward(x2, w, y)
+    keep = torch.ones(300, dtype=torch.bool, device=DEV)
+    keep[[7, 200]] = False
+    assert torch.equal(f[0][keep], clean[0][keep]) and not f[0][7].isfinite() and not f[0][200].isfinite()
+    dx, dw = layers.vocab_loss_backward(x2, w, y, f[1], grad_scale=1.0)
+    good, _ = layers.vocab_loss_backward(x, w, y, clean[1], grad_scale=1.0)
+    assert torch.equal(dx[keep], good[keep]) and not dx[7].isfinite().any()
+    assert not dw.isfinite().all()
+
+
+def test_vocab_loss_partial_gradients():
+    """Either gradient alone, through the C entry, equals the one of the full call."""
+    x, w, y = head_inputs(100, 700, 72)
+    f = layers.vocab_loss_forward(x, w, y)
+    dx, dw = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2])
+    ws = torch.empty(layers.vocab_loss_workspace(100, 700, 72)[1], dtype=torch.uint8, device=DEV)
+    vp = lambda t: C.c_void_p(t.data_ptr() if t is not None else None)
+    for keep in (0, 1):
+        out = [torch.zeros_like(dx), None] if keep == 0 else [None, torch.zeros_like(dw)]
+        rc = capi.lib().b200opt_vocab_loss_bwd(
+            100, 700, 72, vp(x), 72, vp(w), 72, vp(y), 8, vp(f[1]), vp(f[2]), 1.0, None, vp(out[0]),
+            72, vp(out[1]), 72, 0, vp(ws), ws.numel(),
+            C.c_void_p(torch.cuda.current_stream().cuda_stream))
+        assert rc == capi.OK
+        assert torch.equal(out[keep], (dx, dw)[keep])
+
+
+def test_vocab_loss_gradient_against_differences():
+    """<dL/dx, s> against (L(x + e s) - L(x - e s)) / 2e, s = +-1, e = 2^-5, x on a grid that
+    keeps x +- e exact in fp16.  The losses are off by their bound; the difference by e^2/6 of a
+    third derivative, at most (2 max|w s|_1)^3 per token, which the grid of weights keeps small."""
+    g = gen(31)
+    tokens, vocab, dim = 24, 500, 64
+    x = torch.round(normal(g, tokens, dim, dtype=torch.float32) * 32).div(32).half()
+    w = normal(g, vocab, dim, std=0.02)
+    y = integers(g, tokens, 0, vocab)
+    s = torch.sign(normal(g, tokens, dim, dtype=torch.float32)).half()
+    e = 2.0 ** -5
+    loss = [layers.vocab_loss_forward(x + k * e * s, w, y)[0].double() for k in (1, -1)]
+    bound = sum(float(head_exact(x + k * e * s, w, y, 1.0)["e_loss"].sum()) for k in (1, -1))
+    _, lse, _ = layers.vocab_loss_forward(x, w, y)
+    dx, _ = layers.vocab_loss_backward(x, w, y, lse, grad_scale=1024.0)
+    r = head_exact(x, w, y, 1024.0, mean=False)
+    span = (s.double() @ w.double().t()).abs().amax(1) * 2
+    tol = bound / (2 * e) + float((span ** 3).sum()) * e * e / 6
+    tol += float((r["e_dx"] + half_step(r["dx"], torch.float16)).sum()) / 1024
+    diff = float((loss[0] - loss[1]).sum() / (2 * e))
+    assert abs(float((dx.double() * s.double()).sum()) / 1024 - diff) <= tol * SLACK
+
+
+# -------------------------------------------- streams, graphs, several at once
+
+def _calls():
+    """A call of each kind: (inputs that change, a function that runs it, its outputs)."""
+    g = gen(4)
+    vocab, dim, tokens = 700, 72, 300
+    ids = integers(g, tokens, 0, vocab)
+    table, x = normal(g, vocab, dim, std=0.2), normal(g, tokens, dim)
+    gamma = normal(g, dim, dtype=torch.float32)
+
+    def run(out=None):
+        e = layers.embedding_forward(ids, table)
+        y, mean, rstd = layers.layernorm_forward(x, gamma)
+        loss, lse, stats = layers.vocab_loss_forward(y, table, ids)
+        dh, dw = layers.vocab_loss_backward(y, table, ids, lse, stats=stats, grad_scale=256.0)
+        dx, dg, db = layers.layernorm_backward(dh, x, gamma, mean, rstd)
+        layers.embedding_backward(ids, dx, vocab, grad_weight=dw, accumulate=True)
+        return [e, y, mean, rstd, loss, lse, stats, dh, dx, dg, db, dw]
+    return (ids, x), run
+
+
+def test_captured_and_replayed():
+    inputs, run = _calls()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.synchronize()
+    graphs = []
+    for _ in range(2):                     # two graphs of the same calls, each with its own memory
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            out = run()
+        graphs.append((graph, out))
+    for seed in (1, 2):
+        g = gen(100 + seed)
+        inputs[0].copy_(integers(g, len(inputs[0]), -3, 705))
+        inputs[1].copy_(normal(g, *inputs[1].shape))
+        want = run()
+        torch.cuda.synchronize()
+        streams = [torch.cuda.Stream() for _ in graphs]
+        for (graph, _), s in zip(graphs, streams):    # at the same time
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for _, out in graphs:
+            assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_two_streams_at_once_and_a_raw_stream():
+    inputs, run = _calls()
+    want = run()
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for s in streams:
+        with torch.cuda.stream(s):
+            for _ in range(3):
+                got.append(run())
+    torch.cuda.synchronize()
+    for out in got:
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    ids, x = inputs
+    out = torch.empty(300, 72, dtype=torch.float16, device=DEV)
+    raw = streams[0].cuda_stream
+    layers.layernorm_forward(x, out=out, mean=torch.empty(300, device=DEV), rstd=torch.empty(300, device=DEV), stream=raw)
+    torch.cuda.synchronize()
+    assert torch.equal(out, layers.layernorm_forward(x)[0])
+    with pytest.raises(ValueError):
+        layers.layernorm_forward(x, stream=raw)
+
+
+def test_tensor_refusals():
+    x = torch.zeros(4, 16, device=DEV)
+    ids = torch.zeros(4, dtype=torch.int64, device=DEV)
+    for call in (lambda: layers.embedding_forward(ids.float(), x),
+                 lambda: layers.embedding_forward(ids, x.double()),
+                 lambda: layers.embedding_forward(ids.cpu(), x),
+                 lambda: layers.embedding_forward(ids, x, out=torch.zeros(3, 16, device=DEV)),
+                 lambda: layers.embedding_backward(ids[:3], x, 10),
+                 lambda: layers.embedding_backward(ids, x, 10, accumulate=True),
+                 lambda: layers.layernorm_forward(x, gamma=torch.zeros(15, device=DEV)),
+                 lambda: layers.layernorm_forward(x, out=x.half()),
+                 lambda: layers.layernorm_forward(x, beta=torch.zeros(16, device=DEV).half()),
+                 lambda: layers.vocab_loss_forward(x, x, ids),
+                 lambda: layers.vocab_loss_forward(x.half(), x.half(), ids[:2]),
+                 lambda: layers.vocab_loss_forward(x.half()[:, :12], x.half()[:, :12], ids),
+                 lambda: layers.vocab_loss_forward(x.half(), x.half()[:, :8], ids)):
+        with pytest.raises((ValueError, TypeError, capi.B200OptError)):
+            call()
+
+
+# -------------------------------------------------- together with the optimizer
+
+def test_training_step_of_a_tied_model_through_the_optimizer():
+    """Embedding -> layer norm -> vocabulary loss with one table for both ends, gradients written
+    into the optimizer's flat buffers (fp16 and fp32 group), loss scale kept on the device: the
+    gradients against torch's in 64 bits, then the fused step, for three steps; then a scale so
+    large that the step must see an overflow and halve it."""
+    vocab, dim, tokens = 1000, 64, 200
+    half, flt = FlatLayout([vocab * dim]), FlatLayout([dim, dim])
+    group = AdamGroup.create(0, 1, 0, half.total, flt.total)
+    try:
+        (wh, gh), (wf, gf) = group.buffers(capi.HALF), group.buffers(capi.FLOAT)
+        pick = lambda buf, lay, k, *shape: buf[lay.slices()[k]].view(*shape)
+        table, d_table = pick(wh, half, 0, vocab, dim), pick(gh, half, 0, vocab, dim)
+        gamma, d_gamma = pick(wf, flt, 0, dim), pick(gf, flt, 0, dim)
+        beta, d_beta = pick(wf, flt, 1, dim), pick(gf, flt, 1, dim)
+        g = gen(77)
+        table.copy_(normal(g, vocab, dim, std=0.1))
+        gamma.fill_(1.0), beta.fill_(0.0)
+        stream = torch.cuda.current_stream().cuda_stream
+        group.init_master(stream)
+        group.device_scale_enable(1024.0)
+        scale_ptr = group.device_scale_ptr()
+        scale = 1024.0
+        for step in range(4):
+            if step == 3:
+                group.device_scale_enable(2.0 ** 40)
+                scale = 2.0 ** 40
+            ids, y = integers(g, tokens, 0, vocab), integers(g, tokens, 0, vocab)
+            y[::5] = -100
+            h = layers.embedding_forward(ids, table, scale=8.0)
+            n, mean, rstd = layers.layernorm_forward(h, gamma, beta)
+            loss, lse, stats = layers.vocab_loss_forward(n, table, y)
+            dn, _ = layers.vocab_loss_backward(n, table, y, lse, stats=stats, loss_scale=scale_ptr,
+                                               grad_weight=d_table)
+            dh, _, _ = layers.layernorm_backward(dn, h, gamma, mean, rstd, grad_gamma=d_gamma,
+                                                 grad_beta=d_beta)
+            layers.embedding_backward(ids, dh, vocab, scale=8.0, grad_weight=d_table, accumulate=True)
+            if step < 3:
+                leaf = [t.double().requires_grad_() for t in (table, gamma, beta)]
+                e = leaf[0][ids] * 8.0
+                nn = torch.nn.functional.layer_norm(e, (dim,), leaf[1], leaf[2], 1e-5)
+                want = torch.nn.functional.cross_entropy(nn @ leaf[0].t(), y, ignore_index=-100)
+                want.backward()
+                # activations and gradients pass five fp16 roundings on the way: 2^-11 each
+                for got, ref in zip((d_table, d_gamma, d_beta), leaf):
+                    ref = ref.grad * scale
+                    rel = float((got.double() - ref).norm() / ref.norm())
+                    assert rel <= 5 * 2.0 ** -11, rel
+                assert abs(float(stats[0] / stats[1]) - float(want)) <= 5 * 2.0 ** -11 * float(want)
+                before = table.clone()
+            group.exec_device_scale(1e-2, 0.0, stream)
+            new, log = group.device_scale_read(stream)
+            if step < 3:
+                assert log[-1][:3] == (0, 0, 0)
+                scale = float(new)
+                moved = (table != before).any(1)
+                assert moved[ids].all()           # every row that was looked up has been updated
+            else:
+                assert log[-1][1] + log[-1][2] > 0 and float(new) == 2.0 ** 39
+    finally:
+        group.destroy()
