@@ -15,7 +15,7 @@ LIB = os.path.join(HERE, "libb200opt.so")
 SOURCES = ["b200opt.cu", "host_logic.cpp", "nccl_path.cpp", "fabric.cpp", "checkpoint.cpp",
            "embedding.cu", "layernorm.cu", "vocab_loss.cu"]
 HEADERS = ["fused_step.cuh", "staged_step.cuh", "nvls_step.cuh", "nccl_path.h", "fabric.h",
-           "lm_common.cuh",
+           "lm_common.cuh", "tc_gemm.cuh",
            os.path.join("..", "..", "include", "b200opt.h")]
 
 

@@ -1,0 +1,452 @@
+// The matrix product of the vocabulary loss: fp16 operands, fp32 accumulation
+// on the tensor cores (tcgen05), with the loss's own epilogues.
+//
+//   acc[m][n] = sum_k A[m][k] B[n][k]
+//
+// A pair of CTAs (a cluster of two) computes a 256 x 256 tile with one
+// cta_group::2 instruction stream: each CTA holds 128 rows of A and 128 rows of
+// B in shared memory and 128 rows x 256 columns of the result in its tensor
+// memory.  A single CTA's 128 x 256 tile would fetch 1.5 times as many bytes from
+// L2 for the same arithmetic (85 against 128 flops a byte), which at the measured
+// tensor rate is more than L2 delivers.
+//
+// Either operand may be "K-major" (k contiguous in memory) or "MN-major" (m or n
+// contiguous): TMA brings boxes of 64 contiguous elements (128 bytes, swizzled)
+// and the shared-memory descriptors say which way they lie, so that no operand
+// is ever transposed in memory.
+//
+// Warps: 0 issues the TMA loads, 1 (of the even CTA) the MMAs, 2 owns the tensor
+// memory, 4..11 are the epilogue.  Two accumulators alternate, so the epilogue
+// of a tile runs beside the main loop of the next one.
+//
+// Every wait is bounded: one that runs out makes the epilogue write NaN for the
+// tiles it did not get, which the loss and the optimizer's overflow flags show.
+#pragma once
+
+#include <cuda.h>
+
+#include "lm_common.cuh"
+
+namespace b200 {
+
+constexpr int kTcTile = 256;    // tile of a CTA pair, both ways
+constexpr int kTcHalf = 128;    // a CTA's rows of A, of B and of the result
+constexpr int kTcK = 64;        // k per stage: 128 bytes, the swizzle's span
+constexpr int kTcStages = 6;
+constexpr int kTcOperand = kTcHalf * kTcK * 2;  // bytes of one operand of a stage in a CTA
+constexpr int kTcThreads = 384;
+constexpr int kTcSmem = kTcStages * 2 * kTcOperand + 1024;
+constexpr unsigned long long kTcWaitNs = 2000000000ull;
+
+struct TcShape {
+    // sizes in elements; a dynamic size is read from *count on the device
+    // and held to at least one row (which the operands then hold as zeros)
+    int m, n, k;
+    const int *count;   // replaces m (dyn_m) or k (dyn_k)
+    int dyn_m, dyn_k;
+    int a_row0, b_row0;  // first row of the tensor maps' outer dimension that is used
+    int splits;          // the k range is cut into so many parts
+    int group;           // m tiles that are walked through before the next n tile
+};
+
+// --------------------------------------------------------------- primitives
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p)
+{
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+__device__ __forceinline__ unsigned long long tc_now()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Waits for the phase; false when the time ran out here or elsewhere in the CTA.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead)
+{
+    for(int i = 0; i < 64; i++)
+        if(mbar_try(bar, parity))
+            return true;
+    const unsigned long long began = tc_now();
+    while(!mbar_try(bar, parity)) {
+        if(*dead || tc_now() - began > kTcWaitNs) {
+            *dead = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank()
+{
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+
+// Address of the same shared variable in another CTA of the cluster.
+__device__ __forceinline__ uint32_t map_to(uint32_t addr, uint32_t rank)
+{
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+    return r;
+}
+
+__device__ __forceinline__ void cluster_sync()
+{
+    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::
+                     : "memory");
+}
+
+// A box of the tensor into this CTA's shared memory; its bytes count on `bar`,
+// a barrier of either CTA of the pair.
+__device__ __forceinline__ void tma_load(uint32_t dst, const CUtensorMap *map, int x, int y,
+                                         uint32_t bar)
+{
+    asm volatile(
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes"
+        " [%0], [%1, {%2, %3}], [%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+}
+
+// Shared-memory descriptor of an operand: 128-byte swizzle.  K-major: rows of
+// 128 bytes, groups of eight rows 1024 bytes apart.  MN-major: one row of 128
+// bytes (64 elements of m or n) per k, groups of eight k 1024 bytes apart, the
+// next 64 elements of m or n 8192 bytes further (one box of 64 k).
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(uint32_t addr)
+{
+    uint64_t d = (uint64_t)((addr & 0x3ffff) >> 4);
+    d |= (uint64_t)(MN ? 8192 >> 4 : 1) << 16;
+    d |= (uint64_t)(1024 >> 4) << 32;
+    d |= (uint64_t)1 << 46;
+    d |= (uint64_t)2 << 61;
+    return d;
+}
+
+// 16 elements of k further within a stage
+template <bool MN>
+__device__ __forceinline__ uint64_t k_step()
+{
+    return (MN ? 16 * 128 : 16 * 2) >> 4;
+}
+
+// kind::f16, fp32 accumulator, fp16 operands, 256 x 256
+template <bool A_MN, bool B_MN>
+__device__ __forceinline__ constexpr uint32_t instruction_desc()
+{
+    return (1u << 4) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u) |
+           ((uint32_t)(kTcTile >> 3) << 17) | ((uint32_t)(kTcTile >> 4) << 24);
+}
+
+__device__ __forceinline__ void mma(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add)
+{
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.u32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add)
+        : "memory");
+}
+
+// Arrives on this barrier of both CTAs when the MMAs issued so far are done.
+__device__ __forceinline__ void mma_commit(uint32_t bar)
+{
+    asm volatile(
+        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64"
+        " [%0], %1;" ::"r"(bar),
+        "h"((uint16_t)3)
+        : "memory");
+}
+
+// 32 columns of this thread's row of the accumulator
+__device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32])
+{
+    uint32_t *r = reinterpret_cast<uint32_t *>(v);
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+          "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+          "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]),
+          "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(addr));
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// ------------------------------------------------------------------- kernel
+
+// Which tile is the i-th: groups of `group` m tiles, within a group n by n.
+struct TcTiles {
+    int mt, nt, group, splits, kblocks;
+    __device__ __forceinline__ TcTiles(const TcShape &s)
+    {
+        const int c = s.dyn_m || s.dyn_k ? max(*s.count, 1) : 0;
+        const int m = s.dyn_m ? c : s.m, k = s.dyn_k ? c : s.k;
+        mt = (m + kTcTile - 1) / kTcTile;
+        nt = (s.n + kTcTile - 1) / kTcTile;
+        kblocks = (k + kTcK - 1) / kTcK;
+        group = s.group;
+        splits = s.splits;
+    }
+    __device__ __forceinline__ long long count() const { return (long long)mt * nt * splits; }
+    __device__ __forceinline__ void at(long long i, int &m, int &n, int &part, int &k0, int &k1) const
+    {
+        const long long tiles = (long long)mt * nt;
+        part = (int)(i / tiles);
+        const long long t = i - part * tiles;
+        const long long per = (long long)group * nt;
+        const int g = (int)(t / per);
+        const int rows = min(group, mt - g * group);
+        const long long r = t - g * per;
+        m = g * group + (int)(r % rows);
+        n = (int)(r / rows);
+        k0 = (int)((long long)kblocks * part / splits);
+        k1 = (int)((long long)kblocks * (part + 1) / splits);
+    }
+};
+
+// Epi: the epilogue.  begin(row, col, part) gives a thread's state for its row
+// of a tile and the 128 columns from col; columns(state, row, col, v) gets 32
+// columns at a time; end(state, row, col) closes them.  Rows and columns beyond
+// the matrix come too and are for the epilogue to leave out.
+template <bool A_MN, bool B_MN, typename Epi>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
+    tc_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
+                   const TcShape shape, const Epi epi)
+{
+    extern __shared__ char smem_raw[];
+    __shared__ __align__(8) uint64_t full[kTcStages], empty[kTcStages], acc_full[2], acc_empty[2];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int dead_word;
+    volatile int *dead = &dead_word;
+
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = cluster_rank();
+    const uint32_t base = (smem_u32(smem_raw) + 1023) & ~1023u;
+
+    if(threadIdx.x == 0) {
+        dead_word = 0;
+        for(int i = 0; i < kTcStages; i++) {
+            mbar_init(smem_u32(&full[i]), 1);
+            mbar_init(smem_u32(&empty[i]), 1);
+        }
+        for(int i = 0; i < 2; i++) {
+            mbar_init(smem_u32(&acc_full[i]), 1);
+            mbar_init(smem_u32(&acc_empty[i]), 2 * 8);  // the epilogue warps of both CTAs
+        }
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if(warp == 2) {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                         smem_u32(&tmem_slot))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
+
+    const TcTiles tiles(shape);
+    const long long total = tiles.count();
+    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+
+    if(warp == 0 && lane == 0) {
+        int stage = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for(long long i = pair; ok && i < total; i += pairs) {
+            int m, n, part, k0, k1;
+            tiles.at(i, m, n, part, k0, k1);
+            const int am = m * kTcTile + (int)rank * kTcHalf, bn = n * kTcTile + (int)rank * kTcHalf;
+            for(int kb = k0; kb < k1; kb++) {
+                if(!(ok = mbar_wait(smem_u32(&empty[stage]), phase ^ 1, dead)))
+                    break;
+                const uint32_t a = base + stage * 2 * kTcOperand, b = a + kTcOperand;
+                const uint32_t bar = map_to(smem_u32(&full[stage]), 0);
+                if(rank == 0)
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
+                                     smem_u32(&full[stage])),
+                                 "r"(4 * kTcOperand)
+                                 : "memory");
+                const int k = kb * kTcK;
+                if(A_MN) {
+                    tma_load(a, &map_a, am, shape.a_row0 + k, bar);
+                    tma_load(a + kTcOperand / 2, &map_a, am + 64, shape.a_row0 + k, bar);
+                } else {
+                    tma_load(a, &map_a, k, shape.a_row0 + am, bar);
+                }
+                if(B_MN) {
+                    tma_load(b, &map_b, bn, shape.b_row0 + k, bar);
+                    tma_load(b + kTcOperand / 2, &map_b, bn + 64, shape.b_row0 + k, bar);
+                } else {
+                    tma_load(b, &map_b, k, shape.b_row0 + bn, bar);
+                }
+                if(++stage == kTcStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+        }
+        if(!ok)  // let the copies in flight land before the CTA's memory goes
+            for(int i = 0; i < 1000; i++)
+                __nanosleep(1000);
+    } else if(warp == 1 && lane == 0 && rank == 0) {
+        constexpr uint32_t idesc = instruction_desc<A_MN, B_MN>();
+        int stage = 0, acc = 0;
+        uint32_t phase = 0, acc_phase = 0;
+        bool ok = true;
+        for(long long i = pair; ok && i < total; i += pairs) {
+            int m, n, part, k0, k1;
+            tiles.at(i, m, n, part, k0, k1);
+            if(!(ok = mbar_wait(smem_u32(&acc_empty[acc]), acc_phase ^ 1, dead)))
+                break;
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            for(int kb = k0; kb < k1; kb++) {
+                if(!(ok = mbar_wait(smem_u32(&full[stage]), phase, dead)))
+                    break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                const uint32_t a = base + stage * 2 * kTcOperand;
+                uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + kTcOperand);
+#pragma unroll
+                for(int s = 0; s < kTcK / 16; s++) {
+                    mma(tmem + acc * kTcTile, da, db, idesc, kb > k0 || s);
+                    da += k_step<A_MN>();
+                    db += k_step<B_MN>();
+                }
+                mma_commit(smem_u32(&empty[stage]));
+                if(++stage == kTcStages) {
+                    stage = 0;
+                    phase ^= 1;
+                }
+            }
+            if(ok)
+                mma_commit(smem_u32(&acc_full[acc]));
+            if(++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1;
+            }
+        }
+    } else if(warp >= 4) {
+        const int quad = warp & 3, side = (warp - 4) >> 2;
+        int acc = 0;
+        uint32_t acc_phase = 0;
+        bool ok = true;
+        for(long long i = pair; i < total; i += pairs) {
+            int m, n, part, k0, k1;
+            tiles.at(i, m, n, part, k0, k1);
+            ok = ok && mbar_wait(smem_u32(&acc_full[acc]), acc_phase, dead);
+            ok = __all_sync(0xffffffffu, ok);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            const int row = m * kTcTile + (int)rank * kTcHalf + quad * 32 + lane;
+            const int col = n * kTcTile + side * kTcHalf;
+            const uint32_t from =
+                tmem + ((uint32_t)(quad * 32) << 16) + acc * kTcTile + side * kTcHalf;
+            auto state = epi.begin(row, col, part);
+#pragma unroll 1
+            for(int c = 0; c < kTcHalf; c += 32) {
+                float v[32];
+                if(ok && k1 > k0) {
+                    tmem_load(from + c, v);
+                } else {  // a part without a share of k, or a wait that ran out
+#pragma unroll
+                    for(int j = 0; j < 32; j++)
+                        v[j] = ok ? 0.0f : __int_as_float(0x7fffffff);
+                }
+                epi.columns(state, row, col + c, v);
+            }
+            epi.end(state, row, col);
+            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+            __syncwarp();
+            if(lane == 0)
+                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                 map_to(smem_u32(&acc_empty[acc]), 0))
+                             : "memory");
+            if(++acc == 2) {
+                acc = 0;
+                acc_phase ^= 1;
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if(warp == 2)
+        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+}
+
+// --------------------------------------------------------------------- host
+
+// Tensor map of a row-major fp16 matrix, boxes of 64 columns x box_rows rows.
+inline bool tc_map(CUtensorMap *map, const void *p, size_t rows, size_t cols, size_t stride,
+                   unsigned box_rows)
+{
+    typedef CUresult (*Encode)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *,
+                               const cuuint64_t *, const cuuint64_t *, const cuuint32_t *,
+                               const cuuint32_t *, CUtensorMapInterleave, CUtensorMapSwizzle,
+                               CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+    static const Encode encode = [] {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q;
+        if(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q) !=
+               cudaSuccess ||
+           q != cudaDriverEntryPointSuccess) {
+            cudaGetLastError();
+            fn = nullptr;
+        }
+        return (Encode)fn;
+    }();
+    if(!encode)
+        return false;
+    const cuuint64_t dims[2] = {cols, rows}, strides[1] = {stride * 2};
+    const cuuint32_t box[2] = {64, box_rows}, steps[2] = {1, 1};
+    return encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, const_cast<void *>(p), dims, strides, box,
+                  steps, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                  CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+// rows of a box: an operand's 128 rows when k is contiguous, 64 k otherwise
+constexpr unsigned tc_box(bool mn) { return mn ? kTcK : kTcHalf; }
+
+template <bool A_MN, bool B_MN, typename Epi>
+bool tc_launch(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, const Epi &epi, int sms,
+               cudaStream_t st)
+{
+    auto *kernel = tc_gemm_kernel<A_MN, B_MN, Epi>;
+    if(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem) != cudaSuccess)
+        return false;
+    const long long tiles = (long long)((s.m + kTcTile - 1) / kTcTile) *
+                            ((s.n + kTcTile - 1) / kTcTile) * s.splits;
+    const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
+    kernel<<<(unsigned)(2 * pairs), kTcThreads, kTcSmem, st>>>(a, b, s, epi);
+    return true;
+}
+
+}  // namespace b200

@@ -1,163 +1,405 @@
 // Softmax cross entropy over the vocabulary with the classifier's product, and
 // its gradient (b200opt_vocab_loss_* of include/b200opt.h).
 #include <algorithm>
+#include <climits>
 
-#include "lm_common.cuh"
+#include "tc_gemm.cuh"
 
 namespace b200 {
 namespace {
 
-constexpr int kTile = 64;
 constexpr size_t kPieceBytes = (size_t)256 << 20;  // of p - onehot held at a time
 constexpr float kLift = 32768.0f;                  // 2^15: see the header
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+constexpr int kPlanPairs = 74;  // CTA pairs that a product is cut for: 148 SMs
 
-// acc[i][j] = sum_k A[m][k] B[n][k] for m = m0 + 4 ty + i, n = n0 + 4 tx + j.
-__device__ __forceinline__ void tile_product(float acc[4][4], const __half *A, size_t am, size_t ak,
-                                             const __half *B, size_t bn, size_t bk, size_t M,
-                                             size_t N, size_t K, size_t m0, size_t n0)
+__device__ __forceinline__ float exp2_fast(float x)
 {
-    __shared__ float sa[16][kTile], sb[16][kTile];
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for(int i = 0; i < 4; i++)
-        for(int j = 0; j < 4; j++)
-            acc[i][j] = 0.0f;
-    for(size_t k0 = 0; k0 < K; k0 += 16) {
-        for(int e = threadIdx.x; e < 16 * kTile; e += 256) {
-            const size_t k = k0 + e / kTile, m = m0 + e % kTile, n = n0 + e % kTile;
-            sa[e / kTile][e % kTile] = k < K && m < M ? __half2float(A[m * am + k * ak]) : 0.0f;
-            sb[e / kTile][e % kTile] = k < K && n < N ? __half2float(B[n * bn + k * bk]) : 0.0f;
-        }
-        __syncthreads();
-        for(int k = 0; k < 16; k++)
-            for(int i = 0; i < 4; i++)
-                for(int j = 0; j < 4; j++)
-                    acc[i][j] += sa[k][4 * ty + i] * sb[k][4 * tx + j];
-        __syncthreads();
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// ------------------------------------------------------------------ forward
+
+// Per row and 128 columns of the vocabulary: the maximum of z log2(e) and the
+// sum of 2^(z log2(e) - maximum), in one pass over the accumulator.  The target's
+// logit goes to zt.
+struct StatsEpilogue {
+    int T, V;
+    const void *y;
+    int wide;
+    float2 *part;
+    float *zt;
+    struct State {
+        float top, sum;
+        int at;
+    };
+    __device__ __forceinline__ State begin(int row, int, int) const
+    {
+        return {-INFINITY, 0.0f, row < T ? lm_index_at(y, wide, row, V) : -1};
     }
-}
+    __device__ __forceinline__ void columns(State &s, int row, int col, float (&v)[32]) const
+    {
+        if(col >= V)
+            return;
+        const int at = s.at - col;
+        if(at >= 0 && at < 32) {
+            float z = v[0];
+#pragma unroll
+            for(int j = 1; j < 32; j++)
+                z = at == j ? v[j] : z;
+            zt[row] = z;
+        }
+        if(V - col < 32) {
+#pragma unroll
+            for(int j = 0; j < 32; j++)
+                v[j] = j < V - col ? v[j] : -INFINITY;
+        }
+        float top = v[0];
+#pragma unroll
+        for(int j = 1; j < 32; j++)
+            top = fmaxf(top, v[j]);
+        top = fmaxf(s.top, top * kLog2e);
+        float sum = s.sum * exp2_fast(s.top - top);
+#pragma unroll
+        for(int j = 0; j < 32; j++)
+            sum += exp2_fast(fmaf(v[j], kLog2e, -top));
+        s.top = top;
+        s.sum = sum;
+    }
+    __device__ __forceinline__ void end(const State &s, int row, int col) const
+    {
+        if(row < T && col < V)
+            part[(size_t)(col / kTcHalf) * T + row] = make_float2(s.top, s.sum);
+    }
+};
 
-// Per row and tile of the vocabulary: the maximum and the sum of exp(z - max).
-__global__ void logits_stats_kernel(size_t T, size_t V, size_t D, const __half *x, size_t xs,
-                                    const __half *w, size_t ws, const void *y, int wide,
-                                    float2 *part, float *zt)
+// Joins the parts of 32 rows: 16 threads a row, then a tree.
+__global__ void __launch_bounds__(512) loss_kernel(int T, int V, int parts, const float2 *part,
+                                                   const float *zt, const void *y, int wide,
+                                                   float *loss, float *lse)
 {
-    __shared__ float z[kTile][kTile + 1];
-    const size_t m0 = (size_t)blockIdx.x * kTile, n0 = (size_t)blockIdx.y * kTile;
-    float acc[4][4];
-    tile_product(acc, x, xs, 1, w, ws, 1, T, V, D, m0, n0);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for(int i = 0; i < 4; i++)
-        for(int j = 0; j < 4; j++)
-            z[4 * ty + i][4 * tx + j] = acc[i][j];
+    __shared__ float2 red[16][33];
+    const int x = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int t = blockIdx.x * 32 + x;
+    float top = -INFINITY, sum = 0.0f;
+    if(t < T)
+        for(int i = w; i < parts; i += 16) {
+            const float2 p = part[(size_t)i * T + t];
+            const float m = fmaxf(top, p.x);
+            sum = sum * exp2_fast(top - m) + p.y * exp2_fast(p.x - m);
+            top = m;
+        }
+    red[w][x] = make_float2(top, sum);
     __syncthreads();
-    const size_t t = m0 + threadIdx.x;
-    if(threadIdx.x >= kTile || t >= T)
+    if(w || t >= T)
         return;
-    const int n = (int)min((size_t)kTile, V - n0), at = lm_index_at(y, wide, t, V);
-    float top = -INFINITY, sum = 0.0f;
-    for(int j = 0; j < n; j++)
-        top = fmaxf(top, z[threadIdx.x][j]);
-    for(int j = 0; j < n; j++)
-        sum += expf(z[threadIdx.x][j] - top);
-    part[blockIdx.y * T + t] = make_float2(top, sum);
-    if(at >= 0 && (size_t)at >= n0 && (size_t)at < n0 + n)
-        zt[t] = z[threadIdx.x][at - n0];
-}
-
-__global__ void loss_kernel(size_t T, size_t V, size_t tiles, const float2 *part, const float *zt,
-                            const void *y, int wide, float *loss, float *lse)
-{
-    const size_t t = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
-    if(t >= T)
-        return;
-    float top = -INFINITY, sum = 0.0f;
-    for(size_t i = 0; i < tiles; i++)
-        top = fmaxf(top, part[i * T + t].x);
-    for(size_t i = 0; i < tiles; i++)
-        sum += part[i * T + t].y * expf(part[i * T + t].x - top);
-    const float l = top + logf(sum);
+    const int used = min(16, parts);
+    for(int i = 1; i < used; i++)
+        top = fmaxf(top, red[i][x].x);
+    sum = 0.0f;
+    for(int i = 0; i < used; i++)
+        sum += red[i][x].y * exp2_fast(red[i][x].x - top);
+    const float l = (top + log2f(sum)) * kLn2;
     lse[t] = l;
     loss[t] = lm_index_at(y, wide, t, V) >= 0 ? l - zt[t] : 0.0f;
 }
 
-__global__ void stats_kernel(size_t T, size_t V, const float *loss, const void *y, int wide,
-                             float *stats)
+__global__ void __launch_bounds__(1024) stats_kernel(int T, int V, const float *loss, const void *y,
+                                                     int wide, float *stats)
 {
     __shared__ float red[32];
-    float s = 0.0f, n = 0.0f;
-    for(size_t t = threadIdx.x; t < T; t += blockDim.x) {
+    float s = 0.0f;
+    int n = 0;
+    for(int t = threadIdx.x; t < T; t += 1024) {
         s += loss[t];
-        n += lm_index_at(y, wide, t, V) >= 0 ? 1.0f : 0.0f;
+        n += lm_index_at(y, wide, t, V) >= 0;
     }
     s = block_sum(s, red);
-    n = block_sum(n, red);
+    const float hi = block_sum((float)(n >> 12), red), lo = block_sum((float)(n & 4095), red);
     if(threadIdx.x == 0) {
         stats[0] = s;
-        stats[1] = n;
+        stats[1] = hi * 4096.0f + lo;  // each sum of whole numbers is exact
     }
 }
 
-// dz[t][v - first] = 2^15 (p - onehot), 0 for ignored tokens
-__global__ void dz_kernel(size_t T, size_t V, size_t D, const __half *x, size_t xs, const __half *w,
-                          size_t ws, const void *y, int wide, const float *lse, size_t first,
-                          size_t count, __half *dz, size_t dzs)
+// ----------------------------------------------------------------- gradient
+
+// The tokens that are not ignored, moved together in their order: their rows of
+// `hidden`, their lse and target, and where they came from.  Ignored tokens then
+// cost nothing in the three products, and what stands in their rows (NaN too)
+// cannot reach the gradient; their rows of grad_hidden are written as zeros
+// here.  Behind the last row, zeros up to the next tile.
+__global__ void __launch_bounds__(256)
+    compact_kernel(int T, int V, int D, int rows_per_block, const __half *x, size_t xs, const void *y,
+                   int wide, const float *lse, __half *xc, float *lsec, int *targetc, int *from,
+                   int *count, __half *dx, size_t dxs)
 {
-    const size_t m0 = (size_t)blockIdx.x * kTile, n0 = (size_t)blockIdx.y * kTile;
-    float acc[4][4];
-    tile_product(acc, x, xs, 1, w + first * ws, ws, 1, T, count, D, m0, n0);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    for(int i = 0; i < 4; i++) {
-        const size_t t = m0 + 4 * ty + i;
-        if(t >= T)
-            continue;
-        const int at = lm_index_at(y, wide, t, V);
-        for(int j = 0; j < 4; j++) {
-            const size_t n = n0 + 4 * tx + j;
-            if(n >= count)
-                continue;
-            const float p = expf(acc[i][j] - lse[t]) - ((size_t)at == first + n ? 1.0f : 0.0f);
-            dz[t * dzs + n] = __float2half_rn(at >= 0 ? p * kLift : 0.0f);
+    __shared__ int before_sum, all_sum, place[32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int r0 = blockIdx.x * rows_per_block;
+    if(tid == 0)
+        before_sum = all_sum = 0;
+    __syncthreads();
+    int before = 0, all = 0;
+    for(int t = tid; t < T; t += 256) {
+        const int ok = lm_index_at(y, wide, t, V) >= 0;
+        all += ok;
+        before += t < r0 && ok;
+    }
+    before = __reduce_add_sync(0xffffffffu, before);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if(lane == 0) {
+        atomicAdd(&before_sum, before);  // whole numbers: any order gives the same
+        atomicAdd(&all_sum, all);
+    }
+    __syncthreads();
+    int next = before_sum;
+    const int total = all_sum, vecs = D / 8;
+    if(blockIdx.x == 0 && tid == 0)
+        *count = total;
+    for(int r = r0; r < min(r0 + rows_per_block, T); r += 32) {
+        if(warp == 0) {
+            const int t = r + lane, id = t < T ? lm_index_at(y, wide, t, V) : -1;
+            const unsigned mask = __ballot_sync(0xffffffffu, id >= 0);
+            const int at = next + __popc(mask & ((1u << lane) - 1));
+            place[lane] = id >= 0 ? at : -1;
+            if(id >= 0) {
+                lsec[at] = lse[t];
+                targetc[at] = id;
+                from[at] = t;
+            }
         }
+        __syncthreads();
+        int seen = 0;
+        for(int j = 0; j < 32; j++)
+            seen += place[j] >= 0;
+        for(int j = warp; j < 32; j += 8) {
+            const int t = r + j, at = place[j];
+            if(t >= T)
+                continue;
+            if(at >= 0) {
+                const uint4 *s = reinterpret_cast<const uint4 *>(x + (size_t)t * xs);
+                uint4 *d = reinterpret_cast<uint4 *>(xc + (size_t)at * D);
+                for(int c = lane; c < vecs; c += 32)
+                    d[c] = s[c];
+            } else if(dx) {
+                uint4 *d = reinterpret_cast<uint4 *>(dx + (size_t)t * dxs);
+                for(int c = lane; c < vecs; c += 32)
+                    d[c] = make_uint4(0, 0, 0, 0);
+            }
+        }
+        next += seen;
+        __syncthreads();
+    }
+    const int pad = max((total + kTcTile - 1) / kTcTile, 1) * kTcTile;
+    for(int r = total + blockIdx.x * 8 + warp; r < pad; r += gridDim.x * 8) {
+        uint4 *d = reinterpret_cast<uint4 *>(xc + (size_t)r * D);
+        for(int c = lane; c < vecs; c += 32)
+            d[c] = make_uint4(0, 0, 0, 0);
     }
 }
 
-__device__ __forceinline__ float factor_of(float scale, const float *loss_scale, const float *stats)
-{
-    const float f = loss_scale ? scale * *loss_scale : scale;
-    return stats ? f / fmaxf(stats[1], 1.0f) : f;
-}
-
-// sum32 += A B^T; with `out`, out = factor 2^-15 sum instead
-__global__ void product_kernel(size_t M, size_t N, size_t K, const __half *A, size_t am, size_t ak,
-                               const __half *B, size_t bn, size_t bk, float *sum32, int begin,
-                               __half *out, size_t os, int accumulate, float scale,
-                               const float *loss_scale, const float *stats)
-{
-    const size_t m0 = (size_t)blockIdx.x * kTile, n0 = (size_t)blockIdx.y * kTile;
-    float acc[4][4];
-    tile_product(acc, A, am, ak, B, bn, bk, M, N, K, m0, n0);
-    const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-    const float f = factor_of(scale, loss_scale, stats) * (1.0f / kLift);
-    for(int i = 0; i < 4; i++)
-        for(int j = 0; j < 4; j++) {
-            const size_t m = m0 + 4 * ty + i, n = n0 + 4 * tx + j;
-            if(m >= M || n >= N)
-                continue;
-            float v = acc[i][j];
-            if(sum32 && !begin)
-                v += sum32[m * N + n];
-            if(out)
-                out[m * os + n] = __float2half_rn(f * v + (accumulate ? __half2float(out[m * os + n]) : 0.0f));
-            else
-                sum32[m * N + n] = v;
+// dz[row][v - first] = 2^15 (p - onehot) in fp16; rows behind the last token are zero
+struct DzEpilogue {
+    const int *count;
+    const float *lse;
+    const int *target;
+    int first;
+    __half *dz;
+    size_t stride;  // a multiple of 256: whole tiles may be written
+    struct State {
+        float c;
+        int at;
+        bool live;
+    };
+    __device__ __forceinline__ State begin(int row, int, int) const
+    {
+        const bool live = row < *count;
+        return {live ? fmaf(lse[row], kLog2e, -15.0f) : 0.0f, live ? target[row] - first : -1, live};
+    }
+    __device__ __forceinline__ void columns(State &s, int row, int col, float (&v)[32]) const
+    {
+        if((size_t)col >= stride)
+            return;
+        const int at = s.at - col;
+        uint4 out[4];
+        __half2 *h = reinterpret_cast<__half2 *>(out);
+#pragma unroll
+        for(int j = 0; j < 32; j++)
+            v[j] = s.live ? exp2_fast(fmaf(v[j], kLog2e, -s.c)) : 0.0f;
+        if(at >= 0 && at < 32) {
+#pragma unroll
+            for(int j = 0; j < 32; j++)
+                v[j] -= at == j ? kLift : 0.0f;
         }
+#pragma unroll
+        for(int j = 0; j < 16; j++)
+            h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
+        uint4 *to = reinterpret_cast<uint4 *>(dz + (size_t)row * stride + col);
+#pragma unroll
+        for(int j = 0; j < 4; j++)
+            to[j] = out[j];
+    }
+    __device__ __forceinline__ void end(const State &, int, int) const {}
+};
+
+struct Factor {
+    float scale;
+    const float *loss_scale, *stats;
+    // of the sums of 2^15 (p - onehot)
+    __device__ __forceinline__ float get() const
+    {
+        const float f = loss_scale ? scale * *loss_scale : scale;
+        return (stats ? f / fmaxf(stats[1], 1.0f) : f) * (1.0f / kLift);
+    }
+};
+
+// One of: sum[part][row] = acc, or += acc; out = factor * (sum + acc) (+ out).
+struct OutEpilogue {
+    int m;
+    const int *count;  // replaces m
+    int n;
+    float *sum;        // fp32, row stride n, one matrix per part; may be null
+    size_t part_stride;
+    int add;           // sum holds earlier pieces
+    __half *out;       // null: into sum
+    size_t stride;
+    const int *rows;   // where a row of the result goes; null: its own place
+    int accumulate;
+    Factor factor;
+    struct State {
+        float *sum;
+        __half *out;
+        float f;
+        bool live;
+    };
+    __device__ __forceinline__ State begin(int row, int, int part) const
+    {
+        State s;
+        s.live = row < (count ? *count : m);
+        s.sum = sum ? sum + part * part_stride + (size_t)row * n : nullptr;
+        s.out = out && s.live ? out + (size_t)(rows ? rows[row] : row) * stride : nullptr;
+        s.f = out ? factor.get() : 0.0f;
+        return s;
+    }
+    __device__ __forceinline__ void columns(State &s, int, int col, float (&v)[32]) const
+    {
+        if(!s.live)
+            return;
+#pragma unroll
+        for(int j = 0; j < 32; j += 8) {
+            if(col + j >= n)  // n is a multiple of 8
+                return;
+            if(sum && add) {
+                const float4 a = *reinterpret_cast<const float4 *>(s.sum + col + j);
+                const float4 b = *reinterpret_cast<const float4 *>(s.sum + col + j + 4);
+                v[j] += a.x, v[j + 1] += a.y, v[j + 2] += a.z, v[j + 3] += a.w;
+                v[j + 4] += b.x, v[j + 5] += b.y, v[j + 6] += b.z, v[j + 7] += b.w;
+            }
+            if(!out) {
+                float4 *to = reinterpret_cast<float4 *>(s.sum + col + j);
+                to[0] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+                to[1] = make_float4(v[j + 4], v[j + 5], v[j + 6], v[j + 7]);
+                continue;
+            }
+            uint4 *to = reinterpret_cast<uint4 *>(s.out + col + j);
+            uint4 bits = accumulate ? *to : make_uint4(0, 0, 0, 0);
+            __half2 *h = reinterpret_cast<__half2 *>(&bits);
+#pragma unroll
+            for(int i = 0; i < 4; i++) {
+                const float2 old = __half22float2(h[i]);
+                float a = s.f * v[j + 2 * i], b = s.f * v[j + 2 * i + 1];
+                if(accumulate)
+                    a += old.x, b += old.y;
+                h[i] = __floats2half2_rn(a, b);
+            }
+            *to = bits;
+        }
+    }
+    __device__ __forceinline__ void end(const State &, int, int) const {}
+};
+
+// Joins the parts of a product that was cut along k, in their order.
+__global__ void __launch_bounds__(256)
+    join_kernel(int m, const int *count, int n, const float *sum, size_t part_stride, int parts,
+                __half *out, size_t stride, const int *rows, int accumulate, Factor factor)
+{
+    const int live = count ? *count : m, vecs = n / 8;
+    const float f = factor.get();
+    const long long total = (long long)live * vecs;
+    for(long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
+        i += (long long)gridDim.x * 256) {
+        const int r = (int)(i / vecs), c = (int)(i % vecs) * 8;
+        float v[8] = {};
+        for(int p = 0; p < parts; p++) {
+            const float4 *s = reinterpret_cast<const float4 *>(sum + p * part_stride + (size_t)r * n + c);
+            const float4 a = s[0], b = s[1];
+            v[0] += a.x, v[1] += a.y, v[2] += a.z, v[3] += a.w;
+            v[4] += b.x, v[5] += b.y, v[6] += b.z, v[7] += b.w;
+        }
+        uint4 *to = reinterpret_cast<uint4 *>(out + (size_t)(rows ? rows[r] : r) * stride + c);
+        uint4 bits = accumulate ? *to : make_uint4(0, 0, 0, 0);
+        __half2 *h = reinterpret_cast<__half2 *>(&bits);
+#pragma unroll
+        for(int j = 0; j < 4; j++) {
+            const float2 old = __half22float2(h[j]);
+            float a = f * v[2 * j], b = f * v[2 * j + 1];
+            if(accumulate)
+                a += old.x, b += old.y;
+            h[j] = __floats2half2_rn(a, b);
+        }
+        *to = bits;
+    }
 }
 
-size_t piece_of(size_t T, size_t V)
+// ------------------------------------------------------------------ planning
+
+size_t tiles_of(size_t n) { return (n + kTcTile - 1) / kTcTile; }
+
+// How many parts the k range of a product is cut into: as many as fill the GPU
+// when its tiles alone do not, each with at least eight stages of k.
+size_t parts_of(size_t m, size_t n, size_t k)
 {
-    const size_t most = std::max<size_t>(kPieceBytes / 2 / std::max<size_t>(T, 1) / 256 * 256, 256);
-    return std::min(lm_up(V, 8), most);
+    const size_t tiles = tiles_of(m) * tiles_of(n), stages = (k + kTcK - 1) / kTcK;
+    return std::max<size_t>(1, std::min(kPlanPairs / tiles, stages / 8));
 }
+
+struct Plan {
+    size_t piece;                    // columns of the vocabulary at a time, a multiple of 256
+    size_t x_parts, w_parts;         // parts of the two gradients' products
+    size_t x_sum, w_sum;             // bytes of their fp32 sums
+    size_t at_x, at_dz, at_lse, at_target, at_from, at_count, at_xsum, at_wsum, bytes;
+    Plan(size_t T, size_t V, size_t D)
+    {
+        T = std::max<size_t>(T, 1);
+        const size_t rows = lm_up(T, kTcTile);
+        const size_t most = std::max<size_t>(kPieceBytes / 2 / rows / kTcTile * kTcTile, kTcTile);
+        piece = std::min(lm_up(V, kTcTile), most);
+        const bool whole = piece >= V;
+        x_parts = parts_of(T, D, std::min(piece, V));
+        w_parts = parts_of(std::min(piece, V), D, T);
+        x_sum = x_parts > 1 || !whole ? x_parts * T * D * 4 : 0;
+        w_sum = w_parts > 1 ? w_parts * std::min(piece, V) * D * 4 : 0;
+        size_t at = 0;
+        auto take = [&](size_t n) {
+            const size_t here = at;
+            at += lm_up(n, 256);
+            return here;
+        };
+        at_x = take(rows * D * 2);
+        at_dz = take(rows * piece * 2);
+        at_lse = take(rows * 4);
+        at_target = take(rows * 4);
+        at_from = take(rows * 4);
+        at_count = take(4);
+        at_xsum = take(x_sum);
+        at_wsum = take(w_sum);
+        bytes = at;
+    }
+};
 
 bool lm_head(size_t T, size_t V, size_t D, const void *x, size_t xs, const void *w, size_t ws,
              const void *y, int index_bytes)
@@ -167,7 +409,17 @@ bool lm_head(size_t T, size_t V, size_t D, const void *x, size_t xs, const void 
            lm_aligned(y, index_bytes);
 }
 
-unsigned tiles_of(size_t n) { return (unsigned)((n + kTile - 1) / kTile); }
+int head_sizes(size_t T, size_t V, size_t D)
+{
+    if(!V || !D)
+        return B200OPT_EINVAL;
+    return T > B200OPT_LM_MAX || V > B200OPT_LM_MAX || D > B200OPT_LM_MAX ? B200OPT_ETOOBIG : B200OPT_OK;
+}
+
+size_t fwd_bytes(size_t T, size_t V)
+{
+    return lm_up(T * 4, 256) + (V + kTcHalf - 1) / kTcHalf * T * 8;
+}
 
 }  // namespace
 }  // namespace b200
@@ -178,11 +430,11 @@ extern "C" {
 
 int b200opt_vocab_loss_fwd_workspace(size_t tokens, size_t vocab, size_t dim, size_t *bytes)
 {
-    if(!bytes || !vocab || !dim)
+    if(!bytes)
         return B200OPT_EINVAL;
-    if(tokens > B200OPT_LM_MAX || vocab > B200OPT_LM_MAX || dim > B200OPT_LM_MAX)
-        return B200OPT_ETOOBIG;
-    *bytes = lm_up(tokens * 4, 256) + (size_t)tiles_of(vocab) * tokens * 8;
+    if(const int rc = head_sizes(tokens, vocab, dim))
+        return rc;
+    *bytes = fwd_bytes(tokens, vocab);
     return B200OPT_OK;
 }
 
@@ -191,10 +443,9 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
                            const void *targets, int index_bytes, float *loss, float *lse,
                            float *stats, void *workspace, size_t workspace_bytes, void *stream)
 {
-    size_t need = 0;
-    const int rc = b200opt_vocab_loss_fwd_workspace(tokens, vocab, dim, &need);
-    if(rc)
+    if(const int rc = head_sizes(tokens, vocab, dim))
         return rc;
+    const size_t need = fwd_bytes(tokens, vocab);
     if(!lm_index(index_bytes) ||
        !lm_head(tokens, vocab, dim, hidden, hidden_stride, weight, weight_stride, targets, index_bytes) ||
        (tokens && (!loss || !lse)) || !lm_aligned(loss, 4) || !lm_aligned(lse, 4) ||
@@ -202,28 +453,35 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
        (need && (!workspace || !lm_aligned(workspace, 256))))
         return B200OPT_EINVAL;
     cudaStream_t st = (cudaStream_t)stream;
-    const int wide = index_bytes == 8;
-    float *zt = (float *)workspace;
-    float2 *part = (float2 *)((char *)workspace + lm_up(tokens * 4, 256));
+    const int wide = index_bytes == 8, T = (int)tokens, V = (int)vocab;
+    if(!tokens && !stats)
+        return B200OPT_OK;
     if(tokens) {
-        logits_stats_kernel<<<dim3(tiles_of(tokens), tiles_of(vocab)), 256, 0, st>>>(
-            tokens, vocab, dim, (const __half *)hidden, hidden_stride, (const __half *)weight,
-            weight_stride, targets, wide, part, zt);
-        loss_kernel<<<(unsigned)((tokens + 127) / 128), 128, 0, st>>>(
-            tokens, vocab, tiles_of(vocab), part, zt, targets, wide, loss, lse);
+        float *zt = (float *)workspace;
+        float2 *part = (float2 *)((char *)workspace + lm_up(tokens * 4, 256));
+        int sms = 0;
+        CUtensorMap mx, mw;
+        if(!lm_sms(&sms) || !tc_map(&mx, hidden, tokens, dim, hidden_stride, tc_box(false)) ||
+           !tc_map(&mw, weight, vocab, dim, weight_stride, tc_box(false)))
+            return B200OPT_ECUDA;
+        TcShape s = {T, V, (int)dim, nullptr, 0, 0, 0, 0, 1, 16};
+        if(!tc_launch<false, false>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt}, sms, st))
+            return B200OPT_ECUDA;
+        loss_kernel<<<(unsigned)((tokens + 31) / 32), 512, 0, st>>>(
+            T, V, (V - 1) / kTcHalf + 1, part, zt, targets, wide, loss, lse);
     }
     if(stats)
-        stats_kernel<<<1, 1024, 0, st>>>(tokens, vocab, loss, targets, wide, stats);
+        stats_kernel<<<1, 1024, 0, st>>>(T, V, loss, targets, wide, stats);
     return lm_launched();
 }
 
 int b200opt_vocab_loss_bwd_workspace(size_t tokens, size_t vocab, size_t dim, size_t *bytes)
 {
-    if(!bytes || !vocab || !dim)
+    if(!bytes)
         return B200OPT_EINVAL;
-    if(tokens > B200OPT_LM_MAX || vocab > B200OPT_LM_MAX || dim > B200OPT_LM_MAX)
-        return B200OPT_ETOOBIG;
-    *bytes = lm_up(tokens * piece_of(tokens, vocab) * 2, 256) + tokens * dim * 4;
+    if(const int rc = head_sizes(tokens, vocab, dim))
+        return rc;
+    *bytes = tokens ? Plan(tokens, vocab, dim).bytes : 0;
     return B200OPT_OK;
 }
 
@@ -235,10 +493,10 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
                            size_t grad_weight_stride, int accumulate, void *workspace,
                            size_t workspace_bytes, void *stream)
 {
-    size_t need = 0;
-    const int rc = b200opt_vocab_loss_bwd_workspace(tokens, vocab, dim, &need);
-    if(rc)
+    if(const int rc = head_sizes(tokens, vocab, dim))
         return rc;
+    const Plan p(tokens, vocab, dim);
+    const size_t need = tokens ? p.bytes : 0;
     if(!lm_index(index_bytes) ||
        !lm_head(tokens, vocab, dim, hidden, hidden_stride, weight, weight_stride, targets, index_bytes) ||
        (tokens && !lse) || !lm_aligned(lse, 4) || !lm_aligned(stats, 4) || !lm_aligned(loss_scale, 4) ||
@@ -249,28 +507,71 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
        workspace_bytes < need || (need && (!workspace || !lm_aligned(workspace, 256))))
         return B200OPT_EINVAL;
     cudaStream_t st = (cudaStream_t)stream;
-    const int wide = index_bytes == 8;
-    const __half *x = (const __half *)hidden, *w = (const __half *)weight;
-    __half *dz = (__half *)workspace;
-    const size_t piece = piece_of(tokens, vocab);
-    float *sum = (float *)((char *)workspace + lm_up(tokens * piece * 2, 256));
-    for(size_t first = 0; first < vocab; first += piece) {
-        const size_t count = std::min(piece, vocab - first);
-        const bool last = first + count == vocab;
-        if(tokens)
-            dz_kernel<<<dim3(tiles_of(tokens), tiles_of(count)), 256, 0, st>>>(
-                tokens, vocab, dim, x, hidden_stride, w, weight_stride, targets, wide, lse, first,
-                count, dz, piece);
-        if(grad_hidden && tokens)
-            product_kernel<<<dim3(tiles_of(tokens), tiles_of(dim)), 256, 0, st>>>(
-                tokens, dim, count, dz, piece, 1, w + first * weight_stride, 1, weight_stride, sum,
-                first == 0, last ? (__half *)grad_hidden : nullptr, grad_hidden_stride, 0, grad_scale,
-                loss_scale, stats);
-        if(grad_weight)
-            product_kernel<<<dim3(tiles_of(count), tiles_of(dim)), 256, 0, st>>>(
-                count, dim, tokens, dz, 1, piece, x, 1, hidden_stride, nullptr, 1,
-                (__half *)grad_weight + first * grad_weight_stride, grad_weight_stride, accumulate,
-                grad_scale, loss_scale, stats);
+    if(!tokens) {
+        if(grad_weight && !accumulate &&
+           cudaMemset2DAsync(grad_weight, grad_weight_stride * 2, 0, dim * 2, vocab, st) != cudaSuccess)
+            return B200OPT_ECUDA;
+        return B200OPT_OK;
+    }
+    int sms = 0;
+    if(!lm_sms(&sms))
+        return B200OPT_ECUDA;
+    const int wide = index_bytes == 8, T = (int)tokens, V = (int)vocab, D = (int)dim;
+    char *ws = (char *)workspace;
+    __half *xc = (__half *)(ws + p.at_x), *dz = (__half *)(ws + p.at_dz);
+    float *lsec = (float *)(ws + p.at_lse);
+    int *target = (int *)(ws + p.at_target), *from = (int *)(ws + p.at_from);
+    int *count = (int *)(ws + p.at_count);
+    float *xsum = p.x_sum ? (float *)(ws + p.at_xsum) : nullptr;
+    float *wsum = p.w_sum ? (float *)(ws + p.at_wsum) : nullptr;
+    const size_t rows = lm_up(tokens, kTcTile);
+    const Factor factor = {grad_scale, loss_scale, stats};
+
+    const int per = (int)std::max<size_t>(32, lm_up((tokens + 4 * sms - 1) / (4 * sms), 32));
+    compact_kernel<<<(T + per - 1) / per, 256, 0, st>>>(
+        T, V, D, per, (const __half *)hidden, hidden_stride, targets, wide, lse, xc, lsec, target, from,
+        count, (__half *)grad_hidden, grad_hidden_stride);
+
+    CUtensorMap x_k, x_mn, w_k, w_mn;
+    if(!tc_map(&x_k, xc, rows, dim, dim, tc_box(false)) || !tc_map(&x_mn, xc, rows, dim, dim, tc_box(true)) ||
+       !tc_map(&w_k, weight, vocab, dim, weight_stride, tc_box(false)) ||
+       !tc_map(&w_mn, weight, vocab, dim, weight_stride, tc_box(true)))
+        return B200OPT_ECUDA;
+    for(size_t first = 0; first < vocab; first += p.piece) {
+        const size_t n = std::min(p.piece, vocab - first);
+        const int N = (int)n, at = (int)first;
+        const bool begin = first == 0, last = first + n == vocab;
+        CUtensorMap dz_k, dz_mn;
+        if(!tc_map(&dz_k, dz, rows, n, p.piece, tc_box(false)) ||
+           !tc_map(&dz_mn, dz, rows, n, p.piece, tc_box(true)))
+            return B200OPT_ECUDA;
+        // dz = p - onehot
+        TcShape s = {T, N, D, count, 1, 0, 0, at, 1, 16};
+        if(!tc_launch<false, false>(x_k, w_k, s, DzEpilogue{count, lsec, target, at, dz, p.piece}, sms, st))
+            return B200OPT_ECUDA;
+        if(grad_hidden) {  // += dz W
+            const bool direct = p.x_parts == 1 && last;
+            s = {T, D, N, count, 1, 0, 0, at, (int)p.x_parts, 8};
+            OutEpilogue e = {T, count, D, xsum, tokens * dim, !begin,
+                             direct ? (__half *)grad_hidden : nullptr, grad_hidden_stride, from, 0, factor};
+            if(!tc_launch<false, true>(dz_k, w_mn, s, e, sms, st))
+                return B200OPT_ECUDA;
+            if(last && !direct)
+                join_kernel<<<sms * 4, 256, 0, st>>>(T, count, D, xsum, tokens * dim, (int)p.x_parts,
+                                                     (__half *)grad_hidden, grad_hidden_stride, from, 0,
+                                                     factor);
+        }
+        if(grad_weight) {  // = dz^T X
+            __half *to = (__half *)grad_weight + first * grad_weight_stride;
+            s = {N, D, T, count, 0, 1, 0, 0, (int)p.w_parts, 8};
+            OutEpilogue e = {N, nullptr, D, wsum, n * dim, 0, p.w_parts == 1 ? to : nullptr,
+                             grad_weight_stride, nullptr, accumulate, factor};
+            if(!tc_launch<true, true>(dz_mn, x_mn, s, e, sms, st))
+                return B200OPT_ECUDA;
+            if(p.w_parts > 1)
+                join_kernel<<<sms * 4, 256, 0, st>>>(N, nullptr, D, wsum, n * dim, (int)p.w_parts, to,
+                                                     grad_weight_stride, nullptr, accumulate, factor);
+        }
     }
     return lm_launched();
 }

@@ -90,6 +90,8 @@ def test_workspace_is_checked(built_library, name, defaults, sizes):
     assert fn(*shape, None) == capi.EINVAL
     n = C.c_size_t()
     assert fn(*([BIG] + shape[1:]), C.byref(n)) == capi.ETOOBIG
+    # no tokens is a size too
+    assert _need(query, *([0] + shape[1:])) <= need
     # larger sizes never need less
     assert _need(query, *[8 * s for s in shape]) >= need
 
@@ -100,6 +102,8 @@ def test_empty_calls_do_nothing(built_library):
     assert _call("b200opt_embedding_fwd", EMB_FWD, tokens=0, **none) == capi.OK
     assert _call("b200opt_embedding_fwd", EMB_FWD, dim=0, **none) == capi.OK
     assert _call("b200opt_embedding_bwd", EMB_BWD, vocab=0, dw=None) == capi.OK
+    assert _call("b200opt_vocab_loss_fwd", VL_FWD, tokens=0, stats=None, x=None, y=None) == capi.OK
+    assert _call("b200opt_vocab_loss_bwd", VL_BWD, tokens=0, dw=None, x=None, y=None) == capi.OK
     assert _call("b200opt_layernorm_fwd", LN_FWD, rows=0, x=None, y=None) == capi.OK
     assert _call("b200opt_layernorm_bwd", LN_BWD, dim=0, x=None, dy=None) == capi.OK
 

@@ -615,7 +615,7 @@ def test_training_step_of_a_tied_model_through_the_optimizer():
                     ref = ref.grad * scale
                     rel = float((got.double() - ref).norm() / ref.norm())
                     assert rel <= 5 * 2.0 ** -11, rel
-                assert abs(float(stats[0] / stats[1]) - float(want)) <= 5 * 2.0 ** -11 * float(want)
+                assert abs(float(stats[0] / stats[1]) - want.item()) <= 5 * 2.0 ** -11 * want.item()
                 before = table.clone()
             group.exec_device_scale(1e-2, 0.0, stream)
             new, log = group.device_scale_read(stream)
