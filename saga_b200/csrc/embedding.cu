@@ -1,39 +1,631 @@
 // Embedding lookup and its gradient (b200opt_embedding_* of include/b200opt.h).
+//
+// Both are bound by memory: the lookup reads and writes `tokens` rows, the
+// gradient reads `tokens` rows and writes the whole table.  Rows are moved in
+// 16-byte vectors where addresses and strides allow it, else element by element.
+#include <algorithm>
+
 #include "lm_common.cuh"
 
 namespace b200 {
 namespace {
 
+// ---------------------------------------------------------- vectors of a row
+
+// N elements of T, moved as one word
+template <typename T, int N>
+struct Vec;
+template <>
+struct Vec<__half, 8> {
+    uint4 w;
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&w);
+#pragma unroll
+        for(int i = 0; i < 4; i++) {
+            const float2 v = __half22float2(h[i]);
+            f[2 * i] = v.x, f[2 * i + 1] = v.y;
+        }
+    }
+    __device__ __forceinline__ void set(const float (&f)[8])
+    {
+        __half2 *h = reinterpret_cast<__half2 *>(&w);
+#pragma unroll
+        for(int i = 0; i < 4; i++)
+            h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    }
+};
+template <>
+struct Vec<float, 4> {
+    float4 w;
+    __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w; }
+    __device__ __forceinline__ void set(const float (&f)[4]) { w = make_float4(f[0], f[1], f[2], f[3]); }
+};
 template <typename T>
-__global__ void embedding_fwd_kernel(size_t vocab, size_t dim, const void *ids, int wide,
-                                     const T *weight, size_t ws, float scale, T *out, size_t os)
+struct Vec<T, 1> {
+    T w;
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = lm_load(&w); }
+    __device__ __forceinline__ void set(const float (&f)[1]) { lm_store(&w, f[0]); }
+};
+
+// ------------------------------------------------------------------- lookup
+
+// `lanes` threads (a power of two) share a row, four vectors each where the row
+// is that long, so that the loads behind an id are in flight together.
+template <typename T, int N>
+__global__ void __launch_bounds__(256)
+    embedding_fwd_kernel(size_t tokens, size_t vocab, size_t vecs, int lanes, const void *ids,
+                         int wide, const T *weight, size_t ws, float scale, T *out, size_t os)
 {
-    const size_t t = blockIdx.x;
-    const int id = lm_index_at(ids, wide, t, vocab);
-    for(size_t d = threadIdx.x; d < dim; d += blockDim.x)
-        lm_store(out + t * os + d, id < 0 ? 0.0f : scale * lm_load(weight + id * ws + d));
+    const int lane = threadIdx.x & (lanes - 1);
+    const size_t groups = (size_t)gridDim.x * (256 / lanes);
+    for(size_t t = (size_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes; t < tokens; t += groups) {
+        const int id = lm_index_at(ids, wide, t, vocab);
+        const Vec<T, N> *from = reinterpret_cast<const Vec<T, N> *>(weight + (id < 0 ? 0 : id) * ws);
+        Vec<T, N> *to = reinterpret_cast<Vec<T, N> *>(out + t * os);
+        for(size_t c0 = lane; c0 < vecs; c0 += 4 * (size_t)lanes) {
+            Vec<T, N> v[4];
+#pragma unroll
+            for(int j = 0; j < 4; j++)
+                if(id >= 0 && c0 + j * lanes < vecs)
+                    v[j] = from[c0 + j * lanes];
+#pragma unroll
+            for(int j = 0; j < 4; j++) {
+                if(c0 + j * lanes >= vecs)
+                    break;
+                float f[N];
+                if(id >= 0)
+                    v[j].get(f);
+#pragma unroll
+                for(int i = 0; i < N; i++)
+                    f[i] = id >= 0 ? scale * f[i] : 0.0f;
+                v[j].set(f);
+                to[c0 + j * lanes] = v[j];
+            }
+        }
+    }
 }
 
-// One block per row of the table: looks for its tokens among all ids.
-template <typename T>
-__global__ void embedding_bwd_kernel(size_t tokens, size_t vocab, size_t dim, const void *ids,
-                                     int wide, const T *dy, size_t ys, float scale, T *dw,
-                                     size_t ws, int accumulate)
+// --------------------------------------------------------- order of the tokens
+//
+// The gradient of a row is the sum over the row's tokens, in ascending token
+// order.  The tokens are brought into that order by a stable radix sort of
+// (id, token), least digit first; ids outside the table get the key `vocab` and
+// end up last.  A warp ranks 32 keys at a time with one match over their digits;
+// a table of counts per warp and digit gives the places.
+
+constexpr int kDigits = 512;      // nine bits a pass: two passes up to 2^18 rows
+constexpr int kSortItems = 16;    // keys a thread holds
+constexpr int kOneBlock = 1024 * kSortItems;  // tokens that one block sorts by itself
+constexpr int kManyThreads = 512;
+constexpr int kManyItems = kManyThreads * kSortItems;
+
+__device__ __forceinline__ uint32_t key_of(const void *ids, int wide, size_t t, size_t vocab)
 {
-    const int v = blockIdx.x;
-    const size_t d = (size_t)blockIdx.y * blockDim.x + threadIdx.x;
-    float sum = 0.0f;
-    bool any = false;
-    for(size_t t = 0; t < tokens; t++)
-        if(lm_index_at(ids, wide, t, vocab) == v) {
-            any = true;
-            if(d < dim)
-                sum += lm_load(dy + t * ys + d);
+    const int id = lm_index_at(ids, wide, t, vocab);
+    return id < 0 ? (uint32_t)vocab : (uint32_t)id;
+}
+
+// Ranks this warp's keys (items i * 32 + lane, i < trips) among its earlier keys
+// of the same digit; count[digit] (this warp's, zeroed) ends as the number of
+// keys.  Keys that do not exist have digit kDigits - 1 + nothing: `live` is false.
+__device__ __forceinline__ void warp_rank(const uint32_t (&key)[kSortItems], int shift, uint32_t mask,
+                                          int trips, unsigned live, uint16_t *count,
+                                          uint16_t (&rank)[kSortItems])
+{
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for(int i = 0; i < kSortItems; i++) {
+        if(i >= trips)
+            break;
+        const bool here = live >> i & 1;
+        const uint32_t d = here ? (key[i] >> shift) & mask : 0xffffffffu;
+        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const int before = __popc(same & ((1u << lane) - 1));
+        if(here)
+            rank[i] = count[d] + before;
+        __syncwarp();
+        if(here && before == 0)
+            count[d] += __popc(same);
+        __syncwarp();
+    }
+}
+
+// One block sorts up to kOneBlock tokens in shared memory.
+__device__ void sort_one_block(int tokens, size_t vocab, int bits, const void *ids, int wide,
+                               char *smem, uint32_t *keys_out, int *order_out)
+{
+    uint32_t *keys = reinterpret_cast<uint32_t *>(smem);
+    uint16_t *order = reinterpret_cast<uint16_t *>(smem + kOneBlock * 4);
+    uint16_t *count = reinterpret_cast<uint16_t *>(smem + kOneBlock * 6);  // [32 warps][kDigits]
+    int *total = reinterpret_cast<int *>(smem + kOneBlock * 6 + 32 * kDigits * 2);  // [kDigits]
+    __shared__ int warp_total[32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int trips = (tokens + 1023) / 1024;
+    const int first = warp * trips * 32 + lane;  // of this thread's keys
+    unsigned live = 0;
+    uint32_t key[kSortItems];
+    uint16_t item[kSortItems], rank[kSortItems];
+#pragma unroll
+    for(int i = 0; i < kSortItems; i++) {
+        const int t = first + 32 * i;
+        if(i < trips && t < tokens) {
+            live |= 1u << i;
+            key[i] = key_of(ids, wide, t, vocab);
+            item[i] = (uint16_t)t;
         }
-    if(d >= dim || (accumulate && !any))
+    }
+    const int passes = (bits + 8) / 9, step = (bits + passes - 1) / passes;
+    for(int p = 0; p < passes; p++) {
+        const int shift = p * step;
+        const uint32_t mask = (1u << step) - 1;
+        for(int i = tid; i < 32 * kDigits / 2; i += 1024)
+            reinterpret_cast<uint32_t *>(count)[i] = 0;
+        __syncthreads();
+        warp_rank(key, shift, mask, trips, live, count + warp * kDigits, rank);
+        __syncthreads();
+        // exclusive sums: digit by digit, within a digit warp by warp
+        int sum = 0;
+        if(tid < kDigits) {
+            for(int w = 0; w < 32; w++) {
+                const int c = count[w * kDigits + tid];
+                count[w * kDigits + tid] = (uint16_t)sum;
+                sum += c;
+            }
+            int run = sum;
+#pragma unroll
+            for(int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, run, o);
+                run += lane >= o ? v : 0;
+            }
+            total[tid] = run - sum;
+            if(lane == 31)
+                warp_total[warp] = run;
+        }
+        __syncthreads();
+        if(tid < kDigits) {
+            int ahead = 0;
+            for(int w = 0; w < warp; w++)
+                ahead += warp_total[w];
+            total[tid] += ahead;
+        }
+        __syncthreads();
+#pragma unroll
+        for(int i = 0; i < kSortItems; i++)
+            if(live >> i & 1) {
+                const uint32_t d = (key[i] >> shift) & mask;
+                const int at = total[d] + count[warp * kDigits + d] + rank[i];
+                keys[at] = key[i];
+                order[at] = item[i];
+            }
+        __syncthreads();
+        if(p + 1 < passes) {
+#pragma unroll
+            for(int i = 0; i < kSortItems; i++)
+                if(live >> i & 1) {
+                    key[i] = keys[first + 32 * i];
+                    item[i] = order[first + 32 * i];
+                }
+        }
+    }
+    for(int i = tid; i < tokens; i += 1024) {
+        keys_out[i] = keys[i];
+        order_out[i] = order[i];
+    }
+}
+
+constexpr int kSortSmem = kOneBlock * 6 + 32 * kDigits * 2 + kDigits * 4;
+
+// More tokens: per pass, counts of every block of keys, their sums, the move.
+// The first pass reads the ids themselves.
+__device__ __forceinline__ unsigned load_keys(size_t tokens, size_t vocab, const void *ids, int wide,
+                                              const uint32_t *keys, const int *order,
+                                              uint32_t (&key)[kSortItems], int (&item)[kSortItems])
+{
+    const size_t first = (size_t)blockIdx.x * kManyItems + (threadIdx.x >> 5) * (32 * kSortItems) +
+                         (threadIdx.x & 31);
+    unsigned live = 0;
+#pragma unroll
+    for(int i = 0; i < kSortItems; i++) {
+        const size_t t = first + 32 * i;
+        if(t < tokens) {
+            live |= 1u << i;
+            key[i] = keys ? keys[t] : key_of(ids, wide, t, vocab);
+            item[i] = keys ? order[t] : (int)t;
+        }
+    }
+    return live;
+}
+
+__global__ void __launch_bounds__(kManyThreads)
+    sort_count_kernel(size_t tokens, size_t vocab, const void *ids, int wide, const uint32_t *keys,
+                      const int *order, int shift, uint32_t mask, int *counts, int blocks)
+{
+    __shared__ int count[kDigits];
+    for(int i = threadIdx.x; i < kDigits; i += kManyThreads)
+        count[i] = 0;
+    __syncthreads();
+    uint32_t key[kSortItems];
+    int item[kSortItems];
+    const unsigned live = load_keys(tokens, vocab, ids, wide, keys, order, key, item);
+#pragma unroll
+    for(int i = 0; i < kSortItems; i++)
+        if(live >> i & 1)
+            atomicAdd(&count[(key[i] >> shift) & mask], 1);  // whole numbers: no order
+    __syncthreads();
+    for(int i = threadIdx.x; i < kDigits; i += kManyThreads)
+        counts[(size_t)i * blocks + blockIdx.x] = count[i];
+}
+
+__global__ void __launch_bounds__(1024) sort_sums_kernel(int *counts, int n)
+{
+    __shared__ int warp_total[32];
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    int base = 0;
+    for(int i0 = 0; i0 < n; i0 += 1024) {
+        const int i = i0 + tid, c = i < n ? counts[i] : 0;
+        int run = c;
+#pragma unroll
+        for(int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, run, o);
+            run += lane >= o ? v : 0;
+        }
+        if(lane == 31)
+            warp_total[warp] = run;
+        __syncthreads();
+        int ahead = 0, all = 0;
+        for(int w = 0; w < 32; w++) {
+            ahead += w < warp ? warp_total[w] : 0;
+            all += warp_total[w];
+        }
+        if(i < n)
+            counts[i] = base + ahead + run - c;
+        base += all;
+        __syncthreads();
+    }
+}
+
+__global__ void __launch_bounds__(kManyThreads)
+    sort_move_kernel(size_t tokens, size_t vocab, const void *ids, int wide, const uint32_t *keys,
+                     const int *order, int shift, uint32_t mask, const int *counts, int blocks,
+                     uint32_t *keys_out, int *order_out)
+{
+    constexpr int kWarps = kManyThreads / 32;
+    __shared__ uint16_t count[kWarps * kDigits];
+    for(int i = threadIdx.x; i < kWarps * kDigits / 2; i += kManyThreads)
+        reinterpret_cast<uint32_t *>(count)[i] = 0;
+    __syncthreads();
+    uint32_t key[kSortItems];
+    int item[kSortItems];
+    uint16_t rank[kSortItems];
+    const int warp = threadIdx.x >> 5;
+    const unsigned live = load_keys(tokens, vocab, ids, wide, keys, order, key, item);
+    warp_rank(key, shift, mask, kSortItems, live, count + warp * kDigits, rank);
+    __syncthreads();
+    for(int d = threadIdx.x; d < kDigits; d += kManyThreads) {
+        int sum = 0;
+        for(int w = 0; w < kWarps; w++) {
+            const int c = count[w * kDigits + d];
+            count[w * kDigits + d] = (uint16_t)sum;
+            sum += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for(int i = 0; i < kSortItems; i++)
+        if(live >> i & 1) {
+            const uint32_t d = (key[i] >> shift) & mask;
+            const int at = counts[(size_t)d * blocks + blockIdx.x] + count[warp * kDigits + d] + rank[i];
+            keys_out[at] = key[i];
+            order_out[at] = item[i];
+        }
+}
+
+// --------------------------------------------------------- rows without tokens
+
+constexpr int kFillRows = 32768;  // rows that a block marks at a time
+
+// Zeros into the rows [v0, v1) that no id names.  With `sorted` the keys are in
+// order and only their stretch of the range is looked at.
+template <typename T, int N>
+__device__ void fill_rows(size_t v0, size_t v1, size_t tokens, size_t vocab, const void *ids, int wide,
+                          const uint32_t *sorted, T *dw, size_t ws, size_t vecs)
+{
+    __shared__ uint32_t named[kFillRows / 32];
+    for(size_t a = v0; a < v1; a += kFillRows) {
+        const size_t b = min(a + kFillRows, v1);
+        for(int i = threadIdx.x; i < kFillRows / 32; i += blockDim.x)
+            named[i] = 0;
+        __syncthreads();
+        size_t lo = 0, hi = tokens;
+        if(sorted) {  // first key >= a
+            while(lo < hi) {
+                const size_t mid = (lo + hi) / 2;
+                if(sorted[mid] < a)
+                    lo = mid + 1;
+                else
+                    hi = mid;
+            }
+        }
+        for(size_t t = lo + threadIdx.x; t < tokens; t += blockDim.x) {
+            const size_t k = sorted ? sorted[t] : key_of(ids, wide, t, vocab);
+            if(k >= a && k < b)
+                atomicOr(&named[(k - a) / 32], 1u << ((k - a) & 31));
+            else if(sorted)
+                break;
+        }
+        __syncthreads();
+        Vec<T, N> zero;
+        float f[N] = {};
+        zero.set(f);
+        if(vecs <= 0xffffffffu / kFillRows) {
+            const uint32_t n = (uint32_t)(b - a) * (uint32_t)vecs, per = (uint32_t)vecs;
+            for(uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
+                const uint32_t r = i / per, c = i - r * per;
+                if(!(named[r / 32] >> (r & 31) & 1))
+                    reinterpret_cast<Vec<T, N> *>(dw + (a + r) * ws)[c] = zero;
+            }
+        } else {
+            for(size_t r = 0; r < b - a; r++)
+                if(!(named[r / 32] >> (r & 31) & 1))
+                    for(size_t c = threadIdx.x; c < vecs; c += blockDim.x)
+                        reinterpret_cast<Vec<T, N> *>(dw + (a + r) * ws)[c] = zero;
+        }
+        __syncthreads();
+    }
+}
+
+// Block 0 sorts; the others, meanwhile, write the rows without tokens.
+template <typename T, int N>
+__global__ void __launch_bounds__(1024)
+    sort_fill_kernel(int tokens, size_t vocab, int bits, const void *ids, int wide, uint32_t *keys,
+                     int *order, T *dw, size_t ws, size_t vecs)
+{
+    extern __shared__ __align__(16) char sort_smem[];
+    if(blockIdx.x == 0) {
+        sort_one_block(tokens, vocab, bits, ids, wide, sort_smem, keys, order);
+    } else {
+        const size_t blocks = gridDim.x - 1, b = blockIdx.x - 1;
+        fill_rows<T, N>(vocab * b / blocks, vocab * (b + 1) / blocks, tokens, vocab, ids, wide, nullptr,
+                        dw, ws, vecs);
+    }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(1024)
+    fill_kernel(size_t tokens, size_t vocab, const uint32_t *sorted, T *dw, size_t ws, size_t vecs)
+{
+    const size_t blocks = gridDim.x, b = blockIdx.x;
+    fill_rows<T, N>(vocab * b / blocks, vocab * (b + 1) / blocks, tokens, vocab, nullptr, 0, sorted, dw,
+                    ws, vecs);
+}
+
+// ----------------------------------------------------------- sums of the rows
+//
+// The sorted tokens are cut into chunks of kChunk whatever their ids are, so a
+// token that fills half the batch is summed by as many groups of threads as any
+// other half.  A run of equal ids that lies inside a chunk is summed and written;
+// of one that does not, each chunk leaves its part: slot 0 for a run that came
+// from the chunk before, slot 1 for one that begins here.  join_kernel adds up
+// the parts, in order.
+
+constexpr int kChunk = 32;
+constexpr int kAhead = 8;  // rows in flight per thread
+
+template <typename T, int N>
+__device__ __forceinline__ void write_row(T *row, size_t c, float (&sum)[N], float scale, int accumulate)
+{
+    Vec<T, N> *to = reinterpret_cast<Vec<T, N> *>(row) + c;
+    float f[N], old[N] = {};
+    if(accumulate)
+        to->get(old);
+#pragma unroll
+    for(int i = 0; i < N; i++)
+        f[i] = accumulate ? fmaf(scale, sum[i], old[i]) : scale * sum[i];
+    Vec<T, N> v;
+    v.set(f);
+    *to = v;
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(256)
+    sum_kernel(size_t tokens, size_t vocab, size_t vecs, int lanes, const uint32_t *keys,
+               const int *order, const T *dy, size_t ys, float scale, T *dw, size_t ws,
+               int accumulate, float *parts)
+{
+    const size_t chunk = (size_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const size_t c = (size_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+    const size_t e0 = chunk * kChunk;
+    if(e0 >= tokens || c >= vecs)
         return;
-    T *to = dw + v * ws + d;
-    lm_store(to, scale * sum + (accumulate ? lm_load(to) : 0.0f));
+    const int n = (int)min((size_t)kChunk, tokens - e0);
+    uint32_t run = keys[e0];
+    bool came = e0 > 0 && keys[e0 - 1] == run;  // the run began in an earlier chunk
+    float sum[N] = {};
+    for(int i0 = 0; i0 < n; i0 += kAhead) {
+        Vec<T, N> v[kAhead];
+        uint32_t next[kAhead];  // the key behind each of the tokens
+#pragma unroll
+        for(int i = 0; i < kAhead; i++)
+            if(i0 + i < n) {
+                v[i] = reinterpret_cast<const Vec<T, N> *>(dy + (size_t)order[e0 + i0 + i] * ys)[c];
+                next[i] = e0 + i0 + i + 1 < tokens ? keys[e0 + i0 + i + 1] : 0xffffffffu;
+            }
+#pragma unroll
+        for(int i = 0; i < kAhead; i++) {
+            if(i0 + i >= n)
+                break;
+            if(run >= vocab)  // ids outside the table: all that follow are
+                return;
+            float f[N];
+            v[i].get(f);
+#pragma unroll
+            for(int j = 0; j < N; j++)
+                sum[j] += f[j];
+            const bool ends = next[i] != run;
+            if(ends || i0 + i + 1 == n) {
+                if(ends && !came) {
+                    write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
+                } else {
+                    float *to = parts + ((chunk * 2 + (came ? 0 : 1)) * vecs + c) * N;
+#pragma unroll
+                    for(int j = 0; j < N; j++)
+                        to[j] = sum[j];
+                }
+#pragma unroll
+                for(int j = 0; j < N; j++)
+                    sum[j] = 0.0f;
+                run = next[i];
+                came = false;
+            }
+        }
+    }
+}
+
+template <typename T, int N>
+__global__ void __launch_bounds__(256)
+    join_rows_kernel(size_t tokens, size_t vocab, size_t vecs, int lanes, const uint32_t *keys,
+                     float scale, T *dw, size_t ws, int accumulate, const float *parts)
+{
+    const size_t chunk = (size_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
+    const size_t c = (size_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+    const size_t e0 = chunk * kChunk, e1 = e0 + kChunk;
+    if(e1 >= tokens || c >= vecs)
+        return;
+    const uint32_t run = keys[e1 - 1];
+    // the run that leaves this chunk, if it began here
+    if(run >= vocab || keys[e1] != run || (e0 > 0 && keys[e0] == run && keys[e0 - 1] == run))
+        return;
+    size_t lo = e1, hi = tokens;  // its end: the first key beyond
+    while(lo < hi) {
+        const size_t mid = (lo + hi) / 2;
+        if(keys[mid] <= run)
+            lo = mid + 1;
+        else
+            hi = mid;
+    }
+    const size_t last = (lo - 1) / kChunk;
+    float sum[N];
+    const float *first = parts + ((chunk * 2 + 1) * vecs + c) * N;
+#pragma unroll
+    for(int j = 0; j < N; j++)
+        sum[j] = first[j];
+#pragma unroll 8
+    for(size_t k = chunk + 1; k <= last; k++) {
+        const float *p = parts + (k * 2 * vecs + c) * N;
+#pragma unroll
+        for(int j = 0; j < N; j++)
+            sum[j] += p[j];
+    }
+    write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
+}
+
+// ---------------------------------------------------------------- host side
+
+// Threads that share a row of `vecs` vectors with `each` of them per thread.
+int lanes_of(size_t vecs, size_t each)
+{
+    int lanes = 1;
+    while(lanes < 256 && lanes * each < vecs)
+        lanes *= 2;
+    return lanes;
+}
+
+bool vectors(const void *p, size_t stride, size_t elem, size_t dim)
+{
+    return lm_aligned(p, 16) && stride * elem % 16 == 0 && dim * elem % 16 == 0;
+}
+
+template <typename T, int N>
+int lookup(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide, const void *weight,
+           size_t ws, float scale, void *out, size_t os, cudaStream_t st)
+{
+    const size_t vecs = dim / N;
+    const int lanes = lanes_of(vecs, 4);
+    const size_t blocks = std::min<size_t>((tokens * lanes + 255) / 256, 1 << 20);
+    embedding_fwd_kernel<T, N><<<(unsigned)blocks, 256, 0, st>>>(
+        tokens, vocab, vecs, lanes, ids, wide, (const T *)weight, ws, scale, (T *)out, os);
+    return lm_launched();
+}
+
+struct Work {
+    size_t blocks;  // of the sort
+    size_t at_keys, at_order, at_keys2, at_order2, at_counts, at_parts, bytes;
+    Work(size_t tokens, size_t dim)
+    {
+        size_t at = 0;
+        auto take = [&](size_t n) {
+            const size_t here = at;
+            at += lm_up(n, 256);
+            return here;
+        };
+        const bool many = tokens > kOneBlock;
+        blocks = (tokens + kManyItems - 1) / kManyItems;
+        at_keys = take(tokens * 4);
+        at_order = take(tokens * 4);
+        at_keys2 = take(many ? tokens * 4 : 0);
+        at_order2 = take(many ? tokens * 4 : 0);
+        at_counts = take(many ? blocks * kDigits * 4 : 0);
+        at_parts = take((tokens + kChunk - 1) / kChunk * 2 * dim * 4);
+        bytes = at;
+    }
+};
+
+template <typename T, int N>
+int gradient(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide, const void *dy,
+             size_t ys, float scale, void *dw, size_t ws, int accumulate, char *work, cudaStream_t st)
+{
+    const Work w(tokens, dim);
+    const size_t vecs = dim / N;
+    uint32_t *keys = (uint32_t *)(work + w.at_keys);
+    int *order = (int *)(work + w.at_order);
+    int sms = 0;
+    if(!lm_sms(&sms))
+        return B200OPT_ECUDA;
+    int bits = 0;  // of the largest key, `vocab`
+    while(vocab >> bits)
+        bits++;
+    const unsigned fill = (unsigned)std::min<size_t>(sms, vocab);
+    if(tokens <= kOneBlock) {
+        if(cudaFuncSetAttribute(sort_fill_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                kSortSmem) != cudaSuccess)
+            return B200OPT_ECUDA;
+        sort_fill_kernel<T, N><<<1 + (accumulate ? 0 : fill), 1024, kSortSmem, st>>>(
+            (int)tokens, vocab, bits, ids, wide, keys, order, (T *)dw, ws, vecs);
+    } else {
+        uint32_t *from_k = nullptr, *to_k = (uint32_t *)(work + w.at_keys2);
+        int *from_o = nullptr, *to_o = (int *)(work + w.at_order2), *counts = (int *)(work + w.at_counts);
+        const int passes = (bits + 8) / 9, step = (bits + passes - 1) / passes;
+        const unsigned blocks = (unsigned)w.blocks;
+        if(passes & 1)  // the last pass ends in keys, order
+            std::swap(keys, to_k), std::swap(order, to_o);
+        for(int p = 0; p < passes; p++) {
+            const uint32_t mask = (1u << step) - 1;
+            sort_count_kernel<<<blocks, kManyThreads, 0, st>>>(tokens, vocab, ids, wide, from_k, from_o,
+                                                               p * step, mask, counts, (int)blocks);
+            sort_sums_kernel<<<1, 1024, 0, st>>>(counts, (int)blocks * kDigits);
+            sort_move_kernel<<<blocks, kManyThreads, 0, st>>>(tokens, vocab, ids, wide, from_k, from_o,
+                                                              p * step, mask, counts, (int)blocks, to_k,
+                                                              to_o);
+            from_k = to_k, from_o = to_o;
+            std::swap(keys, to_k), std::swap(order, to_o);
+        }
+        keys = from_k, order = from_o;
+        if(!accumulate)
+            fill_kernel<T, N><<<fill, 1024, 0, st>>>(tokens, vocab, keys, (T *)dw, ws, vecs);
+    }
+    if(tokens) {
+        const int lanes = lanes_of(vecs, 1);
+        const size_t chunks = (tokens + kChunk - 1) / kChunk, per = 256 / lanes;
+        const dim3 grid((unsigned)((chunks + per - 1) / per), (unsigned)((vecs + lanes - 1) / lanes));
+        float *parts = (float *)(work + w.at_parts);
+        sum_kernel<T, N><<<grid, 256, 0, st>>>(tokens, vocab, vecs, lanes, keys, order, (const T *)dy, ys,
+                                               scale, (T *)dw, ws, accumulate, parts);
+        if(chunks > 1)
+            join_rows_kernel<T, N><<<grid, 256, 0, st>>>(tokens, vocab, vecs, lanes, keys, scale, (T *)dw,
+                                                         ws, accumulate, parts);
+    }
+    return lm_launched();
 }
 
 }  // namespace
@@ -57,14 +649,11 @@ int b200opt_embedding_fwd(int dtype, size_t tokens, size_t vocab, size_t dim, co
     if(!ids || !lm_aligned(ids, index_bytes) ||
        !lm_matrix(weight, vocab, dim, weight_stride, e) || !lm_matrix(out, tokens, dim, out_stride, e))
         return B200OPT_EINVAL;
-    cudaStream_t st = (cudaStream_t)stream;
-    if(dtype == B200OPT_HALF)
-        embedding_fwd_kernel<<<(unsigned)tokens, 256, 0, st>>>(vocab, dim, ids, index_bytes == 8, (const __half *)weight,
-                                                     weight_stride, scale, (__half *)out, out_stride);
-    else
-        embedding_fwd_kernel<<<(unsigned)tokens, 256, 0, st>>>(vocab, dim, ids, index_bytes == 8, (const float *)weight,
-                                                     weight_stride, scale, (float *)out, out_stride);
-    return lm_launched();
+    const bool v = vectors(weight, weight_stride, e, dim) && vectors(out, out_stride, e, dim);
+    auto *f = dtype == B200OPT_HALF ? (v ? lookup<__half, 8> : lookup<__half, 1>)
+                                    : (v ? lookup<float, 4> : lookup<float, 1>);
+    return f(tokens, vocab, dim, ids, index_bytes == 8, weight, weight_stride, scale, out, out_stride,
+             (cudaStream_t)stream);
 }
 
 int b200opt_embedding_bwd_workspace(size_t tokens, size_t vocab, size_t dim, size_t *bytes)
@@ -73,7 +662,7 @@ int b200opt_embedding_bwd_workspace(size_t tokens, size_t vocab, size_t dim, siz
         return B200OPT_EINVAL;
     if(tokens > B200OPT_LM_MAX || vocab > B200OPT_LM_MAX || dim > B200OPT_LM_MAX)
         return B200OPT_ETOOBIG;
-    *bytes = 0;
+    *bytes = Work(tokens, dim).bytes;
     return B200OPT_OK;
 }
 
@@ -88,7 +677,7 @@ int b200opt_embedding_bwd(int dtype, size_t tokens, size_t vocab, size_t dim, co
     const int rc = b200opt_embedding_bwd_workspace(tokens, vocab, dim, &need);
     if(rc)
         return rc;
-    if(!vocab || !dim)
+    if(!vocab || !dim || (!tokens && accumulate))
         return B200OPT_OK;
     const size_t e = lm_size(dtype);
     if((tokens && (!ids || !lm_aligned(ids, index_bytes))) ||
@@ -96,15 +685,12 @@ int b200opt_embedding_bwd(int dtype, size_t tokens, size_t vocab, size_t dim, co
        !lm_matrix(grad_weight, vocab, dim, grad_weight_stride, e) ||
        workspace_bytes < need || (need && (!workspace || !lm_aligned(workspace, 256))))
         return B200OPT_EINVAL;
-    cudaStream_t st = (cudaStream_t)stream;
-    const dim3 grid((unsigned)vocab, (unsigned)((dim + 255) / 256));
-    if(dtype == B200OPT_HALF)
-        embedding_bwd_kernel<<<grid, 256, 0, st>>>(tokens, vocab, dim, ids, index_bytes == 8, (const __half *)grad_out,
-            grad_out_stride, scale, (__half *)grad_weight, grad_weight_stride, accumulate);
-    else
-        embedding_bwd_kernel<<<grid, 256, 0, st>>>(tokens, vocab, dim, ids, index_bytes == 8, (const float *)grad_out,
-            grad_out_stride, scale, (float *)grad_weight, grad_weight_stride, accumulate);
-    return lm_launched();
+    const bool v = vectors(grad_out, grad_out_stride, e, dim) &&
+                   vectors(grad_weight, grad_weight_stride, e, dim);
+    auto *f = dtype == B200OPT_HALF ? (v ? gradient<__half, 8> : gradient<__half, 1>)
+                                    : (v ? gradient<float, 4> : gradient<float, 1>);
+    return f(tokens, vocab, dim, ids, index_bytes == 8, grad_out, grad_out_stride, scale, grad_weight,
+             grad_weight_stride, accumulate, (char *)workspace, (cudaStream_t)stream);
 }
 
 }  // extern "C"
