@@ -39,7 +39,7 @@ def build_library(force=False, verbose=False):
     if not force and not _stale():
         return LIB
     cmd = [
-        _nvcc(), "-std=c++17", "-O3", "-lineinfo",
+        _nvcc(), "-std=c++17", "-O3", "-lineinfo", "--threads", "0",
         "-gencode", "arch=compute_100a,code=sm_100a",
         "-Xcompiler", "-fPIC,-Wall,-fvisibility=hidden",
         "-Xptxas", "-v" if verbose else "-O3",

@@ -10,44 +10,6 @@
 namespace b200 {
 namespace {
 
-// ---------------------------------------------------------- vectors of a row
-
-// N elements of T, moved as one word
-template <typename T, int N>
-struct Vec;
-template <>
-struct Vec<__half, 8> {
-    uint4 w;
-    __device__ __forceinline__ void get(float (&f)[8]) const
-    {
-        const __half2 *h = reinterpret_cast<const __half2 *>(&w);
-#pragma unroll
-        for(int i = 0; i < 4; i++) {
-            const float2 v = __half22float2(h[i]);
-            f[2 * i] = v.x, f[2 * i + 1] = v.y;
-        }
-    }
-    __device__ __forceinline__ void set(const float (&f)[8])
-    {
-        __half2 *h = reinterpret_cast<__half2 *>(&w);
-#pragma unroll
-        for(int i = 0; i < 4; i++)
-            h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
-    }
-};
-template <>
-struct Vec<float, 4> {
-    float4 w;
-    __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w; }
-    __device__ __forceinline__ void set(const float (&f)[4]) { w = make_float4(f[0], f[1], f[2], f[3]); }
-};
-template <typename T>
-struct Vec<T, 1> {
-    T w;
-    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = lm_load(&w); }
-    __device__ __forceinline__ void set(const float (&f)[1]) { lm_store(&w, f[0]); }
-};
-
 // ------------------------------------------------------------------- lookup
 
 // `lanes` threads (a power of two) share a row, four vectors each where the row
@@ -531,11 +493,6 @@ int lanes_of(size_t vecs, size_t each)
     return lanes;
 }
 
-bool vectors(const void *p, size_t stride, size_t elem, size_t dim)
-{
-    return lm_aligned(p, 16) && stride * elem % 16 == 0 && dim * elem % 16 == 0;
-}
-
 template <typename T, int N>
 int lookup(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide, const void *weight,
            size_t ws, float scale, void *out, size_t os, cudaStream_t st)
@@ -649,7 +606,7 @@ int b200opt_embedding_fwd(int dtype, size_t tokens, size_t vocab, size_t dim, co
     if(!ids || !lm_aligned(ids, index_bytes) ||
        !lm_matrix(weight, vocab, dim, weight_stride, e) || !lm_matrix(out, tokens, dim, out_stride, e))
         return B200OPT_EINVAL;
-    const bool v = vectors(weight, weight_stride, e, dim) && vectors(out, out_stride, e, dim);
+    const bool v = lm_vectors(weight, weight_stride, e, dim) && lm_vectors(out, out_stride, e, dim);
     auto *f = dtype == B200OPT_HALF ? (v ? lookup<__half, 8> : lookup<__half, 1>)
                                     : (v ? lookup<float, 4> : lookup<float, 1>);
     return f(tokens, vocab, dim, ids, index_bytes == 8, weight, weight_stride, scale, out, out_stride,
@@ -685,8 +642,8 @@ int b200opt_embedding_bwd(int dtype, size_t tokens, size_t vocab, size_t dim, co
        !lm_matrix(grad_weight, vocab, dim, grad_weight_stride, e) ||
        workspace_bytes < need || (need && (!workspace || !lm_aligned(workspace, 256))))
         return B200OPT_EINVAL;
-    const bool v = vectors(grad_out, grad_out_stride, e, dim) &&
-                   vectors(grad_weight, grad_weight_stride, e, dim);
+    const bool v = lm_vectors(grad_out, grad_out_stride, e, dim) &&
+                   lm_vectors(grad_weight, grad_weight_stride, e, dim);
     auto *f = dtype == B200OPT_HALF ? (v ? gradient<__half, 8> : gradient<__half, 1>)
                                     : (v ? gradient<float, 4> : gradient<float, 1>);
     return f(tokens, vocab, dim, ids, index_bytes == 8, grad_out, grad_out_stride, scale, grad_weight,

@@ -1,31 +1,142 @@
 // Layer norm and its gradient (b200opt_layernorm_* of include/b200opt.h).
+#include <algorithm>
+#include <type_traits>
+
 #include "lm_common.cuh"
 
 namespace b200 {
 namespace {
 
+constexpr int kThreads = 256;
+constexpr int kMaxParts = 444;  // blocks of the gradient kernel: three on each of 148 SMs
+
+// Sums over the threads that share a row: a warp, or the block.  `turn` alternates
+// between two sets of slots, so that one barrier a sum is enough.
+template <int WARPS, int K>
+__device__ __forceinline__ void row_sums(float (&v)[K], float (*slots)[8][K], int &turn)
+{
+#pragma unroll
+    for(int k = 0; k < K; k++)
+        v[k] = warp_sum(v[k]);
+    if(WARPS == 1)
+        return;
+    const int warp = threadIdx.x >> 5;
+    if((threadIdx.x & 31) == 0)
+        for(int k = 0; k < K; k++)
+            slots[turn][warp][k] = v[k];
+    __syncthreads();
+#pragma unroll
+    for(int k = 0; k < K; k++) {
+        v[k] = 0.0f;
+#pragma unroll
+        for(int w = 0; w < WARPS; w++)
+            v[k] += slots[turn][w][k];
+    }
+    turn ^= 1;
+}
+
+template <typename P, int N>
+__device__ __forceinline__ void load_param(const P *p, size_t c, float fill, float (&f)[N])
+{
+    if(p) {
+        reinterpret_cast<const Vec<P, N> *>(p)[c].get(f);
+    } else {
+#pragma unroll
+        for(int i = 0; i < N; i++)
+            f[i] = fill;
+    }
+}
+
+// A row stays in the registers of a warp (WARPS 1) or of the block (WARPS 8), NV
+// vectors of N elements a thread: it is read once, and the variance is taken
+// around the mean in a second pass over the registers.
+template <typename T, typename P, int N, int NV, int WARPS>
+__global__ void __launch_bounds__(kThreads)
+    layernorm_fwd_kernel(size_t rows, size_t dim, const T *x, size_t xs, const P *gamma, const P *beta,
+                         float eps, T *y, size_t ys, float *mean, float *rstd)
+{
+    __shared__ float slots[2][8][1];
+    int turn = 0;
+    constexpr int L = 32 * WARPS;
+    const size_t r = (size_t)blockIdx.x * (8 / WARPS) + threadIdx.x / L;
+    const int l = threadIdx.x % L, vecs = (int)(dim / N);
+    if(WARPS == 1 && r >= rows)
+        return;
+    const Vec<T, N> *from = reinterpret_cast<const Vec<T, N> *>(x + r * xs);
+    Vec<T, N> v[NV];
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+        if(l + i * L < vecs)
+            v[i] = from[l + i * L];
+    float s[1] = {0.0f};
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+        if(l + i * L < vecs) {
+            float f[N];
+            v[i].get(f);
+#pragma unroll
+            for(int j = 0; j < N; j++)
+                s[0] += f[j];
+        }
+    row_sums<WARPS, 1>(s, slots, turn);
+    const float mu = s[0] / (float)dim;
+    s[0] = 0.0f;
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+        if(l + i * L < vecs) {
+            float f[N];
+            v[i].get(f);
+#pragma unroll
+            for(int j = 0; j < N; j++)
+                s[0] += (f[j] - mu) * (f[j] - mu);
+        }
+    row_sums<WARPS, 1>(s, slots, turn);
+    const float rs = 1.0f / sqrtf(s[0] / (float)dim + eps);
+    Vec<T, N> *to = reinterpret_cast<Vec<T, N> *>(y + r * ys);
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+        if(l + i * L < vecs) {
+            float f[N], g[N], b[N];
+            v[i].get(f);
+            load_param<P, N>(gamma, l + i * L, 1.0f, g);
+            load_param<P, N>(beta, l + i * L, 0.0f, b);
+#pragma unroll
+            for(int j = 0; j < N; j++)
+                f[j] = fmaf((f[j] - mu) * rs, g[j], b[j]);
+            v[i].set(f);
+            to[l + i * L] = v[i];
+        }
+    if(l == 0) {
+        if(mean)
+            mean[r] = mu;
+        if(rstd)
+            rstd[r] = rs;
+    }
+}
+
+// Rows too long for the registers: three passes over memory.
 template <typename T, typename P>
-__global__ void layernorm_fwd_kernel(size_t dim, const T *x, size_t xs, const P *gamma,
-                                     const P *beta, float eps, T *y, size_t ys, float *mean,
-                                     float *rstd)
+__global__ void __launch_bounds__(1024)
+    layernorm_fwd_long_kernel(size_t dim, const T *x, size_t xs, const P *gamma, const P *beta,
+                              float eps, T *y, size_t ys, float *mean, float *rstd)
 {
     __shared__ float red[32];
     const size_t r = blockIdx.x;
     x += r * xs;
     y += r * ys;
     float s = 0.0f;
-    for(size_t d = threadIdx.x; d < dim; d += blockDim.x)
+    for(size_t d = threadIdx.x; d < dim; d += 1024)
         s += lm_load(x + d);
     const float mu = block_sum(s, red) / (float)dim;
     s = 0.0f;
-    for(size_t d = threadIdx.x; d < dim; d += blockDim.x) {
+    for(size_t d = threadIdx.x; d < dim; d += 1024) {
         const float c = lm_load(x + d) - mu;
         s += c * c;
     }
     const float rs = 1.0f / sqrtf(block_sum(s, red) / (float)dim + eps);
-    for(size_t d = threadIdx.x; d < dim; d += blockDim.x)
-        lm_store(y + d, (lm_load(x + d) - mu) * rs * (gamma ? lm_load(gamma + d) : 1.0f) +
-                            (beta ? lm_load(beta + d) : 0.0f));
+    for(size_t d = threadIdx.x; d < dim; d += 1024)
+        lm_store(y + d, fmaf((lm_load(x + d) - mu) * rs, gamma ? lm_load(gamma + d) : 1.0f,
+                             beta ? lm_load(beta + d) : 0.0f));
     if(threadIdx.x == 0) {
         if(mean)
             mean[r] = mu;
@@ -34,69 +145,316 @@ __global__ void layernorm_fwd_kernel(size_t dim, const T *x, size_t xs, const P 
     }
 }
 
+// The gradient in one pass over x and grad_y.  A block walks over rows; each
+// thread keeps the parameters' sums of its own columns in registers and leaves
+// them in `parts` at the end, for params_kernel to join in a fixed order.  The
+// next row's vectors are loaded before the present row's sums are waited for.
+template <typename T, typename P, int N, int NV, int WARPS>
+__global__ void __launch_bounds__(kThreads)
+    layernorm_bwd_kernel(size_t rows, size_t dim, const T *dy, size_t ys, const T *x, size_t xs,
+                         const P *gamma, const float *mean, const float *rstd, T *dx, size_t dxs,
+                         float *parts)
+{
+    __shared__ float slots[2][8][2];
+    __shared__ float joined[WARPS == 1 ? 2 * 32 * NV * N : 1];
+    int turn = 0;
+    constexpr int L = 32 * WARPS, R = 8 / WARPS;
+    const int l = threadIdx.x % L, vecs = (int)(dim / N);
+    const size_t step = (size_t)gridDim.x * R;
+    float sg[NV][N], sb[NV][N];
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+#pragma unroll
+        for(int j = 0; j < N; j++)
+            sg[i][j] = sb[i][j] = 0.0f;
+
+    size_t r = (size_t)blockIdx.x * R + threadIdx.x / L;
+    Vec<T, N> vx[NV], vy[NV];
+    float mu = 0.0f, rs = 0.0f;
+    auto fetch = [&](size_t row, Vec<T, N> (&a)[NV], Vec<T, N> (&b)[NV], float &m, float &q) {
+        if(row >= rows)
+            return;
+        m = mean[row];
+        q = rstd[row];
+        const Vec<T, N> *px = reinterpret_cast<const Vec<T, N> *>(x + row * xs);
+        const Vec<T, N> *py = reinterpret_cast<const Vec<T, N> *>(dy + row * ys);
+#pragma unroll
+        for(int i = 0; i < NV; i++)
+            if(l + i * L < vecs) {
+                a[i] = px[l + i * L];
+                b[i] = py[l + i * L];
+            }
+    };
+    fetch(r, vx, vy, mu, rs);
+    // the rows of a block are consecutive steps, so with WARPS 8 all threads agree
+    for(; r < rows; r += step) {
+        Vec<T, N> nx[NV], ny[NV];
+        float nmu = 0.0f, nrs = 0.0f;
+        fetch(r + step, nx, ny, nmu, nrs);
+        float s[2] = {0.0f, 0.0f};
+#pragma unroll
+        for(int i = 0; i < NV; i++)
+            if(l + i * L < vecs) {
+                float fx[N], fy[N], g[N];
+                vx[i].get(fx);
+                vy[i].get(fy);
+                load_param<P, N>(gamma, l + i * L, 1.0f, g);
+#pragma unroll
+                for(int j = 0; j < N; j++) {
+                    const float xh = (fx[j] - mu) * rs, d = fy[j] * g[j];
+                    sg[i][j] = fmaf(fy[j], xh, sg[i][j]);
+                    sb[i][j] += fy[j];
+                    s[0] += d;
+                    s[1] = fmaf(d, xh, s[1]);
+                }
+            }
+        if(dx) {
+            row_sums<WARPS, 2>(s, slots, turn);
+            const float a = s[0] / (float)dim, b = s[1] / (float)dim;
+            Vec<T, N> *to = reinterpret_cast<Vec<T, N> *>(dx + r * dxs);
+#pragma unroll
+            for(int i = 0; i < NV; i++)
+                if(l + i * L < vecs) {
+                    float fx[N], fy[N], g[N];
+                    vx[i].get(fx);
+                    vy[i].get(fy);
+                    load_param<P, N>(gamma, l + i * L, 1.0f, g);
+#pragma unroll
+                    for(int j = 0; j < N; j++) {
+                        const float xh = (fx[j] - mu) * rs;
+                        fx[j] = rs * (fmaf(fy[j], g[j], -a) - xh * b);
+                    }
+                    Vec<T, N> o;
+                    o.set(fx);
+                    to[l + i * L] = o;
+                }
+        }
+#pragma unroll
+        for(int i = 0; i < NV; i++) {
+            vx[i] = nx[i];
+            vy[i] = ny[i];
+        }
+        mu = nmu;
+        rs = nrs;
+    }
+    if(!parts)
+        return;
+    float *pg = parts + (size_t)blockIdx.x * 2 * dim, *pb = pg + dim;
+    if(WARPS == 1) {  // the block's warps have the same columns: joined one after the other
+        for(int w = 0; w < 8; w++) {
+            if(threadIdx.x / 32 == w)
+#pragma unroll
+                for(int i = 0; i < NV; i++)
+                    if(l + i * L < vecs)
+#pragma unroll
+                        for(int j = 0; j < N; j++) {
+                            float *g = joined + (i * L + l) * N + j, *b = g + 32 * NV * N;
+                            *g = w ? *g + sg[i][j] : sg[i][j];
+                            *b = w ? *b + sb[i][j] : sb[i][j];
+                        }
+            __syncthreads();
+        }
+        for(int d = threadIdx.x; d < (int)dim; d += kThreads) {
+            pg[d] = joined[d];
+            pb[d] = joined[32 * NV * N + d];
+        }
+        return;
+    }
+#pragma unroll
+    for(int i = 0; i < NV; i++)
+        if(l + i * L < vecs)
+#pragma unroll
+            for(int j = 0; j < N; j++) {
+                pg[(l + i * L) * N + j] = sg[i][j];
+                pb[(l + i * L) * N + j] = sb[i][j];
+            }
+}
+
+// Joins the blocks' sums: 32 columns and 8 stretches of blocks a block.
+template <typename P>
+__global__ void __launch_bounds__(256)
+    params_kernel(size_t dim, int blocks, const float *parts, P *dgamma, P *dbeta, int accumulate)
+{
+    __shared__ float red[8][33];
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const size_t d = (size_t)blockIdx.x * 32 + lane;
+    P *to = blockIdx.y ? dbeta : dgamma;
+    if(!to)
+        return;
+    float s = 0.0f;
+    if(d < dim)
+#pragma unroll 8
+        for(int b = w; b < blocks; b += 8)
+            s += parts[((size_t)b * 2 + blockIdx.y) * dim + d];
+    red[w][lane] = s;
+    __syncthreads();
+    if(w || d >= dim)
+        return;
+    for(int i = 1; i < 8; i++)
+        s += red[i][lane];
+    lm_store(to + d, accumulate ? s + lm_load(to + d) : s);
+}
+
+// Rows too long for that: grad_x row by row, the parameters' sums column by column.
 template <typename T, typename P>
-__global__ void layernorm_bwd_x_kernel(size_t dim, const T *dy, size_t ys, const T *x, size_t xs,
-                                       const P *gamma, const float *mean, const float *rstd, T *dx,
-                                       size_t dxs)
+__global__ void __launch_bounds__(1024)
+    layernorm_bwd_long_kernel(size_t dim, const T *dy, size_t ys, const T *x, size_t xs,
+                              const P *gamma, const float *mean, const float *rstd, T *dx, size_t dxs)
 {
     __shared__ float red[32];
     const size_t r = blockIdx.x;
     const float mu = mean[r], rs = rstd[r];
     float a = 0.0f, b = 0.0f;
-    for(size_t d = threadIdx.x; d < dim; d += blockDim.x) {
+    for(size_t d = threadIdx.x; d < dim; d += 1024) {
         const float g = lm_load(dy + r * ys + d) * (gamma ? lm_load(gamma + d) : 1.0f);
         a += g;
         b += g * ((lm_load(x + r * xs + d) - mu) * rs);
     }
     a = block_sum(a, red) / (float)dim;
     b = block_sum(b, red) / (float)dim;
-    for(size_t d = threadIdx.x; d < dim; d += blockDim.x) {
+    for(size_t d = threadIdx.x; d < dim; d += 1024) {
         const float g = lm_load(dy + r * ys + d) * (gamma ? lm_load(gamma + d) : 1.0f);
         lm_store(dx + r * dxs + d, rs * (g - a - (lm_load(x + r * xs + d) - mu) * rs * b));
     }
 }
 
 template <typename T, typename P>
-__global__ void layernorm_bwd_params_kernel(size_t rows, size_t dim, const T *dy, size_t ys,
-                                            const T *x, size_t xs, const float *mean,
-                                            const float *rstd, P *dgamma, P *dbeta, int accumulate)
+__global__ void __launch_bounds__(128)
+    layernorm_params_long_kernel(size_t rows, size_t dim, const T *dy, size_t ys, const T *x, size_t xs,
+                                 const float *mean, const float *rstd, float *parts)
 {
-    const size_t d = (size_t)blockIdx.x * blockDim.x + threadIdx.x;
+    // blockIdx.y: a stretch of the rows
+    const size_t d = (size_t)blockIdx.x * 128 + threadIdx.x;
     if(d >= dim)
         return;
+    const size_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
     float g = 0.0f, b = 0.0f;
-    for(size_t r = 0; r < rows; r++) {
+#pragma unroll 4
+    for(size_t r = r0; r < r1; r++) {
         const float v = lm_load(dy + r * ys + d);
         g += v * ((lm_load(x + r * xs + d) - mean[r]) * rstd[r]);
         b += v;
     }
-    if(dgamma)
-        lm_store(dgamma + d, g + (accumulate ? lm_load(dgamma + d) : 0.0f));
-    if(dbeta)
-        lm_store(dbeta + d, b + (accumulate ? lm_load(dbeta + d) : 0.0f));
+    parts[(size_t)blockIdx.y * 2 * dim + d] = g;
+    parts[((size_t)blockIdx.y * 2 + 1) * dim + d] = b;
 }
 
-template <typename T, typename P>
-int fwd(size_t rows, size_t dim, const void *x, size_t xs, const void *gamma, const void *beta,
-        float eps, void *y, size_t ys, float *mean, float *rstd, cudaStream_t st)
+// ---------------------------------------------------------------- host side
+
+struct Args {
+    size_t rows, dim, xs, ys, dxs;
+    const void *x, *dy, *gamma, *beta;
+    float eps;
+    void *y, *dx, *dgamma, *dbeta;
+    float *mean, *rstd;
+    const float *mean_in, *rstd_in;
+    int accumulate;
+    float *parts;
+    cudaStream_t st;
+};
+
+// Vectors a thread holds: the smallest power of two up to MAX that covers a row
+// with a warp, else with the block; 0 threads' worth: the long kernels.
+template <int N, int NV, int MAX, typename F>
+bool pick(size_t vecs, F &&f)
 {
-    layernorm_fwd_kernel<<<(unsigned)rows, 256, 0, st>>>(dim, (const T *)x, xs, (const P *)gamma,
-                                               (const P *)beta, eps, (T *)y, ys, mean, rstd);
+    if(vecs <= (size_t)32 * NV) {
+        f(std::integral_constant<int, NV>(), std::integral_constant<int, 1>());
+        return true;
+    }
+    if constexpr(NV < MAX) {
+        return pick<N, 2 * NV, MAX>(vecs, f);
+    } else {
+        return false;
+    }
+}
+template <int N, int NV, int MAX, typename F>
+bool pick_block(size_t vecs, F &&f)
+{
+    if(vecs <= (size_t)256 * NV) {
+        f(std::integral_constant<int, NV>(), std::integral_constant<int, 8>());
+        return true;
+    }
+    if constexpr(NV < MAX) {
+        return pick_block<N, 2 * NV, MAX>(vecs, f);
+    } else {
+        return false;
+    }
+}
+
+template <typename T, typename P, int N>
+int fwd_with(const Args &a)
+{
+    auto launch = [&](auto nv, auto warps) {
+        constexpr int NV = decltype(nv)::value, W = decltype(warps)::value;
+        const size_t blocks = (a.rows + 8 / W - 1) / (8 / W);
+        layernorm_fwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, kThreads, 0, a.st>>>(
+            a.rows, a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y,
+            a.ys, a.mean, a.rstd);
+    };
+    const size_t vecs = a.dim / N;
+    if(!pick<N, 1, 16>(vecs, launch) && !pick_block<N, 4, 16>(vecs, launch))
+        layernorm_fwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
+            a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y, a.ys,
+            a.mean, a.rstd);
+    return lm_launched();
+}
+
+template <typename T, typename P, int N>
+int bwd_with(const Args &a)
+{
+    const bool want = a.dgamma || a.dbeta;
+    float *parts = want ? a.parts : nullptr;
+    size_t blocks = 0;
+    auto launch = [&](auto nv, auto warps) {
+        constexpr int NV = decltype(nv)::value, W = decltype(warps)::value;
+        blocks = std::min<size_t>((a.rows + 8 / W - 1) / (8 / W), kMaxParts);
+        if(blocks)
+            layernorm_bwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, kThreads, 0, a.st>>>(
+                a.rows, a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma,
+                a.mean_in, a.rstd_in, (T *)a.dx, a.dxs, parts);
+    };
+    const size_t vecs = a.dim / N;
+    constexpr int kWarp = N == 1 ? 16 : 16 / N * 2, kBlock = 32 / N;
+    if(!pick<N, 1, kWarp>(vecs, launch) && !pick_block<N, kWarp / 4, kBlock>(vecs, launch)) {
+        if(a.dx && a.rows)
+            layernorm_bwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
+                a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma, a.mean_in,
+                a.rstd_in, (T *)a.dx, a.dxs);
+        blocks = std::min<size_t>((a.rows + 63) / 64, kMaxParts);
+        if(want && blocks)
+            layernorm_params_long_kernel<T, P>
+                <<<dim3((unsigned)((a.dim + 127) / 128), (unsigned)blocks), 128, 0, a.st>>>(
+                    a.rows, a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, a.mean_in, a.rstd_in,
+                    parts);
+    }
+    if(want)
+        params_kernel<P><<<dim3((unsigned)((a.dim + 31) / 32), 2), 256, 0, a.st>>>(
+            a.dim, (int)blocks, parts, (P *)a.dgamma, (P *)a.dbeta, a.accumulate);
     return lm_launched();
 }
 
 template <typename T, typename P>
-int bwd(size_t rows, size_t dim, const void *dy, size_t ys, const void *x, size_t xs,
-        const void *gamma, const float *mean, const float *rstd, void *dx, size_t dxs, void *dgamma,
-        void *dbeta, int accumulate, cudaStream_t st)
+int fwd(const Args &a)
 {
-    if(dx && rows)
-        layernorm_bwd_x_kernel<<<(unsigned)rows, 256, 0, st>>>(dim, (const T *)dy, ys, (const T *)x, xs,
-                                                     (const P *)gamma, mean, rstd, (T *)dx, dxs);
-    if(dgamma || dbeta)
-        layernorm_bwd_params_kernel<<<(unsigned)((dim + 255) / 256), 256, 0, st>>>(
-            rows, dim, (const T *)dy, ys, (const T *)x, xs, mean, rstd, (P *)dgamma, (P *)dbeta, accumulate);
-    return lm_launched();
+    constexpr int N = 16 / sizeof(T);
+    const bool v = lm_vectors(a.x, a.xs, sizeof(T), a.dim) && lm_vectors(a.y, a.ys, sizeof(T), a.dim) &&
+                   lm_aligned(a.gamma, 16) && lm_aligned(a.beta, 16);
+    return v ? fwd_with<T, P, N>(a) : fwd_with<T, P, 1>(a);
+}
+
+template <typename T, typename P>
+int bwd(const Args &a)
+{
+    constexpr int N = 16 / sizeof(T);
+    const bool v = lm_vectors(a.x, a.xs, sizeof(T), a.dim) && lm_vectors(a.dy, a.ys, sizeof(T), a.dim) &&
+                   (!a.dx || lm_vectors(a.dx, a.dxs, sizeof(T), a.dim)) && lm_aligned(a.gamma, 16);
+    return v ? bwd_with<T, P, N>(a) : bwd_with<T, P, 1>(a);
+}
+
+size_t bwd_bytes(size_t rows, size_t dim)
+{
+    return std::min<size_t>(rows, kMaxParts) * 2 * dim * 4;
 }
 
 }  // namespace
@@ -121,12 +479,12 @@ int b200opt_layernorm_fwd(int dtype, int param_dtype, size_t rows, size_t dim, c
     if(!lm_matrix(x, rows, dim, x_stride, e) || !lm_matrix(y, rows, dim, y_stride, e) ||
        !lm_aligned(gamma, p) || !lm_aligned(beta, p) || !lm_aligned(mean, 4) || !lm_aligned(rstd, 4))
         return B200OPT_EINVAL;
-    cudaStream_t st = (cudaStream_t)stream;
-    if(dtype == B200OPT_FLOAT)
-        return fwd<float, float>(rows, dim, x, x_stride, gamma, beta, eps, y, y_stride, mean, rstd, st);
-    if(param_dtype == B200OPT_FLOAT)
-        return fwd<__half, float>(rows, dim, x, x_stride, gamma, beta, eps, y, y_stride, mean, rstd, st);
-    return fwd<__half, __half>(rows, dim, x, x_stride, gamma, beta, eps, y, y_stride, mean, rstd, st);
+    Args a = {};
+    a.rows = rows, a.dim = dim, a.x = x, a.xs = x_stride, a.gamma = gamma, a.beta = beta, a.eps = eps;
+    a.y = y, a.ys = y_stride, a.mean = mean, a.rstd = rstd, a.st = (cudaStream_t)stream;
+    return dtype == B200OPT_FLOAT         ? fwd<float, float>(a)
+           : param_dtype == B200OPT_FLOAT ? fwd<__half, float>(a)
+                                          : fwd<__half, __half>(a);
 }
 
 int b200opt_layernorm_bwd_workspace(size_t rows, size_t dim, size_t *bytes)
@@ -135,7 +493,7 @@ int b200opt_layernorm_bwd_workspace(size_t rows, size_t dim, size_t *bytes)
         return B200OPT_EINVAL;
     if(rows > B200OPT_LM_MAX || dim > B200OPT_LM_MAX)
         return B200OPT_ETOOBIG;
-    *bytes = 0;
+    *bytes = bwd_bytes(rows, dim);
     return B200OPT_OK;
 }
 
@@ -161,15 +519,16 @@ int b200opt_layernorm_bwd(int dtype, int param_dtype, size_t rows, size_t dim, c
        !lm_aligned(grad_gamma, p) || !lm_aligned(grad_beta, p) || workspace_bytes < need ||
        (need && (!workspace || !lm_aligned(workspace, 256))))
         return B200OPT_EINVAL;
-    cudaStream_t st = (cudaStream_t)stream;
-    if(dtype == B200OPT_FLOAT)
-        return bwd<float, float>(rows, dim, grad_y, grad_y_stride, x, x_stride, gamma, mean, rstd,
-                                 grad_x, grad_x_stride, grad_gamma, grad_beta, accumulate, st);
-    if(param_dtype == B200OPT_FLOAT)
-        return bwd<__half, float>(rows, dim, grad_y, grad_y_stride, x, x_stride, gamma, mean, rstd,
-                                  grad_x, grad_x_stride, grad_gamma, grad_beta, accumulate, st);
-    return bwd<__half, __half>(rows, dim, grad_y, grad_y_stride, x, x_stride, gamma, mean, rstd,
-                               grad_x, grad_x_stride, grad_gamma, grad_beta, accumulate, st);
+    Args a = {};
+    a.rows = rows, a.dim = dim, a.x = x, a.xs = x_stride, a.gamma = gamma;
+    a.dy = grad_y, a.ys = grad_y_stride, a.mean_in = mean, a.rstd_in = rstd;
+    a.dx = grad_x, a.dxs = grad_x_stride, a.dgamma = grad_gamma, a.dbeta = grad_beta;
+    a.accumulate = accumulate, a.parts = (float *)workspace, a.st = (cudaStream_t)stream;
+    if(!grad_x && !grad_gamma && !grad_beta)
+        return B200OPT_OK;
+    return dtype == B200OPT_FLOAT         ? bwd<float, float>(a)
+           : param_dtype == B200OPT_FLOAT ? bwd<__half, float>(a)
+                                          : bwd<__half, __half>(a);
 }
 
 }  // extern "C"

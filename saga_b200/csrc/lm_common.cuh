@@ -49,6 +49,58 @@ __device__ __forceinline__ float lm_load(const float *p) { return *p; }
 __device__ __forceinline__ void lm_store(__half *p, float v) { *p = __float2half_rn(v); }
 __device__ __forceinline__ void lm_store(float *p, float v) { *p = v; }
 
+// ---------------------------------------------------------- vectors of a row
+
+// N elements of T, moved as one word
+template <typename T, int N>
+struct Vec;
+template <>
+struct Vec<__half, 8> {
+    uint4 w;
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+        const __half2 *h = reinterpret_cast<const __half2 *>(&w);
+#pragma unroll
+        for(int i = 0; i < 4; i++) {
+            const float2 v = __half22float2(h[i]);
+            f[2 * i] = v.x, f[2 * i + 1] = v.y;
+        }
+    }
+    __device__ __forceinline__ void set(const float (&f)[8])
+    {
+        __half2 *h = reinterpret_cast<__half2 *>(&w);
+#pragma unroll
+        for(int i = 0; i < 4; i++)
+            h[i] = __floats2half2_rn(f[2 * i], f[2 * i + 1]);
+    }
+};
+template <>
+struct Vec<float, 4> {
+    float4 w;
+    __device__ __forceinline__ void get(float (&f)[4]) const { f[0] = w.x, f[1] = w.y, f[2] = w.z, f[3] = w.w; }
+    __device__ __forceinline__ void set(const float (&f)[4]) { w = make_float4(f[0], f[1], f[2], f[3]); }
+};
+template <>
+struct Vec<float, 8> {
+    float4 a, b;
+    __device__ __forceinline__ void get(float (&f)[8]) const
+    {
+        f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
+    }
+};
+template <typename T>
+struct Vec<T, 1> {
+    T w;
+    __device__ __forceinline__ void get(float (&f)[1]) const { f[0] = lm_load(&w); }
+    __device__ __forceinline__ void set(const float (&f)[1]) { lm_store(&w, f[0]); }
+};
+
+// Whether a matrix can be moved in 16-byte vectors.
+inline bool lm_vectors(const void *p, size_t stride, size_t elem, size_t dim)
+{
+    return lm_aligned(p, 16) && stride * elem % 16 == 0 && dim * elem % 16 == 0;
+}
+
 // Element i of an index array, or -1 when it lies outside [0, vocab).
 __device__ __forceinline__ int lm_index_at(const void *ids, int wide, size_t i, size_t vocab)
 {

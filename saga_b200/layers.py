@@ -15,6 +15,7 @@ not pass (outputs, workspace) from torch's allocator, which is refused for a raw
 stream, because that allocator would not know of it.
 """
 import ctypes as C
+import functools
 import math
 
 import torch
@@ -23,41 +24,47 @@ from . import capi
 from .capi import check, lib
 
 _DTYPES = {torch.float16: capi.HALF, torch.float32: capi.FLOAT}
+_raw_stream = torch._C._cuda_getCurrentRawStream     # what current_stream().cuda_stream is, without the object
 
 
 def _dtype(t, what):
-    if t.dtype not in _DTYPES:
+    kind = _DTYPES.get(t.dtype)
+    if kind is None:
         raise TypeError(f"{what} is {t.dtype}: float16 or float32 expected")
-    return _DTYPES[t.dtype]
+    return kind
 
 
-def _on(device, what, t):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda" or t.device != device:
-        raise ValueError(f"{what} must be a CUDA tensor on {device}")
-    return t
-
-
-def _cuda(t, what):
-    if not isinstance(t, torch.Tensor) or t.device.type != "cuda":
+def _device(t, what):
+    """Index of the CUDA device that the tensor is on."""
+    index = t.get_device() if isinstance(t, torch.Tensor) else -1
+    if index < 0 or not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
-    return t.device
+    return index
+
+
+def _on(index, what, t):
+    if _device(t, what) != index:
+        raise ValueError(f"{what} must be on cuda:{index}")
 
 
 def _rows(t, what, cols=None, dtype=None):
     """(rows, row length, row stride) of a tensor seen as a matrix of its last dimension."""
-    if t.dim() < 1:
+    shape = t.shape
+    if not shape:
         raise ValueError(f"{what} needs at least one dimension")
-    if cols is not None and t.shape[-1] != cols:
-        raise ValueError(f"{what} has rows of {t.shape[-1]} elements, {cols} expected")
+    d = shape[-1]
+    if cols is not None and d != cols:
+        raise ValueError(f"{what} has rows of {d} elements, {cols} expected")
     if dtype is not None and t.dtype != dtype:
         raise TypeError(f"{what} is {t.dtype}, {dtype} expected")
-    n, d = math.prod(t.shape[:-1]), t.shape[-1]
-    if t.numel() == 0:
+    n = math.prod(shape[:-1])
+    if n == 0 or d == 0 or t.is_contiguous():
         return n, d, max(d, 1)
-    if d > 1 and t.stride(-1) != 1:
+    strides = t.stride()
+    if d > 1 and strides[-1] != 1:
         raise ValueError(f"{what} must be contiguous in its last dimension")
     stride, expect = d, None
-    for size, step in zip(reversed(t.shape[:-1]), reversed(t.stride()[:-1])):
+    for size, step in zip(reversed(shape[:-1]), reversed(strides[:-1])):
         if size == 1:
             continue
         if expect is None:
@@ -70,19 +77,19 @@ def _rows(t, what, cols=None, dtype=None):
     return n, d, max(stride, d)
 
 
-def _matrix(t, what, rows, cols, dtype, device):
+def _matrix(t, what, rows, cols, dtype, index):
     """Row stride of an output or gradient that must have the given shape."""
-    _on(device, what, t)
+    _on(index, what, t)
     n, _, stride = _rows(t, what, cols, dtype)
     if n != rows:
         raise ValueError(f"{what} has {n} rows, {rows} expected")
     return stride
 
 
-def _vector(t, what, n, dtype, device):
+def _vector(t, what, n, dtype, index):
     if t is None:
         return None
-    _on(device, what, t)
+    _on(index, what, t)
     if t.dtype != dtype:
         raise TypeError(f"{what} is {t.dtype}, {dtype} expected")
     if t.numel() != n or not t.is_contiguous():
@@ -90,171 +97,167 @@ def _vector(t, what, n, dtype, device):
     return t.data_ptr()
 
 
-def _index(t, what, device):
-    _on(device, what, t)
-    if t.dtype not in (torch.int32, torch.int64):
+def _index(t, what, index):
+    _on(index, what, t)
+    if t.dtype != torch.int64 and t.dtype != torch.int32:
         raise TypeError(f"{what} is {t.dtype}: int32 or int64 expected")
     if not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous")
     return t.data_ptr(), t.element_size()
 
 
-class _Call:
-    """Current device and stream of one call, and what it allocates."""
+def _new(like, shape, dtype, what, stream):
+    if stream is not None:
+        raise ValueError(f"pass {what} when a raw stream is given")
+    return like.new_empty(shape, dtype=dtype)
 
-    def __init__(self, device, stream):
-        self.device, self.raw = device, stream
-        self.guard = torch.cuda.device(device)
 
-    def __enter__(self):
-        self.guard.__enter__()
-        self.stream = (torch.cuda.current_stream(self.device).cuda_stream if self.raw is None
-                       else self.raw)
-        return self
+@functools.lru_cache(maxsize=1024)
+def _bytes(query, *sizes):
+    """What a _workspace function says: it depends on the sizes alone."""
+    need = C.c_size_t()
+    check(getattr(lib(), query)(*sizes, C.byref(need)))
+    return need.value
 
-    def __exit__(self, *exc):
-        return self.guard.__exit__(*exc)
 
-    def new(self, what, shape, dtype):
-        if self.raw is not None:
-            raise ValueError(f"pass {what} when a raw stream is given")
-        return torch.empty(shape, dtype=dtype, device=self.device)
-
-    def workspace(self, given, query, *sizes):
-        """(tensor, address, bytes) of the caller's workspace or of a new one."""
-        need = C.c_size_t()
-        check(getattr(lib(), query)(*sizes, C.byref(need)))
-        if given is None:
-            given = self.new("workspace", (need.value,), torch.uint8) if need.value else None
-        if given is None:
+def _workspace(given, need, like, index, stream):
+    """(tensor, address, bytes) of the caller's workspace or of a new one."""
+    if given is None:
+        if not need:
             return None, None, 0
-        _on(self.device, "workspace", given)
+        given = _new(like, (need,), torch.uint8, "workspace", stream)
+    else:
+        _on(index, "workspace", given)
         if not given.is_contiguous():
             raise ValueError("workspace must be contiguous")
-        return given, given.data_ptr(), given.numel() * given.element_size()
+    return given, given.data_ptr(), given.numel() * given.element_size()
+
+
+def _call(function, index, stream, *args):
+    """Runs a C entry with the tensors' device current, on the given or torch's current stream."""
+    if torch._C._cuda_getDevice() == index:
+        check(function(*args, _raw_stream(index) if stream is None else stream))
+    else:
+        with torch.cuda.device(index):
+            check(function(*args, _raw_stream(index) if stream is None else stream))
 
 
 def embedding_forward(ids, weight, scale=1.0, out=None, stream=None):
     """out[...] = scale * weight[ids[...]]; an id outside the table gives a row of zeros."""
-    device = _cuda(weight, "weight")
+    dev = _device(weight, "weight")
     vocab, dim, ws = _rows(weight, "weight")
     dtype = _dtype(weight, "weight")
-    ids_ptr, wide = _index(ids, "ids", device)
-    with _Call(device, stream) as call:
-        if out is None:
-            out = call.new("out", (*ids.shape, dim), weight.dtype)
-        os = _matrix(out, "out", ids.numel(), dim, weight.dtype, device)
-        check(lib().b200opt_embedding_fwd(dtype, ids.numel(), vocab, dim, ids_ptr, wide,
-                                          weight.data_ptr(), ws, scale, out.data_ptr(), os,
-                                          call.stream))
+    ids_ptr, wide = _index(ids, "ids", dev)
+    tokens = ids.numel()
+    if out is None:
+        out, os = _new(weight, (*ids.shape, dim), weight.dtype, "out", stream), max(dim, 1)
+    else:
+        os = _matrix(out, "out", tokens, dim, weight.dtype, dev)
+    _call(lib().b200opt_embedding_fwd, dev, stream, dtype, tokens, vocab, dim, ids_ptr, wide,
+          weight.data_ptr(), ws, scale, out.data_ptr(), os)
     return out
 
 
 def embedding_workspace(tokens, vocab, dim):
     """Bytes of workspace that embedding_backward needs."""
-    need = C.c_size_t()
-    check(lib().b200opt_embedding_bwd_workspace(tokens, vocab, dim, C.byref(need)))
-    return need.value
+    return _bytes("b200opt_embedding_bwd_workspace", tokens, vocab, dim)
 
 
 def embedding_backward(ids, grad_out, vocab, scale=1.0, grad_weight=None, accumulate=False,
                        workspace=None, stream=None):
     """The dense gradient [vocab, dim] of the table; rows that no id names become zero, or keep
     their values with ``accumulate`` (which needs ``grad_weight``)."""
-    device = _cuda(grad_out, "grad_out")
+    dev = _device(grad_out, "grad_out")
     tokens, dim, ys = _rows(grad_out, "grad_out")
     dtype = _dtype(grad_out, "grad_out")
-    ids_ptr, wide = _index(ids, "ids", device)
-    if ids.numel() != tokens and dim:
+    ids_ptr, wide = _index(ids, "ids", dev)
+    if ids.numel() != tokens:
         raise ValueError(f"{ids.numel()} ids, but {tokens} rows in grad_out")
-    if accumulate and grad_weight is None:
+    if grad_weight is not None:
+        gs = _matrix(grad_weight, "grad_weight", vocab, dim, grad_out.dtype, dev)
+    elif accumulate:
         raise ValueError("accumulate needs grad_weight")
-    with _Call(device, stream) as call:
-        if grad_weight is None:
-            grad_weight = call.new("grad_weight", (vocab, dim), grad_out.dtype)
-        gs = _matrix(grad_weight, "grad_weight", vocab, dim, grad_out.dtype, device)
-        keep, wp, wb = call.workspace(workspace, "b200opt_embedding_bwd_workspace", tokens, vocab,
-                                      dim)
-        check(lib().b200opt_embedding_bwd(dtype, tokens, vocab, dim, ids_ptr, wide,
-                                          grad_out.data_ptr(), ys, scale, grad_weight.data_ptr(),
-                                          gs, int(accumulate), wp, wb, call.stream))
+    else:
+        grad_weight = _new(grad_out, (vocab, dim), grad_out.dtype, "grad_weight", stream)
+        gs = max(dim, 1)
+    keep, wp, wb = _workspace(workspace, embedding_workspace(tokens, vocab, dim), grad_out, dev, stream)
+    _call(lib().b200opt_embedding_bwd, dev, stream, dtype, tokens, vocab, dim, ids_ptr, wide,
+          grad_out.data_ptr(), ys, scale, grad_weight.data_ptr(), gs, int(accumulate), wp, wb)
     return grad_weight
 
 
 def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None, mean=None, rstd=None,
                       stream=None):
     """(y, mean, rstd) over the last dimension; mean and rstd are fp32, one per row."""
-    device = _cuda(x, "x")
+    dev = _device(x, "x")
     rows, dim, xs = _rows(x, "x")
     dtype = _dtype(x, "x")
     given = gamma if gamma is not None else beta
     params = given.dtype if given is not None else torch.float32
-    g = _vector(gamma, "gamma", dim, params, device)
-    b = _vector(beta, "beta", dim, params, device)
-    with _Call(device, stream) as call:
-        out = call.new("out", x.shape, x.dtype) if out is None else out
-        mean = call.new("mean", x.shape[:-1], torch.float32) if mean is None else mean
-        rstd = call.new("rstd", x.shape[:-1], torch.float32) if rstd is None else rstd
-        ys = _matrix(out, "out", rows, dim, x.dtype, device)
-        check(lib().b200opt_layernorm_fwd(
-            dtype, _dtype(given, "gamma") if given is not None else capi.FLOAT, rows, dim,
-            x.data_ptr(), xs, g, b, eps, out.data_ptr(), ys,
-            _vector(mean, "mean", rows, torch.float32, device),
-            _vector(rstd, "rstd", rows, torch.float32, device), call.stream))
+    if out is None:
+        out, ys = _new(x, x.shape, x.dtype, "out", stream), max(dim, 1)
+    else:
+        ys = _matrix(out, "out", rows, dim, x.dtype, dev)
+    if mean is None:
+        mean = _new(x, x.shape[:-1], torch.float32, "mean", stream)
+    if rstd is None:
+        rstd = _new(x, x.shape[:-1], torch.float32, "rstd", stream)
+    _call(lib().b200opt_layernorm_fwd, dev, stream, dtype, _DTYPES.get(params, -1), rows, dim,
+          x.data_ptr(), xs, _vector(gamma, "gamma", dim, params, dev),
+          _vector(beta, "beta", dim, params, dev), eps, out.data_ptr(), ys,
+          _vector(mean, "mean", rows, torch.float32, dev),
+          _vector(rstd, "rstd", rows, torch.float32, dev))
     return out, mean, rstd
 
 
 def layernorm_workspace(rows, dim):
     """Bytes of workspace that layernorm_backward needs."""
-    need = C.c_size_t()
-    check(lib().b200opt_layernorm_bwd_workspace(rows, dim, C.byref(need)))
-    return need.value
+    return _bytes("b200opt_layernorm_bwd_workspace", rows, dim)
 
 
 def layernorm_backward(grad_y, x, gamma, mean, rstd, grad_x=None, grad_gamma=None, grad_beta=None,
                        accumulate=False, workspace=None, stream=None):
     """(grad_x, grad_gamma, grad_beta); the last two in gamma's dtype (fp32 without gamma)."""
-    device = _cuda(x, "x")
+    dev = _device(x, "x")
     rows, dim, xs = _rows(x, "x")
     dtype = _dtype(x, "x")
     params = gamma.dtype if gamma is not None else torch.float32
-    g = _vector(gamma, "gamma", dim, params, device)
-    ys = _matrix(grad_y, "grad_y", rows, dim, x.dtype, device)
-    mu = _vector(mean, "mean", rows, torch.float32, device)
-    rs = _vector(rstd, "rstd", rows, torch.float32, device)
+    ys = _matrix(grad_y, "grad_y", rows, dim, x.dtype, dev)
     if accumulate and (grad_gamma is None or grad_beta is None):
         raise ValueError("accumulate needs grad_gamma and grad_beta")
-    with _Call(device, stream) as call:
-        grad_x = call.new("grad_x", x.shape, x.dtype) if grad_x is None else grad_x
-        grad_gamma = call.new("grad_gamma", (dim,), params) if grad_gamma is None else grad_gamma
-        grad_beta = call.new("grad_beta", (dim,), params) if grad_beta is None else grad_beta
-        dxs = _matrix(grad_x, "grad_x", rows, dim, x.dtype, device)
-        keep, wp, wb = call.workspace(workspace, "b200opt_layernorm_bwd_workspace", rows, dim)
-        check(lib().b200opt_layernorm_bwd(
-            dtype, _DTYPES.get(params, -1), rows, dim, grad_y.data_ptr(), ys, x.data_ptr(), xs, g,
-            mu, rs, grad_x.data_ptr(), dxs, _vector(grad_gamma, "grad_gamma", dim, params, device),
-            _vector(grad_beta, "grad_beta", dim, params, device), int(accumulate), wp, wb,
-            call.stream))
+    if grad_x is None:
+        grad_x, dxs = _new(x, x.shape, x.dtype, "grad_x", stream), max(dim, 1)
+    else:
+        dxs = _matrix(grad_x, "grad_x", rows, dim, x.dtype, dev)
+    if grad_gamma is None:
+        grad_gamma = _new(x, (dim,), params, "grad_gamma", stream)
+    if grad_beta is None:
+        grad_beta = _new(x, (dim,), params, "grad_beta", stream)
+    keep, wp, wb = _workspace(workspace, layernorm_workspace(rows, dim), x, dev, stream)
+    _call(lib().b200opt_layernorm_bwd, dev, stream, dtype, _DTYPES.get(params, -1), rows, dim,
+          grad_y.data_ptr(), ys, x.data_ptr(), xs, _vector(gamma, "gamma", dim, params, dev),
+          _vector(mean, "mean", rows, torch.float32, dev),
+          _vector(rstd, "rstd", rows, torch.float32, dev), grad_x.data_ptr(), dxs,
+          _vector(grad_gamma, "grad_gamma", dim, params, dev),
+          _vector(grad_beta, "grad_beta", dim, params, dev), int(accumulate), wp, wb)
     return grad_x, grad_gamma, grad_beta
 
 
 def _head(hidden, weight, targets):
-    device = _cuda(hidden, "hidden")
-    _on(device, "weight", weight)
+    dev = _device(hidden, "hidden")
+    _on(dev, "weight", weight)
     tokens, dim, xs = _rows(hidden, "hidden", dtype=torch.float16)
     vocab, _, ws = _rows(weight, "weight", dim, torch.float16)
-    y, wide = _index(targets, "targets", device)
+    y, wide = _index(targets, "targets", dev)
     if targets.numel() != tokens:
         raise ValueError(f"{targets.numel()} targets, but {tokens} rows in hidden")
-    return device, (tokens, vocab, dim), (hidden.data_ptr(), xs, weight.data_ptr(), ws, y, wide)
+    return dev, (tokens, vocab, dim), (hidden.data_ptr(), xs, weight.data_ptr(), ws, y, wide)
 
 
 def vocab_loss_workspace(tokens, vocab, dim):
     """Bytes of workspace that (vocab_loss_forward, vocab_loss_backward) need."""
-    a, b = C.c_size_t(), C.c_size_t()
-    check(lib().b200opt_vocab_loss_fwd_workspace(tokens, vocab, dim, C.byref(a)))
-    check(lib().b200opt_vocab_loss_bwd_workspace(tokens, vocab, dim, C.byref(b)))
-    return a.value, b.value
+    return (_bytes("b200opt_vocab_loss_fwd_workspace", tokens, vocab, dim),
+            _bytes("b200opt_vocab_loss_bwd_workspace", tokens, vocab, dim))
 
 
 def vocab_loss_forward(hidden, weight, targets, loss=None, lse=None, stats=None, workspace=None,
@@ -262,16 +265,19 @@ def vocab_loss_forward(hidden, weight, targets, loss=None, lse=None, stats=None,
     """(loss, lse, stats) of softmax cross entropy with logits hidden @ weight.T, which are never
     stored.  loss and lse: fp32 per token; stats: fp32 {sum of losses, tokens counted}.  Targets
     outside the vocabulary are ignored."""
-    device, sizes, args = _head(hidden, weight, targets)
-    with _Call(device, stream) as call:
-        loss = call.new("loss", targets.shape, torch.float32) if loss is None else loss
-        lse = call.new("lse", targets.shape, torch.float32) if lse is None else lse
-        stats = call.new("stats", (2,), torch.float32) if stats is None else stats
-        keep, wp, wb = call.workspace(workspace, "b200opt_vocab_loss_fwd_workspace", *sizes)
-        check(lib().b200opt_vocab_loss_fwd(
-            *sizes, *args, _vector(loss, "loss", sizes[0], torch.float32, device),
-            _vector(lse, "lse", sizes[0], torch.float32, device),
-            _vector(stats, "stats", 2, torch.float32, device), wp, wb, call.stream))
+    dev, sizes, args = _head(hidden, weight, targets)
+    if loss is None:
+        loss = _new(hidden, targets.shape, torch.float32, "loss", stream)
+    if lse is None:
+        lse = _new(hidden, targets.shape, torch.float32, "lse", stream)
+    if stats is None:
+        stats = _new(hidden, (2,), torch.float32, "stats", stream)
+    keep, wp, wb = _workspace(workspace, _bytes("b200opt_vocab_loss_fwd_workspace", *sizes), hidden,
+                              dev, stream)
+    _call(lib().b200opt_vocab_loss_fwd, dev, stream, *sizes, *args,
+          _vector(loss, "loss", sizes[0], torch.float32, dev),
+          _vector(lse, "lse", sizes[0], torch.float32, dev),
+          _vector(stats, "stats", 2, torch.float32, dev), wp, wb)
     return loss, lse, stats
 
 
@@ -281,23 +287,26 @@ def vocab_loss_backward(hidden, weight, targets, lse, stats=None, grad_scale=1.0
     """(grad_hidden, grad_weight) of the losses' mean (``stats`` of the forward pass given) or sum,
     times grad_scale and times the loss scale: a one-element fp32 tensor, or a device address such
     as ``AdamGroup.device_scale_ptr()`` returns."""
-    device, sizes, args = _head(hidden, weight, targets)
+    dev, sizes, args = _head(hidden, weight, targets)
     tokens, vocab, dim = sizes
-    lse_ptr = _vector(lse, "lse", tokens, torch.float32, device)
-    stats_ptr = _vector(stats, "stats", 2, torch.float32, device)
-    scale_ptr = (loss_scale if loss_scale is None or isinstance(loss_scale, int)
-                 else _vector(loss_scale, "loss_scale", 1, torch.float32, device))
     if accumulate and grad_weight is None:
         raise ValueError("accumulate needs grad_weight")
-    with _Call(device, stream) as call:
-        if grad_hidden is None:
-            grad_hidden = call.new("grad_hidden", hidden.shape, torch.float16)
-        if grad_weight is None:
-            grad_weight = call.new("grad_weight", weight.shape, torch.float16)
-        xs = _matrix(grad_hidden, "grad_hidden", tokens, dim, torch.float16, device)
-        ws = _matrix(grad_weight, "grad_weight", vocab, dim, torch.float16, device)
-        keep, wp, wb = call.workspace(workspace, "b200opt_vocab_loss_bwd_workspace", *sizes)
-        check(lib().b200opt_vocab_loss_bwd(
-            *sizes, *args, lse_ptr, stats_ptr, grad_scale, scale_ptr, grad_hidden.data_ptr(), xs,
-            grad_weight.data_ptr(), ws, int(accumulate), wp, wb, call.stream))
+    if grad_hidden is None:
+        grad_hidden = _new(hidden, hidden.shape, torch.float16, "grad_hidden", stream)
+        xs = dim
+    else:
+        xs = _matrix(grad_hidden, "grad_hidden", tokens, dim, torch.float16, dev)
+    if grad_weight is None:
+        grad_weight = _new(weight, weight.shape, torch.float16, "grad_weight", stream)
+        ws = dim
+    else:
+        ws = _matrix(grad_weight, "grad_weight", vocab, dim, torch.float16, dev)
+    if loss_scale is not None and not isinstance(loss_scale, int):
+        loss_scale = _vector(loss_scale, "loss_scale", 1, torch.float32, dev)
+    keep, wp, wb = _workspace(workspace, _bytes("b200opt_vocab_loss_bwd_workspace", *sizes), hidden,
+                              dev, stream)
+    _call(lib().b200opt_vocab_loss_bwd, dev, stream, *sizes, *args,
+          _vector(lse, "lse", tokens, torch.float32, dev),
+          _vector(stats, "stats", 2, torch.float32, dev), grad_scale, loss_scale,
+          grad_hidden.data_ptr(), xs, grad_weight.data_ptr(), ws, int(accumulate), wp, wb)
     return grad_hidden, grad_weight
