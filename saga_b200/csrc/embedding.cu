@@ -70,19 +70,24 @@ __device__ __forceinline__ uint32_t key_of(const void *ids, int wide, size_t t, 
 
 // Ranks this warp's keys (items i * 32 + lane, i < trips) among its earlier keys
 // of the same digit; count[digit] (this warp's, zeroed) ends as the number of
-// keys.  Keys that do not exist have digit kDigits - 1 + nothing: `live` is false.
-__device__ __forceinline__ void warp_rank(const uint32_t (&key)[kSortItems], int shift, uint32_t mask,
+// keys.  The lanes with the same digit are found by one ballot per bit of it.
+__device__ __forceinline__ void warp_rank(const uint32_t (&key)[kSortItems], int shift, int bits,
                                           int trips, unsigned live, uint16_t *count,
                                           uint16_t (&rank)[kSortItems])
 {
     const int lane = threadIdx.x & 31;
+    const uint32_t mask = (1u << bits) - 1;
 #pragma unroll
     for(int i = 0; i < kSortItems; i++) {
         if(i >= trips)
             break;
         const bool here = live >> i & 1;
-        const uint32_t d = here ? (key[i] >> shift) & mask : 0xffffffffu;
-        const unsigned same = __match_any_sync(0xffffffffu, d);
+        const uint32_t d = here ? (key[i] >> shift) & mask : 0;
+        unsigned same = __ballot_sync(0xffffffffu, here);
+        for(int b = 0; b < bits; b++) {
+            const unsigned set = __ballot_sync(0xffffffffu, d >> b & 1);
+            same &= d >> b & 1 ? set : ~set;
+        }
         const int before = __popc(same & ((1u << lane) - 1));
         if(here)
             rank[i] = count[d] + before;
@@ -124,15 +129,19 @@ __device__ void sort_one_block(int tokens, size_t vocab, int bits, const void *i
         for(int i = tid; i < 32 * kDigits / 2; i += 1024)
             reinterpret_cast<uint32_t *>(count)[i] = 0;
         __syncthreads();
-        warp_rank(key, shift, mask, trips, live, count + warp * kDigits, rank);
+        warp_rank(key, shift, step, trips, live, count + warp * kDigits, rank);
         __syncthreads();
         // exclusive sums: digit by digit, within a digit warp by warp
         int sum = 0;
         if(tid < kDigits) {
+            int c[32];
+#pragma unroll
+            for(int w = 0; w < 32; w++)
+                c[w] = count[w * kDigits + tid];
+#pragma unroll
             for(int w = 0; w < 32; w++) {
-                const int c = count[w * kDigits + tid];
                 count[w * kDigits + tid] = (uint16_t)sum;
-                sum += c;
+                sum += c[w];
             }
             int run = sum;
 #pragma unroll
@@ -249,10 +258,11 @@ __global__ void __launch_bounds__(1024) sort_sums_kernel(int *counts, int n)
 
 __global__ void __launch_bounds__(kManyThreads)
     sort_move_kernel(size_t tokens, size_t vocab, const void *ids, int wide, const uint32_t *keys,
-                     const int *order, int shift, uint32_t mask, const int *counts, int blocks,
+                     const int *order, int shift, int bits, const int *counts, int blocks,
                      uint32_t *keys_out, int *order_out)
 {
     constexpr int kWarps = kManyThreads / 32;
+    const uint32_t mask = (1u << bits) - 1;
     __shared__ uint16_t count[kWarps * kDigits];
     for(int i = threadIdx.x; i < kWarps * kDigits / 2; i += kManyThreads)
         reinterpret_cast<uint32_t *>(count)[i] = 0;
@@ -262,7 +272,7 @@ __global__ void __launch_bounds__(kManyThreads)
     uint16_t rank[kSortItems];
     const int warp = threadIdx.x >> 5;
     const unsigned live = load_keys(tokens, vocab, ids, wide, keys, order, key, item);
-    warp_rank(key, shift, mask, kSortItems, live, count + warp * kDigits, rank);
+    warp_rank(key, shift, bits, kSortItems, live, count + warp * kDigits, rank);
     __syncthreads();
     for(int d = threadIdx.x; d < kDigits; d += kManyThreads) {
         int sum = 0;
@@ -371,8 +381,7 @@ __global__ void __launch_bounds__(1024)
 // from the chunk before, slot 1 for one that begins here.  join_kernel adds up
 // the parts, in order.
 
-constexpr int kChunk = 32;
-constexpr int kAhead = 8;  // rows in flight per thread
+constexpr int kChunk = 16;  // all rows of a chunk are in flight at once
 
 template <typename T, int N>
 __device__ __forceinline__ void write_row(T *row, size_t c, float (&sum)[N], float scale, int accumulate)
@@ -401,45 +410,54 @@ __global__ void __launch_bounds__(256)
     if(e0 >= tokens || c >= vecs)
         return;
     const int n = (int)min((size_t)kChunk, tokens - e0);
-    uint32_t run = keys[e0];
-    bool came = e0 > 0 && keys[e0 - 1] == run;  // the run began in an earlier chunk
+    // keys and order of the chunk as whole words; behind the last token stands
+    // what the workspace held, which no sum uses
+    union {
+        uint4 q[kChunk / 4];
+        uint32_t k[kChunk];
+    } key;
+    union {
+        int4 q[kChunk / 4];
+        int t[kChunk];
+    } from;
+#pragma unroll
+    for(int i = 0; i < kChunk / 4; i++) {
+        key.q[i] = reinterpret_cast<const uint4 *>(keys + e0)[i];
+        from.q[i] = reinterpret_cast<const int4 *>(order + e0)[i];
+    }
+    const uint32_t behind = e0 + kChunk < tokens ? keys[e0 + kChunk] : 0xffffffffu;
+    bool came = e0 > 0 && keys[e0 - 1] == key.k[0];  // the run began in an earlier chunk
+    Vec<T, N> v[kChunk];
+#pragma unroll
+    for(int i = 0; i < kChunk; i++)
+        if(i < n && key.k[i] < vocab)
+            v[i] = reinterpret_cast<const Vec<T, N> *>(dy + (size_t)from.t[i] * ys)[c];
     float sum[N] = {};
-    for(int i0 = 0; i0 < n; i0 += kAhead) {
-        Vec<T, N> v[kAhead];
-        uint32_t next[kAhead];  // the key behind each of the tokens
 #pragma unroll
-        for(int i = 0; i < kAhead; i++)
-            if(i0 + i < n) {
-                v[i] = reinterpret_cast<const Vec<T, N> *>(dy + (size_t)order[e0 + i0 + i] * ys)[c];
-                next[i] = e0 + i0 + i + 1 < tokens ? keys[e0 + i0 + i + 1] : 0xffffffffu;
+    for(int i = 0; i < kChunk; i++) {
+        const uint32_t run = key.k[i];
+        if(i >= n || run >= vocab)  // ids outside the table: all that follow are
+            return;
+        float f[N];
+        v[i].get(f);
+#pragma unroll
+        for(int j = 0; j < N; j++)
+            sum[j] += f[j];
+        const uint32_t next = i + 1 < n ? key.k[i + 1 < kChunk ? i + 1 : i] : behind;
+        const bool ends = next != run;
+        if(ends || i + 1 == n) {
+            if(ends && !came) {
+                write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
+            } else {
+                Vec<float, N> part;
+                part.set(sum);
+                *reinterpret_cast<Vec<float, N> *>(
+                    parts + ((chunk * 2 + (came ? 0 : 1)) * vecs + c) * N) = part;
             }
-#pragma unroll
-        for(int i = 0; i < kAhead; i++) {
-            if(i0 + i >= n)
-                break;
-            if(run >= vocab)  // ids outside the table: all that follow are
-                return;
-            float f[N];
-            v[i].get(f);
 #pragma unroll
             for(int j = 0; j < N; j++)
-                sum[j] += f[j];
-            const bool ends = next[i] != run;
-            if(ends || i0 + i + 1 == n) {
-                if(ends && !came) {
-                    write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
-                } else {
-                    float *to = parts + ((chunk * 2 + (came ? 0 : 1)) * vecs + c) * N;
-#pragma unroll
-                    for(int j = 0; j < N; j++)
-                        to[j] = sum[j];
-                }
-#pragma unroll
-                for(int j = 0; j < N; j++)
-                    sum[j] = 0.0f;
-                run = next[i];
-                came = false;
-            }
+                sum[j] = 0.0f;
+            came = false;
         }
     }
 }
@@ -458,26 +476,31 @@ __global__ void __launch_bounds__(256)
     // the run that leaves this chunk, if it began here
     if(run >= vocab || keys[e1] != run || (e0 > 0 && keys[e0] == run && keys[e0 - 1] == run))
         return;
-    size_t lo = e1, hi = tokens;  // its end: the first key beyond
-    while(lo < hi) {
-        const size_t mid = (lo + hi) / 2;
-        if(keys[mid] <= run)
-            lo = mid + 1;
-        else
-            hi = mid;
+    // the chunk it ends in: the first whose next chunk does not begin with it
+    const size_t chunks = (tokens + kChunk - 1) / kChunk;
+    auto inside = [&](size_t k) { return k + 1 < chunks && keys[(k + 1) * kChunk] == run; };
+    size_t last = chunk + 1, hop = 1;
+    while(inside(last + hop - 1)) {
+        last += hop;
+        hop *= 2;
     }
-    const size_t last = (lo - 1) / kChunk;
+    while(hop > 1) {  // inside(last - 1) holds
+        hop /= 2;
+        if(inside(last + hop - 1))
+            last += hop;
+    }
     float sum[N];
-    const float *first = parts + ((chunk * 2 + 1) * vecs + c) * N;
-#pragma unroll
-    for(int j = 0; j < N; j++)
-        sum[j] = first[j];
+    reinterpret_cast<const Vec<float, N> *>(parts + ((chunk * 2 + 1) * vecs + c) * N)->get(sum);
+    const float *p = parts + ((chunk + 1) * 2 * vecs + c) * N;
 #pragma unroll 8
-    for(size_t k = chunk + 1; k <= last; k++) {
-        const float *p = parts + (k * 2 * vecs + c) * N;
+    for(size_t k = chunk + 1; k <= last; k++, p += 2 * vecs * N) {
+        Vec<float, N> v;
+        float f[N];
+        v = *reinterpret_cast<const Vec<float, N> *>(p);
+        v.get(f);
 #pragma unroll
         for(int j = 0; j < N; j++)
-            sum[j] += p[j];
+            sum[j] += f[j];
     }
     write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
 }
@@ -518,10 +541,10 @@ struct Work {
         };
         const bool many = tokens > kOneBlock;
         blocks = (tokens + kManyItems - 1) / kManyItems;
-        at_keys = take(tokens * 4);
-        at_order = take(tokens * 4);
-        at_keys2 = take(many ? tokens * 4 : 0);
-        at_order2 = take(many ? tokens * 4 : 0);
+        at_keys = take(lm_up(tokens, kChunk) * 4);
+        at_order = take(lm_up(tokens, kChunk) * 4);
+        at_keys2 = take(many ? lm_up(tokens, kChunk) * 4 : 0);
+        at_order2 = take(many ? lm_up(tokens, kChunk) * 4 : 0);
         at_counts = take(many ? blocks * kDigits * 4 : 0);
         at_parts = take((tokens + kChunk - 1) / kChunk * 2 * dim * 4);
         bytes = at;
@@ -562,7 +585,7 @@ int gradient(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide,
                                                                p * step, mask, counts, (int)blocks);
             sort_sums_kernel<<<1, 1024, 0, st>>>(counts, (int)blocks * kDigits);
             sort_move_kernel<<<blocks, kManyThreads, 0, st>>>(tokens, vocab, ids, wide, from_k, from_o,
-                                                              p * step, mask, counts, (int)blocks, to_k,
+                                                              p * step, step, counts, (int)blocks, to_k,
                                                               to_o);
             from_k = to_k, from_o = to_o;
             std::swap(keys, to_k), std::swap(order, to_o);

@@ -149,8 +149,16 @@ __global__ void __launch_bounds__(1024)
 // thread keeps the parameters' sums of its own columns in registers and leaves
 // them in `parts` at the end, for params_kernel to join in a fixed order.  The
 // next row's vectors are loaded before the present row's sums are waited for.
+#ifndef B16
+#define B16 2
+#endif
+#ifndef FWDW
+#define FWDW 16
+#endif
+constexpr int bwd_blocks(int columns) { return columns <= 8 ? 3 : columns <= 16 ? B16 : 1; }
+
 template <typename T, typename P, int N, int NV, int WARPS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(kThreads, bwd_blocks(N * NV))
     layernorm_bwd_kernel(size_t rows, size_t dim, const T *dy, size_t ys, const T *x, size_t xs,
                          const P *gamma, const float *mean, const float *rstd, T *dx, size_t dxs,
                          float *parts)
@@ -258,16 +266,16 @@ __global__ void __launch_bounds__(kThreads)
             pg[d] = joined[d];
             pb[d] = joined[32 * NV * N + d];
         }
-        return;
+    } else {
+#pragma unroll
+        for(int i = 0; i < NV; i++)
+            if(l + i * L < vecs)
+#pragma unroll
+                for(int j = 0; j < N; j++) {
+                    pg[(l + i * L) * N + j] = sg[i][j];
+                    pb[(l + i * L) * N + j] = sb[i][j];
+                }
     }
-#pragma unroll
-    for(int i = 0; i < NV; i++)
-        if(l + i * L < vecs)
-#pragma unroll
-            for(int j = 0; j < N; j++) {
-                pg[(l + i * L) * N + j] = sg[i][j];
-                pb[(l + i * L) * N + j] = sb[i][j];
-            }
 }
 
 // Joins the blocks' sums: 32 columns and 8 stretches of blocks a block.
@@ -393,7 +401,7 @@ int fwd_with(const Args &a)
             a.ys, a.mean, a.rstd);
     };
     const size_t vecs = a.dim / N;
-    if(!pick<N, 1, 16>(vecs, launch) && !pick_block<N, 4, 16>(vecs, launch))
+    if(!pick<N, 1, FWDW>(vecs, launch) && !pick_block<N, FWDW/4, 16>(vecs, launch))
         layernorm_fwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
             a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y, a.ys,
             a.mean, a.rstd);
@@ -408,7 +416,7 @@ int bwd_with(const Args &a)
     size_t blocks = 0;
     auto launch = [&](auto nv, auto warps) {
         constexpr int NV = decltype(nv)::value, W = decltype(warps)::value;
-        blocks = std::min<size_t>((a.rows + 8 / W - 1) / (8 / W), kMaxParts);
+        blocks = std::min<size_t>((a.rows + 8 / W - 1) / (8 / W), 148 * bwd_blocks(N * NV));
         if(blocks)
             layernorm_bwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, kThreads, 0, a.st>>>(
                 a.rows, a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma,

@@ -87,6 +87,10 @@ struct Vec<float, 8> {
     {
         f[0] = a.x, f[1] = a.y, f[2] = a.z, f[3] = a.w, f[4] = b.x, f[5] = b.y, f[6] = b.z, f[7] = b.w;
     }
+    __device__ __forceinline__ void set(const float (&f)[8])
+    {
+        a = make_float4(f[0], f[1], f[2], f[3]), b = make_float4(f[4], f[5], f[6], f[7]);
+    }
 };
 template <typename T>
 struct Vec<T, 1> {
