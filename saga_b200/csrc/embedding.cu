@@ -51,325 +51,161 @@ __global__ void __launch_bounds__(256)
 // --------------------------------------------------------- order of the tokens
 //
 // The gradient of a row is the sum over the row's tokens, in ascending token
-// order.  The tokens are brought into that order by a stable radix sort of
-// (id, token), least digit first; ids outside the table get the key `vocab` and
-// end up last.  A warp ranks 32 keys at a time with one match over their digits;
-// a table of counts per warp and digit gives the places.
+// order, so the tokens are brought together by id.  Block b takes the ids that
+// are b modulo the number of blocks: neighbouring ids, frequent ones among them,
+// fall to different blocks.  Every block looks at all ids (64 KB of int32 for 16384
+// tokens, from L2), counts its own by their quotient, knows from the count of
+// smaller remainders where its tokens begin, and moves them there by one stable
+// counting pass: ranks within a warp's stretch, then sums over warps and digits.
 
-constexpr int kDigits = 512;      // nine bits a pass: two passes up to 2^18 rows
-constexpr int kSortItems = 16;    // keys a thread holds
-constexpr int kOneBlock = 1024 * kSortItems;  // tokens that one block sorts by itself
-constexpr int kManyThreads = 512;
-constexpr int kManyItems = kManyThreads * kSortItems;
+constexpr int kChunk = 16;  // tokens summed by one group of threads
+constexpr int kOrderThreads = 1024;
+constexpr int kOrderWarps = kOrderThreads / 32;
+constexpr int kStretch = 512;                             // consecutive tokens of a warp
+constexpr int kOrderChunk = kOrderWarps * kStretch;       // tokens at a time
+constexpr int kDigits = 512;                              // rows a block can have
+constexpr int kOrderSmem = kOrderChunk * 4 + kOrderWarps * kDigits * 2;
 
-__device__ __forceinline__ uint32_t key_of(const void *ids, int wide, size_t t, size_t vocab)
+// keys: the ids in their new order, `vocab` behind the last; order: the tokens;
+// ends: where a run of equal ids ends (at its first kChunk tokens).  named: for
+// each row, whether it has a token.
+//
+// The loops stay rolled: the code runs once per block, so its length, fetched cold,
+// would cost more than the branches (unrolled over the ids of a thread it took 9 us
+// for 64 tokens).
+__global__ void __launch_bounds__(kOrderThreads, 1)
+    order_kernel(size_t tokens, size_t vocab, const void *ids, int wide, uint32_t *keys, int *order,
+                 int *ends, unsigned char *named)
 {
-    const int id = lm_index_at(ids, wide, t, vocab);
-    return id < 0 ? (uint32_t)vocab : (uint32_t)id;
-}
-
-// Ranks this warp's keys (items i * 32 + lane, i < trips) among its earlier keys
-// of the same digit; count[digit] (this warp's, zeroed) ends as the number of
-// keys.  The lanes with the same digit are found by one ballot per bit of it.
-__device__ __forceinline__ void warp_rank(const uint32_t (&key)[kSortItems], int shift, int bits,
-                                          int trips, unsigned live, uint16_t *count,
-                                          uint16_t (&rank)[kSortItems])
-{
-    const int lane = threadIdx.x & 31;
-    const uint32_t mask = (1u << bits) - 1;
-#pragma unroll
-    for(int i = 0; i < kSortItems; i++) {
-        if(i >= trips)
-            break;
-        const bool here = live >> i & 1;
-        const uint32_t d = here ? (key[i] >> shift) & mask : 0;
-        unsigned same = __ballot_sync(0xffffffffu, here);
-        for(int b = 0; b < bits; b++) {
-            const unsigned set = __ballot_sync(0xffffffffu, d >> b & 1);
-            same &= d >> b & 1 ? set : ~set;
-        }
-        const int before = __popc(same & ((1u << lane) - 1));
-        if(here)
-            rank[i] = count[d] + before;
-        __syncwarp();
-        if(here && before == 0)
-            count[d] += __popc(same);
-        __syncwarp();
-    }
-}
-
-// One block sorts up to kOneBlock tokens in shared memory.
-__device__ void sort_one_block(int tokens, size_t vocab, int bits, const void *ids, int wide,
-                               char *smem, uint32_t *keys_out, int *order_out)
-{
-    uint32_t *keys = reinterpret_cast<uint32_t *>(smem);
-    uint16_t *order = reinterpret_cast<uint16_t *>(smem + kOneBlock * 4);
-    uint16_t *count = reinterpret_cast<uint16_t *>(smem + kOneBlock * 6);  // [32 warps][kDigits]
-    int *total = reinterpret_cast<int *>(smem + kOneBlock * 6 + 32 * kDigits * 2);  // [kDigits]
-    __shared__ int warp_total[32];
+    extern __shared__ __align__(16) char order_smem[];
+    // this block's tokens, in order, for each warp: place in its stretch << 20 | rank << 9 | digit
+    uint32_t *list = reinterpret_cast<uint32_t *>(order_smem) + (threadIdx.x >> 5) * kStretch;
+    uint16_t *counts = reinterpret_cast<uint16_t *>(order_smem + kOrderChunk * 4);
+    __shared__ int base[kDigits], warp_sums[kOrderWarps], before_sum, valid_sum;
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int trips = (tokens + 1023) / 1024;
-    const int first = warp * trips * 32 + lane;  // of this thread's keys
-    unsigned live = 0;
-    uint32_t key[kSortItems];
-    uint16_t item[kSortItems], rank[kSortItems];
-#pragma unroll
-    for(int i = 0; i < kSortItems; i++) {
-        const int t = first + 32 * i;
-        if(i < trips && t < tokens) {
-            live |= 1u << i;
-            key[i] = key_of(ids, wide, t, vocab);
-            item[i] = (uint16_t)t;
-        }
-    }
-    const int passes = (bits + 8) / 9, step = (bits + passes - 1) / passes;
-    for(int p = 0; p < passes; p++) {
-        const int shift = p * step;
-        const uint32_t mask = (1u << step) - 1;
-        for(int i = tid; i < 32 * kDigits / 2; i += 1024)
-            reinterpret_cast<uint32_t *>(count)[i] = 0;
-        __syncthreads();
-        warp_rank(key, shift, step, trips, live, count + warp * kDigits, rank);
-        __syncthreads();
-        // exclusive sums: digit by digit, within a digit warp by warp
-        int sum = 0;
-        if(tid < kDigits) {
-            int c[32];
-#pragma unroll
-            for(int w = 0; w < 32; w++)
-                c[w] = count[w * kDigits + tid];
-#pragma unroll
-            for(int w = 0; w < 32; w++) {
-                count[w * kDigits + tid] = (uint16_t)sum;
-                sum += c[w];
-            }
-            int run = sum;
-#pragma unroll
-            for(int o = 1; o < 32; o <<= 1) {
-                const int v = __shfl_up_sync(0xffffffffu, run, o);
-                run += lane >= o ? v : 0;
-            }
-            total[tid] = run - sum;
-            if(lane == 31)
-                warp_total[warp] = run;
-        }
-        __syncthreads();
-        if(tid < kDigits) {
-            int ahead = 0;
-            for(int w = 0; w < warp; w++)
-                ahead += warp_total[w];
-            total[tid] += ahead;
-        }
-        __syncthreads();
-#pragma unroll
-        for(int i = 0; i < kSortItems; i++)
-            if(live >> i & 1) {
-                const uint32_t d = (key[i] >> shift) & mask;
-                const int at = total[d] + count[warp * kDigits + d] + rank[i];
-                keys[at] = key[i];
-                order[at] = item[i];
-            }
-        __syncthreads();
-        if(p + 1 < passes) {
-#pragma unroll
-            for(int i = 0; i < kSortItems; i++)
-                if(live >> i & 1) {
-                    key[i] = keys[first + 32 * i];
-                    item[i] = order[first + 32 * i];
+    const uint32_t blocks = gridDim.x, me = blockIdx.x;
+    // id / blocks by a rounded-down reciprocal: at most one too small below 2^31
+    const uint32_t inverse = 0xffffffffu / blocks;
+    const int digits = (int)((vocab - me + blocks - 1) / blocks);  // this block's rows
+    uint16_t *count = counts + warp * kDigits;
+    // a warp's stretch: shorter where there are few tokens, so that all warps have some
+    const int stretch =
+        (int)min((tokens + kOrderThreads - 1) / kOrderThreads * 32, (size_t)kStretch);
+    const size_t step = (size_t)stretch * kOrderWarps;
+    if(tid < kDigits)
+        base[tid] = 0;
+    if(tid == 0)
+        before_sum = valid_sum = 0;
+    __syncthreads();
+
+    int n = 0, before = 0, valid = 0, my_start = 0, my_end = 0;
+    for(int pass = 0; pass < 2; pass++) {
+        for(size_t c0 = 0; c0 < tokens; c0 += step) {
+            const size_t first = c0 + warp * stretch;
+            if(pass == 0 || tokens > step) {
+                n = 0;
+                // the stretch's ids, many loads in flight; the block's own replace them
+                const int here = (int)min((size_t)stretch, tokens > first ? tokens - first : 0);
+                __syncwarp();
+#pragma unroll 16
+                for(int i = lane; i < here; i += 32)
+                    list[i] = (uint32_t)lm_index_at(ids, wide, first + i, vocab);
+                __syncwarp();
+                for(int i = lane; i - lane < here; i += 32) {
+                    const int id = i < here ? (int)list[i] : -1;
+                    uint32_t q = __umulhi((uint32_t)id, inverse), r = (uint32_t)id - q * blocks;
+                    if(r >= blocks)
+                        q++, r -= blocks;
+                    const bool mine = id >= 0 && r == me;
+                    if(pass == 0) {
+                        before += id >= 0 && r < me;
+                        valid += id >= 0;
+                        if(mine)
+                            atomicAdd(&base[q], 1);  // whole numbers: any order gives the same
+                    }
+                    const unsigned who = __ballot_sync(0xffffffffu, mine);
+                    if(mine)
+                        list[n + __popc(who & ((1u << lane) - 1))] = (uint32_t)i << 20 | q;
+                    n += __popc(who);
                 }
-        }
-    }
-    for(int i = tid; i < tokens; i += 1024) {
-        keys_out[i] = keys[i];
-        order_out[i] = order[i];
-    }
-}
-
-constexpr int kSortSmem = kOneBlock * 6 + 32 * kDigits * 2 + kDigits * 4;
-
-// More tokens: per pass, counts of every block of keys, their sums, the move.
-// The first pass reads the ids themselves.
-__device__ __forceinline__ unsigned load_keys(size_t tokens, size_t vocab, const void *ids, int wide,
-                                              const uint32_t *keys, const int *order,
-                                              uint32_t (&key)[kSortItems], int (&item)[kSortItems])
-{
-    const size_t first = (size_t)blockIdx.x * kManyItems + (threadIdx.x >> 5) * (32 * kSortItems) +
-                         (threadIdx.x & 31);
-    unsigned live = 0;
+            }
+            if(pass == 0)
+                continue;
+            for(int i = lane; i < kDigits / 2; i += 32)
+                reinterpret_cast<uint32_t *>(count)[i] = 0;
+            __syncwarp();
+            for(int i = 0; i < n; i += 32) {  // ranks among the warp's tokens of the same digit
+                if(i + lane < n) {
+                    const unsigned here = __activemask();
+                    const uint32_t e = list[i + lane], d = e & (kDigits - 1);
+                    const unsigned same = __match_any_sync(here, d);
+                    const int lower = __popc(same & ((1u << lane) - 1)), seen = count[d];
+                    __syncwarp(here);
+                    if(lower == 0)
+                        count[d] = (uint16_t)(seen + __popc(same));
+                    list[i + lane] = e | (uint32_t)(seen + lower) << 9;
+                }
+                __syncwarp();
+            }
+            __syncthreads();
+            int total = 0;
+            if(tid < kDigits)
+                for(int w = 0; w < kOrderWarps; w += 8) {
+                    int c[8];
 #pragma unroll
-    for(int i = 0; i < kSortItems; i++) {
-        const size_t t = first + 32 * i;
-        if(t < tokens) {
-            live |= 1u << i;
-            key[i] = keys ? keys[t] : key_of(ids, wide, t, vocab);
-            item[i] = keys ? order[t] : (int)t;
-        }
-    }
-    return live;
-}
-
-__global__ void __launch_bounds__(kManyThreads)
-    sort_count_kernel(size_t tokens, size_t vocab, const void *ids, int wide, const uint32_t *keys,
-                      const int *order, int shift, uint32_t mask, int *counts, int blocks)
-{
-    __shared__ int count[kDigits];
-    for(int i = threadIdx.x; i < kDigits; i += kManyThreads)
-        count[i] = 0;
-    __syncthreads();
-    uint32_t key[kSortItems];
-    int item[kSortItems];
-    const unsigned live = load_keys(tokens, vocab, ids, wide, keys, order, key, item);
+                    for(int k = 0; k < 8; k++)
+                        c[k] = counts[(w + k) * kDigits + tid];
 #pragma unroll
-    for(int i = 0; i < kSortItems; i++)
-        if(live >> i & 1)
-            atomicAdd(&count[(key[i] >> shift) & mask], 1);  // whole numbers: no order
-    __syncthreads();
-    for(int i = threadIdx.x; i < kDigits; i += kManyThreads)
-        counts[(size_t)i * blocks + blockIdx.x] = count[i];
-}
-
-__global__ void __launch_bounds__(1024) sort_sums_kernel(int *counts, int n)
-{
-    __shared__ int warp_total[32];
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    int base = 0;
-    for(int i0 = 0; i0 < n; i0 += 1024) {
-        const int i = i0 + tid, c = i < n ? counts[i] : 0;
-        int run = c;
+                    for(int k = 0; k < 8; k++) {
+                        counts[(w + k) * kDigits + tid] = (uint16_t)total;
+                        total += c[k];
+                    }
+                }
+            __syncthreads();
+            for(int i = lane; i < n; i += 32) {
+                const uint32_t e = list[i], d = e & (kDigits - 1);
+                const int at = base[d] + count[d] + (int)(e >> 9 & 0x7ff);
+                keys[at] = d * blocks + me;
+                order[at] = (int)(first + (e >> 20));
+            }
+            __syncthreads();
+            if(tid < kDigits)
+                base[tid] += total;
+        }
+        if(pass)
+            break;
+        // base: from numbers to places
+        before = __reduce_add_sync(0xffffffffu, before);
+        valid = __reduce_add_sync(0xffffffffu, valid);
+        if(lane == 0) {
+            atomicAdd(&before_sum, before);
+            atomicAdd(&valid_sum, valid);
+        }
+        __syncthreads();
+        const int mine = tid < kDigits ? base[tid] : 0;
+        int run = mine;
 #pragma unroll
         for(int o = 1; o < 32; o <<= 1) {
             const int v = __shfl_up_sync(0xffffffffu, run, o);
             run += lane >= o ? v : 0;
         }
         if(lane == 31)
-            warp_total[warp] = run;
+            warp_sums[warp] = run;
         __syncthreads();
-        int ahead = 0, all = 0;
-        for(int w = 0; w < 32; w++) {
-            ahead += w < warp ? warp_total[w] : 0;
-            all += warp_total[w];
-        }
-        if(i < n)
-            counts[i] = base + ahead + run - c;
-        base += all;
-        __syncthreads();
+        my_end = before_sum + run +
+                 __reduce_add_sync(0xffffffffu, lane < warp ? warp_sums[lane] : 0);
+        my_start = my_end - mine;
+        if(tid < kDigits)
+            base[tid] = my_start;
+        if(tid < digits)
+            named[(size_t)tid * blocks + me] = mine > 0;
     }
-}
-
-__global__ void __launch_bounds__(kManyThreads)
-    sort_move_kernel(size_t tokens, size_t vocab, const void *ids, int wide, const uint32_t *keys,
-                     const int *order, int shift, int bits, const int *counts, int blocks,
-                     uint32_t *keys_out, int *order_out)
-{
-    constexpr int kWarps = kManyThreads / 32;
-    const uint32_t mask = (1u << bits) - 1;
-    __shared__ uint16_t count[kWarps * kDigits];
-    for(int i = threadIdx.x; i < kWarps * kDigits / 2; i += kManyThreads)
-        reinterpret_cast<uint32_t *>(count)[i] = 0;
-    __syncthreads();
-    uint32_t key[kSortItems];
-    int item[kSortItems];
-    uint16_t rank[kSortItems];
-    const int warp = threadIdx.x >> 5;
-    const unsigned live = load_keys(tokens, vocab, ids, wide, keys, order, key, item);
-    warp_rank(key, shift, bits, kSortItems, live, count + warp * kDigits, rank);
-    __syncthreads();
-    for(int d = threadIdx.x; d < kDigits; d += kManyThreads) {
-        int sum = 0;
-        for(int w = 0; w < kWarps; w++) {
-            const int c = count[w * kDigits + d];
-            count[w * kDigits + d] = (uint16_t)sum;
-            sum += c;
-        }
-    }
-    __syncthreads();
-#pragma unroll
-    for(int i = 0; i < kSortItems; i++)
-        if(live >> i & 1) {
-            const uint32_t d = (key[i] >> shift) & mask;
-            const int at = counts[(size_t)d * blocks + blockIdx.x] + count[warp * kDigits + d] + rank[i];
-            keys_out[at] = key[i];
-            order_out[at] = item[i];
-        }
-}
-
-// --------------------------------------------------------- rows without tokens
-
-constexpr int kFillRows = 32768;  // rows that a block marks at a time
-
-// Zeros into the rows [v0, v1) that no id names.  With `sorted` the keys are in
-// order and only their stretch of the range is looked at.
-template <typename T, int N>
-__device__ void fill_rows(size_t v0, size_t v1, size_t tokens, size_t vocab, const void *ids, int wide,
-                          const uint32_t *sorted, T *dw, size_t ws, size_t vecs)
-{
-    __shared__ uint32_t named[kFillRows / 32];
-    for(size_t a = v0; a < v1; a += kFillRows) {
-        const size_t b = min(a + kFillRows, v1);
-        for(int i = threadIdx.x; i < kFillRows / 32; i += blockDim.x)
-            named[i] = 0;
-        __syncthreads();
-        size_t lo = 0, hi = tokens;
-        if(sorted) {  // first key >= a
-            while(lo < hi) {
-                const size_t mid = (lo + hi) / 2;
-                if(sorted[mid] < a)
-                    lo = mid + 1;
-                else
-                    hi = mid;
-            }
-        }
-        for(size_t t = lo + threadIdx.x; t < tokens; t += blockDim.x) {
-            const size_t k = sorted ? sorted[t] : key_of(ids, wide, t, vocab);
-            if(k >= a && k < b)
-                atomicOr(&named[(k - a) / 32], 1u << ((k - a) & 31));
-            else if(sorted)
-                break;
-        }
-        __syncthreads();
-        Vec<T, N> zero;
-        float f[N] = {};
-        zero.set(f);
-        if(vecs <= 0xffffffffu / kFillRows) {
-            const uint32_t n = (uint32_t)(b - a) * (uint32_t)vecs, per = (uint32_t)vecs;
-            for(uint32_t i = threadIdx.x; i < n; i += blockDim.x) {
-                const uint32_t r = i / per, c = i - r * per;
-                if(!(named[r / 32] >> (r & 31) & 1))
-                    reinterpret_cast<Vec<T, N> *>(dw + (a + r) * ws)[c] = zero;
-            }
-        } else {
-            for(size_t r = 0; r < b - a; r++)
-                if(!(named[r / 32] >> (r & 31) & 1))
-                    for(size_t c = threadIdx.x; c < vecs; c += blockDim.x)
-                        reinterpret_cast<Vec<T, N> *>(dw + (a + r) * ws)[c] = zero;
-        }
-        __syncthreads();
-    }
-}
-
-// Block 0 sorts; the others, meanwhile, write the rows without tokens.
-template <typename T, int N>
-__global__ void __launch_bounds__(1024)
-    sort_fill_kernel(int tokens, size_t vocab, int bits, const void *ids, int wide, uint32_t *keys,
-                     int *order, T *dw, size_t ws, size_t vecs)
-{
-    extern __shared__ __align__(16) char sort_smem[];
-    if(blockIdx.x == 0) {
-        sort_one_block(tokens, vocab, bits, ids, wide, sort_smem, keys, order);
-    } else {
-        const size_t blocks = gridDim.x - 1, b = blockIdx.x - 1;
-        fill_rows<T, N>(vocab * b / blocks, vocab * (b + 1) / blocks, tokens, vocab, ids, wide, nullptr,
-                        dw, ws, vecs);
-    }
-}
-
-template <typename T, int N>
-__global__ void __launch_bounds__(1024)
-    fill_kernel(size_t tokens, size_t vocab, const uint32_t *sorted, T *dw, size_t ws, size_t vecs)
-{
-    const size_t blocks = gridDim.x, b = blockIdx.x;
-    fill_rows<T, N>(vocab * b / blocks, vocab * (b + 1) / blocks, tokens, vocab, nullptr, 0, sorted, dw,
-                    ws, vecs);
+    // where a run ends, at its first tokens: as far as the chunk it begins in can reach
+    if(tid < kDigits)
+        for(int i = my_start; i < min(my_end, my_start + kChunk); i++)
+            ends[i] = my_end;
+    for(size_t i = (size_t)valid_sum + me * kOrderThreads + tid; i < tokens; i += blocks * kOrderThreads)
+        keys[i] = (uint32_t)vocab;
 }
 
 // ----------------------------------------------------------- sums of the rows
@@ -380,8 +216,6 @@ __global__ void __launch_bounds__(1024)
 // of one that does not, each chunk leaves its part: slot 0 for a run that came
 // from the chunk before, slot 1 for one that begins here.  join_kernel adds up
 // the parts, in order.
-
-constexpr int kChunk = 16;  // all rows of a chunk are in flight at once
 
 template <typename T, int N>
 __device__ __forceinline__ void write_row(T *row, size_t c, float (&sum)[N], float scale, int accumulate)
@@ -398,14 +232,61 @@ __device__ __forceinline__ void write_row(T *row, size_t c, float (&sum)[N], flo
     *to = v;
 }
 
+// Zeros into the rows that no token names: kFill vectors of the table a block, or
+// kFillRows rows a block, a warp each, where rows are not whole vectors.
+constexpr int kFill = 4096;
+constexpr int kFillRows = 32;
+
 template <typename T, int N>
-__global__ void __launch_bounds__(256)
-    sum_kernel(size_t tokens, size_t vocab, size_t vecs, int lanes, const uint32_t *keys,
-               const int *order, const T *dy, size_t ys, float scale, T *dw, size_t ws,
-               int accumulate, float *parts)
+__device__ __forceinline__ void fill_rows(size_t block, size_t vocab, size_t vecs,
+                                          const unsigned char *named, T *dw, size_t ws)
 {
-    const size_t chunk = (size_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
-    const size_t c = (size_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+    if(N > 1) {
+        const size_t at = block * kFill, row0 = at / vecs;
+        const uint32_t col0 = (uint32_t)(at - row0 * vecs), per = (uint32_t)vecs;
+        const uint32_t n = (uint32_t)min((size_t)kFill, vocab * vecs - at);
+#pragma unroll 4
+        for(uint32_t i = threadIdx.x; i < n; i += 256) {
+            const uint32_t r = (col0 + i) / per, c = col0 + i - r * per;
+            if(!named[row0 + r])
+                reinterpret_cast<uint4 *>(dw + (row0 + r) * ws)[c] = make_uint4(0, 0, 0, 0);
+        }
+        return;
+    }
+    const int lane = threadIdx.x & 31;
+    for(int i = threadIdx.x >> 5; i < kFillRows; i += 8) {
+        const size_t r = block * kFillRows + i;
+        if(r >= vocab || named[r])
+            continue;
+        T *row = dw + r * ws;
+        // up to the first 16-byte boundary, whole words, the rest
+        const size_t head = min(((16 - ((uintptr_t)row & 15)) & 15) / sizeof(T), vecs);
+        const size_t words = (vecs - head) * sizeof(T) / 16, tail = head + words * (16 / sizeof(T));
+        if(lane < head)
+            lm_store(row + lane, 0.0f);
+        for(size_t w = lane; w < words; w += 32)
+            reinterpret_cast<uint4 *>(row + head)[w] = make_uint4(0, 0, 0, 0);
+        if(tail + lane < vecs)
+            lm_store(row + tail + lane, 0.0f);
+    }
+}
+
+// `sums` blocks add up rows of grad_out, the others write zeros; both kinds are
+// spread evenly over the grid, so that the reads of the one run beside the writes
+// of the other.
+template <typename T, int N>
+__global__ void __launch_bounds__(256, 2)
+    sum_kernel(size_t tokens, size_t vocab, size_t vecs, int lanes, size_t sums, size_t slices,
+               const uint32_t *keys, const int *order, const unsigned char *named, const T *dy,
+               size_t ys, float scale, T *dw, size_t ws, int accumulate, float *parts)
+{
+    const size_t block = blockIdx.x * sums / gridDim.x;  // sum blocks before this one
+    if((blockIdx.x + 1) * sums / gridDim.x == block) {
+        fill_rows<T, N>(blockIdx.x - block, vocab, vecs, named, dw, ws);
+        return;
+    }
+    const size_t chunk = block / slices * (256 / lanes) + threadIdx.x / lanes;
+    const size_t c = block % slices * lanes + (threadIdx.x & (lanes - 1));
     const size_t e0 = chunk * kChunk;
     if(e0 >= tokens || c >= vecs)
         return;
@@ -462,47 +343,89 @@ __global__ void __launch_bounds__(256)
     }
 }
 
+// A warp looks at one chunk and 32 vectors of the row, a block at eight chunks.  A
+// run of a few parts is joined by its warp, a long one by the block: each warp
+// adds up every eighth part, then the eight sums are added in order.
+constexpr size_t kWarpParts = 16;
+
 template <typename T, int N>
-__global__ void __launch_bounds__(256)
-    join_rows_kernel(size_t tokens, size_t vocab, size_t vecs, int lanes, const uint32_t *keys,
-                     float scale, T *dw, size_t ws, int accumulate, const float *parts)
+__global__ void __launch_bounds__(256, 4)
+    join_rows_kernel(size_t tokens, size_t vocab, size_t vecs, size_t slices, const uint32_t *keys,
+                     const int *ends, float scale, T *dw, size_t ws, int accumulate,
+                     const float *parts)
 {
-    const size_t chunk = (size_t)blockIdx.x * (256 / lanes) + threadIdx.x / lanes;
-    const size_t c = (size_t)blockIdx.y * lanes + (threadIdx.x & (lanes - 1));
+    __shared__ size_t last_of[8];
+    __shared__ Vec<float, N> joined[8][32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const size_t chunk0 = blockIdx.x / slices * 8, chunk = chunk0 + warp;
+    const size_t c = blockIdx.x % slices * 32 + lane;
     const size_t e0 = chunk * kChunk, e1 = e0 + kChunk;
-    if(e1 >= tokens || c >= vecs)
-        return;
-    const uint32_t run = keys[e1 - 1];
-    // the run that leaves this chunk, if it began here
-    if(run >= vocab || keys[e1] != run || (e0 > 0 && keys[e0] == run && keys[e0 - 1] == run))
-        return;
-    // the chunk it ends in: the first whose next chunk does not begin with it
-    const size_t chunks = (tokens + kChunk - 1) / kChunk;
-    auto inside = [&](size_t k) { return k + 1 < chunks && keys[(k + 1) * kChunk] == run; };
-    size_t last = chunk + 1, hop = 1;
-    while(inside(last + hop - 1)) {
-        last += hop;
-        hop *= 2;
+    size_t last = 0;  // the chunk that a run ends in which leaves this one and began here
+    uint32_t run = 0;
+    if(e1 < tokens) {
+        run = keys[e1 - 1];
+        const uint32_t next = keys[e1], first = keys[e0];
+        const uint32_t earlier = e0 > 0 ? keys[e0 - 1] : 0xffffffffu;
+        const int end = ends[e1 - 1];
+        if(run < vocab && next == run && !(first == run && earlier == run))
+            last = (size_t)(end - 1) / kChunk;
     }
-    while(hop > 1) {  // inside(last - 1) holds
-        hop /= 2;
-        if(inside(last + hop - 1))
-            last += hop;
-    }
-    float sum[N];
-    reinterpret_cast<const Vec<float, N> *>(parts + ((chunk * 2 + 1) * vecs + c) * N)->get(sum);
-    const float *p = parts + ((chunk + 1) * 2 * vecs + c) * N;
-#pragma unroll 8
-    for(size_t k = chunk + 1; k <= last; k++, p += 2 * vecs * N) {
-        Vec<float, N> v;
-        float f[N];
-        v = *reinterpret_cast<const Vec<float, N> *>(p);
-        v.get(f);
+    auto part = [&](size_t from, size_t k) {  // part k of the run that begins in chunk `from`
+        const size_t slot = (from + k) * 2 + (k ? 0 : 1);
+        return reinterpret_cast<const Vec<float, N> *>(parts)[slot * vecs + c];
+    };
+    auto add_parts = [&](size_t from, size_t k0, size_t n, size_t step, float (&sum)[N]) {
+        for(; k0 < n; k0 += 4 * step) {
+            Vec<float, N> v[4];
 #pragma unroll
-        for(int j = 0; j < N; j++)
-            sum[j] += f[j];
+            for(int i = 0; i < 4; i++)
+                if(k0 + i * step < n)
+                    v[i] = part(from, k0 + i * step);
+#pragma unroll
+            for(int i = 0; i < 4; i++)
+                if(k0 + i * step < n) {
+                    float f[N];
+                    v[i].get(f);
+#pragma unroll
+                    for(int j = 0; j < N; j++)
+                        sum[j] += f[j];
+                }
+        }
+    };
+    if(last && last - chunk < kWarpParts) {
+        if(c < vecs) {
+            float sum[N] = {};
+            add_parts(chunk, 0, last - chunk + 1, 1, sum);
+            write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
+        }
+        last = 0;
     }
-    write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
+    if(lane == 0)
+        last_of[warp] = last;
+    if(!__syncthreads_or(last != 0))
+        return;
+    for(int i = 0; i < 8; i++) {
+        const size_t end = last_of[i], from = chunk0 + i;
+        if(!end)
+            continue;
+        float sum[N] = {};
+        if(c < vecs)
+            add_parts(from, warp, end - from + 1, 8, sum);
+        joined[warp][lane].set(sum);
+        __syncthreads();
+        if(warp == i && c < vecs) {
+#pragma unroll
+            for(int w = 0; w < 8; w++) {
+                float f[N];
+                joined[w][lane].get(f);
+#pragma unroll
+                for(int j = 0; j < N; j++)
+                    sum[j] = w ? sum[j] + f[j] : f[j];
+            }
+            write_row<T, N>(dw + (size_t)run * ws, c, sum, scale, accumulate);
+        }
+        __syncthreads();
+    }
 }
 
 // ---------------------------------------------------------------- host side
@@ -510,10 +433,13 @@ __global__ void __launch_bounds__(256)
 // Threads that share a row of `vecs` vectors with `each` of them per thread.
 int lanes_of(size_t vecs, size_t each)
 {
-    int lanes = 1;
+    size_t lanes = 1;
     while(lanes < 256 && lanes * each < vecs)
         lanes *= 2;
-    return lanes;
+    // not with more than an eighth of the threads idle in the last stretch of a row
+    while(lanes > 32 && (vecs + lanes - 1) / lanes * lanes - vecs > vecs / 8)
+        lanes /= 2;
+    return (int)lanes;
 }
 
 template <typename T, int N>
@@ -529,9 +455,8 @@ int lookup(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide, c
 }
 
 struct Work {
-    size_t blocks;  // of the sort
-    size_t at_keys, at_order, at_keys2, at_order2, at_counts, at_parts, bytes;
-    Work(size_t tokens, size_t dim)
+    size_t at_keys, at_order, at_ends, at_named, at_parts, bytes;
+    Work(size_t tokens, size_t vocab, size_t dim)
     {
         size_t at = 0;
         auto take = [&](size_t n) {
@@ -539,13 +464,10 @@ struct Work {
             at += lm_up(n, 256);
             return here;
         };
-        const bool many = tokens > kOneBlock;
-        blocks = (tokens + kManyItems - 1) / kManyItems;
         at_keys = take(lm_up(tokens, kChunk) * 4);
         at_order = take(lm_up(tokens, kChunk) * 4);
-        at_keys2 = take(many ? lm_up(tokens, kChunk) * 4 : 0);
-        at_order2 = take(many ? lm_up(tokens, kChunk) * 4 : 0);
-        at_counts = take(many ? blocks * kDigits * 4 : 0);
+        at_ends = take(lm_up(tokens, kChunk) * 4);
+        at_named = take(vocab);
         at_parts = take((tokens + kChunk - 1) / kChunk * 2 * dim * 4);
         bytes = at;
     }
@@ -555,55 +477,38 @@ template <typename T, int N>
 int gradient(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide, const void *dy,
              size_t ys, float scale, void *dw, size_t ws, int accumulate, char *work, cudaStream_t st)
 {
-    const Work w(tokens, dim);
+    const Work w(tokens, vocab, dim);
     const size_t vecs = dim / N;
     uint32_t *keys = (uint32_t *)(work + w.at_keys);
-    int *order = (int *)(work + w.at_order);
+    int *order = (int *)(work + w.at_order), *ends = (int *)(work + w.at_ends);
+    unsigned char *named = (unsigned char *)(work + w.at_named);
+    float *parts = (float *)(work + w.at_parts);
     int sms = 0;
-    if(!lm_sms(&sms))
+    if(!lm_sms(&sms) ||
+       cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOrderSmem) !=
+           cudaSuccess)
         return B200OPT_ECUDA;
-    int bits = 0;  // of the largest key, `vocab`
-    while(vocab >> bits)
-        bits++;
-    const unsigned fill = (unsigned)std::min<size_t>(sms, vocab);
-    if(tokens <= kOneBlock) {
-        if(cudaFuncSetAttribute(sort_fill_kernel<T, N>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                kSortSmem) != cudaSuccess)
-            return B200OPT_ECUDA;
-        sort_fill_kernel<T, N><<<1 + (accumulate ? 0 : fill), 1024, kSortSmem, st>>>(
-            (int)tokens, vocab, bits, ids, wide, keys, order, (T *)dw, ws, vecs);
-    } else {
-        uint32_t *from_k = nullptr, *to_k = (uint32_t *)(work + w.at_keys2);
-        int *from_o = nullptr, *to_o = (int *)(work + w.at_order2), *counts = (int *)(work + w.at_counts);
-        const int passes = (bits + 8) / 9, step = (bits + passes - 1) / passes;
-        const unsigned blocks = (unsigned)w.blocks;
-        if(passes & 1)  // the last pass ends in keys, order
-            std::swap(keys, to_k), std::swap(order, to_o);
-        for(int p = 0; p < passes; p++) {
-            const uint32_t mask = (1u << step) - 1;
-            sort_count_kernel<<<blocks, kManyThreads, 0, st>>>(tokens, vocab, ids, wide, from_k, from_o,
-                                                               p * step, mask, counts, (int)blocks);
-            sort_sums_kernel<<<1, 1024, 0, st>>>(counts, (int)blocks * kDigits);
-            sort_move_kernel<<<blocks, kManyThreads, 0, st>>>(tokens, vocab, ids, wide, from_k, from_o,
-                                                              p * step, step, counts, (int)blocks, to_k,
-                                                              to_o);
-            from_k = to_k, from_o = to_o;
-            std::swap(keys, to_k), std::swap(order, to_o);
-        }
-        keys = from_k, order = from_o;
-        if(!accumulate)
-            fill_kernel<T, N><<<fill, 1024, 0, st>>>(tokens, vocab, keys, (T *)dw, ws, vecs);
-    }
-    if(tokens) {
-        const int lanes = lanes_of(vecs, 1);
-        const size_t chunks = (tokens + kChunk - 1) / kChunk, per = 256 / lanes;
-        const dim3 grid((unsigned)((chunks + per - 1) / per), (unsigned)((vecs + lanes - 1) / lanes));
-        float *parts = (float *)(work + w.at_parts);
-        sum_kernel<T, N><<<grid, 256, 0, st>>>(tokens, vocab, vecs, lanes, keys, order, (const T *)dy, ys,
-                                               scale, (T *)dw, ws, accumulate, parts);
-        if(chunks > 1)
-            join_rows_kernel<T, N><<<grid, 256, 0, st>>>(tokens, vocab, vecs, lanes, keys, scale, (T *)dw,
-                                                         ws, accumulate, parts);
+    // one block an SM, more where a block would get more rows than it has digits for
+    const size_t blocks = std::min(vocab, std::max<size_t>(sms, (vocab + kDigits - 1) / kDigits));
+    order_kernel<<<(unsigned)blocks, kOrderThreads, kOrderSmem, st>>>(tokens, vocab, ids, wide, keys, order, ends,
+                                                             named);
+    const int lanes = lanes_of(vecs, 1);
+    const size_t chunks = (tokens + kChunk - 1) / kChunk, per = 256 / lanes;
+    const size_t groups = (chunks + per - 1) / per, slices = (vecs + lanes - 1) / lanes;
+    const size_t fills = accumulate ? 0
+                         : N > 1    ? (vocab * vecs + kFill - 1) / kFill
+                                    : (vocab + kFillRows - 1) / kFillRows;
+    if(groups * slices + fills > 0x7fffffff)
+        return B200OPT_ETOOBIG;
+    sum_kernel<T, N><<<(unsigned)(groups * slices + fills), 256, 0, st>>>(
+        tokens, vocab, vecs, lanes, groups * slices, slices, keys, order, named, (const T *)dy, ys, scale,
+        (T *)dw, ws, accumulate, parts);
+    if(chunks > 1) {
+        const size_t cuts = (vecs + 31) / 32;
+        if((chunks + 7) / 8 * cuts > 0x7fffffff)
+            return B200OPT_ETOOBIG;
+        join_rows_kernel<T, N><<<(unsigned)((chunks + 7) / 8 * cuts), 256, 0, st>>>(
+            tokens, vocab, vecs, cuts, keys, ends, scale, (T *)dw, ws, accumulate, parts);
     }
     return lm_launched();
 }
@@ -642,7 +547,7 @@ int b200opt_embedding_bwd_workspace(size_t tokens, size_t vocab, size_t dim, siz
         return B200OPT_EINVAL;
     if(tokens > B200OPT_LM_MAX || vocab > B200OPT_LM_MAX || dim > B200OPT_LM_MAX)
         return B200OPT_ETOOBIG;
-    *bytes = Work(tokens, dim).bytes;
+    *bytes = tokens || vocab ? Work(tokens, vocab, dim).bytes : 0;
     return B200OPT_OK;
 }
 

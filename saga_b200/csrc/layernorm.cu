@@ -7,13 +7,15 @@
 namespace b200 {
 namespace {
 
-constexpr int kThreads = 256;
+// threads of a block: eight rows of a warp each, or one row of WARPS warps
+__host__ __device__ constexpr int threads_of(int warps) { return warps == 1 ? 256 : 32 * warps; }
+__host__ __device__ constexpr int rows_of(int warps) { return warps == 1 ? 8 : 1; }
 constexpr int kMaxParts = 444;  // blocks of the gradient kernel: three on each of 148 SMs
 
 // Sums over the threads that share a row: a warp, or the block.  `turn` alternates
 // between two sets of slots, so that one barrier a sum is enough.
 template <int WARPS, int K>
-__device__ __forceinline__ void row_sums(float (&v)[K], float (*slots)[8][K], int &turn)
+__device__ __forceinline__ void row_sums(float (&v)[K], float (*slots)[16][K], int &turn)
 {
 #pragma unroll
     for(int k = 0; k < K; k++)
@@ -51,14 +53,14 @@ __device__ __forceinline__ void load_param(const P *p, size_t c, float fill, flo
 // vectors of N elements a thread: it is read once, and the variance is taken
 // around the mean in a second pass over the registers.
 template <typename T, typename P, int N, int NV, int WARPS>
-__global__ void __launch_bounds__(kThreads)
+__global__ void __launch_bounds__(threads_of(WARPS))
     layernorm_fwd_kernel(size_t rows, size_t dim, const T *x, size_t xs, const P *gamma, const P *beta,
                          float eps, T *y, size_t ys, float *mean, float *rstd)
 {
-    __shared__ float slots[2][8][1];
+    __shared__ float slots[2][16][1];
     int turn = 0;
     constexpr int L = 32 * WARPS;
-    const size_t r = (size_t)blockIdx.x * (8 / WARPS) + threadIdx.x / L;
+    const size_t r = (size_t)blockIdx.x * rows_of(WARPS) + threadIdx.x / L;
     const int l = threadIdx.x % L, vecs = (int)(dim / N);
     if(WARPS == 1 && r >= rows)
         return;
@@ -149,24 +151,36 @@ __global__ void __launch_bounds__(1024)
 // thread keeps the parameters' sums of its own columns in registers and leaves
 // them in `parts` at the end, for params_kernel to join in a fixed order.  The
 // next row's vectors are loaded before the present row's sums are waited for.
+#ifndef B8
+#define B8 2
+#endif
 #ifndef B16
 #define B16 2
 #endif
-#ifndef FWDW
-#define FWDW 16
+#ifndef BW
+#define BW 8
 #endif
-constexpr int bwd_blocks(int columns) { return columns <= 8 ? 3 : columns <= 16 ? B16 : 1; }
+#ifndef FW1
+#define FW1 4
+#endif
+#ifndef FW
+#define FW 4
+#endif
+#ifndef FNV
+#define FNV 2
+#endif
+__host__ __device__ constexpr int bwd_blocks(int columns) { return columns <= 8 ? B8 : columns <= 16 ? B16 : 1; }
 
 template <typename T, typename P, int N, int NV, int WARPS>
-__global__ void __launch_bounds__(kThreads, bwd_blocks(N * NV))
+__global__ void __launch_bounds__(threads_of(WARPS), bwd_blocks(N * NV))
     layernorm_bwd_kernel(size_t rows, size_t dim, const T *dy, size_t ys, const T *x, size_t xs,
                          const P *gamma, const float *mean, const float *rstd, T *dx, size_t dxs,
                          float *parts)
 {
-    __shared__ float slots[2][8][2];
+    __shared__ float slots[2][16][2];
     __shared__ float joined[WARPS == 1 ? 2 * 32 * NV * N : 1];
     int turn = 0;
-    constexpr int L = 32 * WARPS, R = 8 / WARPS;
+    constexpr int L = 32 * WARPS, R = rows_of(WARPS);
     const int l = threadIdx.x % L, vecs = (int)(dim / N);
     const size_t step = (size_t)gridDim.x * R;
     float sg[NV][N], sb[NV][N];
@@ -199,7 +213,7 @@ __global__ void __launch_bounds__(kThreads, bwd_blocks(N * NV))
         Vec<T, N> nx[NV], ny[NV];
         float nmu = 0.0f, nrs = 0.0f;
         fetch(r + step, nx, ny, nmu, nrs);
-        float s[2] = {0.0f, 0.0f};
+        float s[2] = {0.0f, 0.0f}, xh[NV][N], d[NV][N];
 #pragma unroll
         for(int i = 0; i < NV; i++)
             if(l + i * L < vecs) {
@@ -209,11 +223,12 @@ __global__ void __launch_bounds__(kThreads, bwd_blocks(N * NV))
                 load_param<P, N>(gamma, l + i * L, 1.0f, g);
 #pragma unroll
                 for(int j = 0; j < N; j++) {
-                    const float xh = (fx[j] - mu) * rs, d = fy[j] * g[j];
-                    sg[i][j] = fmaf(fy[j], xh, sg[i][j]);
+                    xh[i][j] = (fx[j] - mu) * rs;
+                    d[i][j] = fy[j] * g[j];
+                    sg[i][j] = fmaf(fy[j], xh[i][j], sg[i][j]);
                     sb[i][j] += fy[j];
-                    s[0] += d;
-                    s[1] = fmaf(d, xh, s[1]);
+                    s[0] += d[i][j];
+                    s[1] = fmaf(d[i][j], xh[i][j], s[1]);
                 }
             }
         if(dx) {
@@ -223,17 +238,12 @@ __global__ void __launch_bounds__(kThreads, bwd_blocks(N * NV))
 #pragma unroll
             for(int i = 0; i < NV; i++)
                 if(l + i * L < vecs) {
-                    float fx[N], fy[N], g[N];
-                    vx[i].get(fx);
-                    vy[i].get(fy);
-                    load_param<P, N>(gamma, l + i * L, 1.0f, g);
+                    float f[N];
 #pragma unroll
-                    for(int j = 0; j < N; j++) {
-                        const float xh = (fx[j] - mu) * rs;
-                        fx[j] = rs * (fmaf(fy[j], g[j], -a) - xh * b);
-                    }
+                    for(int j = 0; j < N; j++)
+                        f[j] = rs * fmaf(-b, xh[i][j], d[i][j] - a);
                     Vec<T, N> o;
-                    o.set(fx);
+                    o.set(f);
                     to[l + i * L] = o;
                 }
         }
@@ -262,7 +272,7 @@ __global__ void __launch_bounds__(kThreads, bwd_blocks(N * NV))
                         }
             __syncthreads();
         }
-        for(int d = threadIdx.x; d < (int)dim; d += kThreads) {
+        for(int d = threadIdx.x; d < (int)dim; d += 256) {
             pg[d] = joined[d];
             pb[d] = joined[32 * NV * N + d];
         }
@@ -361,30 +371,17 @@ struct Args {
     cudaStream_t st;
 };
 
-// Vectors a thread holds: the smallest power of two up to MAX that covers a row
-// with a warp, else with the block; 0 threads' worth: the long kernels.
-template <int N, int NV, int MAX, typename F>
+// Calls f with the smallest number of vectors a thread, NV times a power of two up
+// to MAX, with which WARPS warps hold a row.
+template <int WARPS, int NV, int MAX, typename F>
 bool pick(size_t vecs, F &&f)
 {
-    if(vecs <= (size_t)32 * NV) {
-        f(std::integral_constant<int, NV>(), std::integral_constant<int, 1>());
+    if(vecs <= (size_t)32 * WARPS * NV) {
+        f(std::integral_constant<int, NV>(), std::integral_constant<int, WARPS>());
         return true;
     }
-    if constexpr(NV < MAX) {
-        return pick<N, 2 * NV, MAX>(vecs, f);
-    } else {
-        return false;
-    }
-}
-template <int N, int NV, int MAX, typename F>
-bool pick_block(size_t vecs, F &&f)
-{
-    if(vecs <= (size_t)256 * NV) {
-        f(std::integral_constant<int, NV>(), std::integral_constant<int, 8>());
-        return true;
-    }
-    if constexpr(NV < MAX) {
-        return pick_block<N, 2 * NV, MAX>(vecs, f);
+    if constexpr(2 * NV <= MAX) {
+        return pick<WARPS, 2 * NV, MAX>(vecs, f);
     } else {
         return false;
     }
@@ -395,13 +392,13 @@ int fwd_with(const Args &a)
 {
     auto launch = [&](auto nv, auto warps) {
         constexpr int NV = decltype(nv)::value, W = decltype(warps)::value;
-        const size_t blocks = (a.rows + 8 / W - 1) / (8 / W);
-        layernorm_fwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, kThreads, 0, a.st>>>(
+        const size_t blocks = (a.rows + rows_of(W) - 1) / rows_of(W);
+        layernorm_fwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, threads_of(W), 0, a.st>>>(
             a.rows, a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y,
             a.ys, a.mean, a.rstd);
     };
     const size_t vecs = a.dim / N;
-    if(!pick<N, 1, FWDW>(vecs, launch) && !pick_block<N, FWDW/4, 16>(vecs, launch))
+    if(!pick<1, 1, FW1>(vecs, launch) && !pick<FW, FNV, 64/FW>(vecs, launch) && !pick<16, 8, 16>(vecs, launch))
         layernorm_fwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
             a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y, a.ys,
             a.mean, a.rstd);
@@ -416,15 +413,15 @@ int bwd_with(const Args &a)
     size_t blocks = 0;
     auto launch = [&](auto nv, auto warps) {
         constexpr int NV = decltype(nv)::value, W = decltype(warps)::value;
-        blocks = std::min<size_t>((a.rows + 8 / W - 1) / (8 / W), 148 * bwd_blocks(N * NV));
+        blocks = std::min<size_t>((a.rows + rows_of(W) - 1) / rows_of(W), 148 * bwd_blocks(N * NV));
         if(blocks)
-            layernorm_bwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, kThreads, 0, a.st>>>(
+            layernorm_bwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, threads_of(W), 0, a.st>>>(
                 a.rows, a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma,
                 a.mean_in, a.rstd_in, (T *)a.dx, a.dxs, parts);
     };
     const size_t vecs = a.dim / N;
     constexpr int kWarp = N == 1 ? 16 : 16 / N * 2, kBlock = 32 / N;
-    if(!pick<N, 1, kWarp>(vecs, launch) && !pick_block<N, kWarp / 4, kBlock>(vecs, launch)) {
+    if(!pick<1, 1, kWarp>(vecs, launch) && !pick<BW, kWarp / 4 * 8 / BW ? kWarp / 4 * 8 / BW : 1, kBlock>(vecs, launch)) {
         if(a.dx && a.rows)
             layernorm_bwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
                 a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma, a.mean_in,
