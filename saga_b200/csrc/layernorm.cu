@@ -151,25 +151,7 @@ __global__ void __launch_bounds__(1024)
 // thread keeps the parameters' sums of its own columns in registers and leaves
 // them in `parts` at the end, for params_kernel to join in a fixed order.  The
 // next row's vectors are loaded before the present row's sums are waited for.
-#ifndef B8
-#define B8 2
-#endif
-#ifndef B16
-#define B16 2
-#endif
-#ifndef BW
-#define BW 8
-#endif
-#ifndef FW1
-#define FW1 4
-#endif
-#ifndef FW
-#define FW 4
-#endif
-#ifndef FNV
-#define FNV 2
-#endif
-__host__ __device__ constexpr int bwd_blocks(int columns) { return columns <= 8 ? B8 : columns <= 16 ? B16 : 1; }
+__host__ __device__ constexpr int bwd_blocks(int columns) { return columns <= 16 ? 2 : 1; }
 
 template <typename T, typename P, int N, int NV, int WARPS>
 __global__ void __launch_bounds__(threads_of(WARPS), bwd_blocks(N * NV))
@@ -398,7 +380,7 @@ int fwd_with(const Args &a)
             a.ys, a.mean, a.rstd);
     };
     const size_t vecs = a.dim / N;
-    if(!pick<1, 1, FW1>(vecs, launch) && !pick<FW, FNV, 64/FW>(vecs, launch) && !pick<16, 8, 16>(vecs, launch))
+    if(!pick<1, 1, 4>(vecs, launch) && !pick<4, 2, 16>(vecs, launch) && !pick<16, 8, 16>(vecs, launch))
         layernorm_fwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
             a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y, a.ys,
             a.mean, a.rstd);
@@ -421,7 +403,7 @@ int bwd_with(const Args &a)
     };
     const size_t vecs = a.dim / N;
     constexpr int kWarp = N == 1 ? 16 : 16 / N * 2, kBlock = 32 / N;
-    if(!pick<1, 1, kWarp>(vecs, launch) && !pick<BW, kWarp / 4 * 8 / BW ? kWarp / 4 * 8 / BW : 1, kBlock>(vecs, launch)) {
+    if(!pick<1, 1, kWarp>(vecs, launch) && !pick<8, kWarp / 4, kBlock>(vecs, launch)) {
         if(a.dx && a.rows)
             layernorm_bwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
                 a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma, a.mean_in,
