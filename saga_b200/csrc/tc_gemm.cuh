@@ -35,7 +35,8 @@ constexpr int kTcK = 64;        // k per stage: 128 bytes, the swizzle's span
 constexpr int kTcStages = 6;
 constexpr int kTcOperand = kTcHalf * kTcK * 2;  // bytes of one operand of a stage in a CTA
 constexpr int kTcThreads = 384;
-constexpr int kTcSmem = kTcStages * 2 * kTcOperand + 1024;
+constexpr int kTcStaging = 4096;  // bytes an epilogue warp turns its columns around in
+constexpr int kTcSmem = kTcStages * 2 * kTcOperand + 8 * kTcStaging + 1024;
 constexpr unsigned long long kTcWaitNs = 2000000000ull;
 
 struct TcShape {
@@ -193,14 +194,47 @@ __device__ __forceinline__ void tmem_load(uint32_t addr, float (&v)[32])
           "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
           "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
         : "r"(addr));
-    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
 }
+
+// Waits for the loads issued so far.  The registers pass through it, so that no use
+// of them can be moved in front of the wait.
+__device__ __forceinline__ void tmem_wait(float (&v)[32])
+{
+    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+    for(int j = 0; j < 32; j++)
+        asm volatile("" : "+f"(v[j]));
+}
+
+// ------------------------------------------------------------- epilogue's turn
+//
+// A thread has 32 columns of one row; written straight to memory that would be a
+// scattered 16 bytes a thread.  A warp therefore passes its 32 rows through shared
+// memory (16-byte words, their places permuted so that neither side meets a bank
+// twice) and comes out with rows side by side: `put` takes word w of this thread's
+// row, `get` gives a word of row `row()`, step by step.
+template <int WORDS>  // 16-byte words of a row: 4 (fp16) or 8 (fp32)
+struct Turn {
+    char *buf;
+    int lane;
+    static constexpr int kSteps = WORDS;  // 32 / WORDS rows a step
+    __device__ __forceinline__ uint4 *at(int row, int word) const
+    {
+        const int key = WORDS == 8 ? row & 7 : (row >> 1) & 3;
+        return reinterpret_cast<uint4 *>(buf + row * (WORDS * 16) + ((word ^ key) << 4));
+    }
+    __device__ __forceinline__ void put(int word, uint4 v) const { *at(lane, word) = v; }
+    __device__ __forceinline__ int row(int step) const { return step * (32 / WORDS) + lane / WORDS; }
+    __device__ __forceinline__ int word() const { return lane % WORDS; }
+    __device__ __forceinline__ uint4 get(int step) const { return *at(row(step), word()); }
+};
 
 // ------------------------------------------------------------------- kernel
 
-// Which tile is the i-th: groups of `group` m tiles, within a group n by n.
+// Which tile is the i-th: groups of `group` m tiles, within a group n by n.  The
+// host has made sure that their number fits 31 bits.
 struct TcTiles {
-    int mt, nt, group, splits, kblocks;
+    uint32_t mt, nt, group, splits, kblocks;
     __device__ __forceinline__ TcTiles(const TcShape &s)
     {
         const int c = s.dyn_m || s.dyn_k ? max(*s.count, 1) : 0;
@@ -211,27 +245,30 @@ struct TcTiles {
         group = s.group;
         splits = s.splits;
     }
-    __device__ __forceinline__ long long count() const { return (long long)mt * nt * splits; }
-    __device__ __forceinline__ void at(long long i, int &m, int &n, int &part, int &k0, int &k1) const
+    __device__ __forceinline__ uint32_t count() const { return mt * nt * splits; }
+    __device__ __forceinline__ void at(uint32_t i, int &m, int &n, int &part, int &k0, int &k1) const
     {
-        const long long tiles = (long long)mt * nt;
-        part = (int)(i / tiles);
-        const long long t = i - part * tiles;
-        const long long per = (long long)group * nt;
-        const int g = (int)(t / per);
-        const int rows = min(group, mt - g * group);
-        const long long r = t - g * per;
-        m = g * group + (int)(r % rows);
-        n = (int)(r / rows);
-        k0 = (int)((long long)kblocks * part / splits);
-        k1 = (int)((long long)kblocks * (part + 1) / splits);
+        const uint32_t tiles = mt * nt;
+        uint32_t t = i;
+        part = 0, k0 = 0, k1 = (int)kblocks;
+        if(splits > 1) {
+            part = (int)(i / tiles);
+            t = i - part * tiles;
+            k0 = (int)((uint64_t)kblocks * part / splits);
+            k1 = (int)((uint64_t)kblocks * (part + 1) / splits);
+        }
+        const uint32_t per = group * nt, g = t / per;
+        const uint32_t rows = min(group, mt - g * group), r = t - g * per, c = r / rows;
+        m = (int)(g * group + r - c * rows);
+        n = (int)c;
     }
 };
 
-// Epi: the epilogue.  begin(row, col, part) gives a thread's state for its row
-// of a tile and the 128 columns from col; columns(state, row, col, v) gets 32
-// columns at a time; end(state, row, col) closes them.  Rows and columns beyond
-// the matrix come too and are for the epilogue to leave out.
+// Epi: the epilogue.  common() is what all tiles share; begin(common, row, col,
+// part) gives a thread's state for its row of a tile and the 128 columns from col;
+// columns(common, state, row, col, v, staging) gets 32 columns at a time, all lanes
+// of a warp together; end(state, row, col) closes them.  Rows and columns beyond the matrix come too and are for the epilogue to
+// leave out.
 template <bool A_MN, bool B_MN, typename Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     tc_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
@@ -272,14 +309,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
 
     const TcTiles tiles(shape);
-    const long long total = tiles.count();
-    const int pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
+    const uint32_t total = tiles.count(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if(warp == 0 && lane == 0) {
         int stage = 0;
         uint32_t phase = 0;
         bool ok = true;
-        for(long long i = pair; ok && i < total; i += pairs) {
+        for(uint32_t i = pair; ok && i < total; i += pairs) {
             int m, n, part, k0, k1;
             tiles.at(i, m, n, part, k0, k1);
             const int am = m * kTcTile + (int)rank * kTcHalf, bn = n * kTcTile + (int)rank * kTcHalf;
@@ -320,7 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
-        for(long long i = pair; ok && i < total; i += pairs) {
+        for(uint32_t i = pair; ok && i < total; i += pairs) {
             int m, n, part, k0, k1;
             tiles.at(i, m, n, part, k0, k1);
             if(!(ok = mbar_wait(smem_u32(&acc_empty[acc]), acc_phase ^ 1, dead)))
@@ -353,31 +389,39 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         }
     } else if(warp >= 4) {
         const int quad = warp & 3, side = (warp - 4) >> 2;
+        char *staging = smem_raw + (base - smem_u32(smem_raw)) + kTcStages * 2 * kTcOperand +
+                        (warp - 4) * kTcStaging;
+        const auto common = epi.common();
         int acc = 0;
         uint32_t acc_phase = 0;
         bool ok = true;
-        for(long long i = pair; i < total; i += pairs) {
+        for(uint32_t i = pair; i < total; i += pairs) {
             int m, n, part, k0, k1;
             tiles.at(i, m, n, part, k0, k1);
-            ok = ok && mbar_wait(smem_u32(&acc_full[acc]), acc_phase, dead);
-            ok = __all_sync(0xffffffffu, ok);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
             const int row = m * kTcTile + (int)rank * kTcHalf + quad * 32 + lane;
             const int col = n * kTcTile + side * kTcHalf;
             const uint32_t from =
                 tmem + ((uint32_t)(quad * 32) << 16) + acc * kTcTile + side * kTcHalf;
-            auto state = epi.begin(row, col, part);
-#pragma unroll 1
-            for(int c = 0; c < kTcHalf; c += 32) {
-                float v[32];
-                if(ok && k1 > k0) {
-                    tmem_load(from + c, v);
-                } else {  // a part without a share of k, or a wait that ran out
+            auto state = epi.begin(common, row, col, part);  // its loads run during the wait
+            ok = ok && mbar_wait(smem_u32(&acc_full[acc]), acc_phase, dead);
+            ok = __all_sync(0xffffffffu, ok);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            float v[2][32];
+            const bool none = !ok || k1 == k0;  // a wait that ran out, or no share of k
+            if(!none)
+                tmem_load(from, v[0]);
+#pragma unroll
+            for(int c = 0; c < kTcHalf / 32; c++) {  // the next columns load meanwhile
+                if(none) {
 #pragma unroll
                     for(int j = 0; j < 32; j++)
-                        v[j] = ok ? 0.0f : __int_as_float(0x7fffffff);
+                        v[c & 1][j] = ok ? 0.0f : __int_as_float(0x7fffffff);
+                } else {
+                    tmem_wait(v[c & 1]);
+                    if(c + 1 < kTcHalf / 32)
+                        tmem_load(from + (c + 1) * 32, v[(c + 1) & 1]);
                 }
-                epi.columns(state, row, col + c, v);
+                epi.columns(common, state, row, col + c * 32, v[c & 1], staging);
             }
             epi.end(state, row, col);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
@@ -442,9 +486,10 @@ bool tc_launch(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, con
     auto *kernel = tc_gemm_kernel<A_MN, B_MN, Epi>;
     if(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem) != cudaSuccess)
         return false;
-    const long long tiles = (long long)((s.m + kTcTile - 1) / kTcTile) *
-                            ((s.n + kTcTile - 1) / kTcTile) * s.splits;
+    const long long tiles = (s.m + kTcTile - 1ll) / kTcTile * ((s.n + kTcTile - 1ll) / kTcTile) * s.splits;
     const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
+    if(tiles > 0x7fffffff)
+        return false;
     kernel<<<(unsigned)(2 * pairs), kTcThreads, kTcSmem, st>>>(a, b, s, epi);
     return true;
 }

@@ -32,15 +32,22 @@ struct StatsEpilogue {
     int wide;
     float2 *part;
     float *zt;
+    unsigned *done;  // of loss_kernel's blocks
     struct State {
         float top, sum;
         int at;
     };
-    __device__ __forceinline__ State begin(int row, int, int) const
+    __device__ __forceinline__ int common() const
+    {
+        if(blockIdx.x == 0 && threadIdx.x == kTcThreads - 1)
+            *done = 0;
+        return 0;
+    }
+    __device__ __forceinline__ State begin(int, int row, int, int) const
     {
         return {-INFINITY, 0.0f, row < T ? lm_index_at(y, wide, row, V) : -1};
     }
-    __device__ __forceinline__ void columns(State &s, int row, int col, float (&v)[32]) const
+    __device__ __forceinline__ void columns(int, State &s, int row, int col, float (&v)[32], char *) const
     {
         if(col >= V)
             return;
@@ -57,17 +64,17 @@ struct StatsEpilogue {
             for(int j = 0; j < 32; j++)
                 v[j] = j < V - col ? v[j] : -INFINITY;
         }
-        float top = v[0];
+        float most[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-        for(int j = 1; j < 32; j++)
-            top = fmaxf(top, v[j]);
-        top = fmaxf(s.top, top * kLog2e);
-        float sum = s.sum * exp2_fast(s.top - top);
+        for(int j = 4; j < 32; j++)
+            most[j & 3] = fmaxf(most[j & 3], v[j]);
+        const float top = fmaxf(s.top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * kLog2e);
+        float sum[4] = {s.sum * exp2_fast(s.top - top), 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for(int j = 0; j < 32; j++)
-            sum += exp2_fast(fmaf(v[j], kLog2e, -top));
+            sum[j & 3] += exp2_fast(fmaf(v[j], kLog2e, -top));
         s.top = top;
-        s.sum = sum;
+        s.sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
     __device__ __forceinline__ void end(const State &s, int row, int col) const
     {
@@ -76,16 +83,19 @@ struct StatsEpilogue {
     }
 };
 
-// Joins the parts of 32 rows: 16 threads a row, then a tree.
-__global__ void __launch_bounds__(512) loss_kernel(int T, int V, int parts, const float2 *part,
-                                                   const float *zt, const void *y, int wide,
-                                                   float *loss, float *lse)
+// Joins the parts of 32 rows: 16 threads a row, then a tree.  The block that
+// finishes last adds up the blocks' sums of losses, in their order.
+__global__ void __launch_bounds__(512)
+    loss_kernel(int T, int V, int parts, const float2 *part, const float *zt, const void *y, int wide,
+                float *loss, float *lse, float2 *block_sums, unsigned *done, float *stats)
 {
     __shared__ float2 red[16][33];
+    __shared__ bool last;
     const int x = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int t = blockIdx.x * 32 + x;
     float top = -INFINITY, sum = 0.0f;
     if(t < T)
+#pragma unroll 4
         for(int i = w; i < parts; i += 16) {
             const float2 p = part[(size_t)i * T + t];
             const float m = fmaxf(top, p.x);
@@ -94,36 +104,56 @@ __global__ void __launch_bounds__(512) loss_kernel(int T, int V, int parts, cons
         }
     red[w][x] = make_float2(top, sum);
     __syncthreads();
-    if(w || t >= T)
+    if(w == 0) {
+        float mine = 0.0f, counted = 0.0f;
+        if(t < T) {
+            const int used = min(16, parts);
+            for(int i = 1; i < used; i++)
+                top = fmaxf(top, red[i][x].x);
+            sum = 0.0f;
+            for(int i = 0; i < used; i++)
+                sum += red[i][x].y * exp2_fast(red[i][x].x - top);
+            const float l = (top + log2f(sum)) * kLn2;
+            lse[t] = l;
+            if(lm_index_at(y, wide, t, V) >= 0) {
+                mine = l - zt[t];
+                counted = 1.0f;
+            }
+            loss[t] = mine;
+        }
+        mine = warp_sum(mine);
+        counted = warp_sum(counted);
+        if(x == 0 && stats) {
+            block_sums[blockIdx.x] = make_float2(mine, counted);
+            __threadfence();
+            last = atomicAdd(done, 1) == gridDim.x - 1;
+        }
+    }
+    if(!stats)
         return;
-    const int used = min(16, parts);
-    for(int i = 1; i < used; i++)
-        top = fmaxf(top, red[i][x].x);
-    sum = 0.0f;
-    for(int i = 0; i < used; i++)
-        sum += red[i][x].y * exp2_fast(red[i][x].x - top);
-    const float l = (top + log2f(sum)) * kLn2;
-    lse[t] = l;
-    loss[t] = lm_index_at(y, wide, t, V) >= 0 ? l - zt[t] : 0.0f;
+    __syncthreads();
+    if(!last)
+        return;
+    __threadfence();
+    float mine = 0.0f;
+    int counted = 0;
+    for(int i = threadIdx.x; i < (int)gridDim.x; i += 512) {
+        const float2 p = __ldcg(block_sums + i);
+        mine += p.x;
+        counted += (int)p.y;
+    }
+    float *slots = &red[0][0].x;
+    mine = block_sum(mine, slots);
+    // whole numbers in two parts, each of which fp32 holds exactly
+    const float hi = block_sum((float)(counted >> 12), slots);
+    const float lo = block_sum((float)(counted & 4095), slots);
+    if(threadIdx.x == 0) {
+        stats[0] = mine;
+        stats[1] = hi * 4096.0f + lo;
+    }
 }
 
-__global__ void __launch_bounds__(1024) stats_kernel(int T, int V, const float *loss, const void *y,
-                                                     int wide, float *stats)
-{
-    __shared__ float red[32];
-    float s = 0.0f;
-    int n = 0;
-    for(int t = threadIdx.x; t < T; t += 1024) {
-        s += loss[t];
-        n += lm_index_at(y, wide, t, V) >= 0;
-    }
-    s = block_sum(s, red);
-    const float hi = block_sum((float)(n >> 12), red), lo = block_sum((float)(n & 4095), red);
-    if(threadIdx.x == 0) {
-        stats[0] = s;
-        stats[1] = hi * 4096.0f + lo;  // each sum of whole numbers is exact
-    }
-}
+__global__ void no_stats_kernel(float *stats) { stats[0] = stats[1] = 0.0f; }
 
 // ----------------------------------------------------------------- gradient
 
@@ -131,7 +161,7 @@ __global__ void __launch_bounds__(1024) stats_kernel(int T, int V, const float *
 // `hidden`, their lse and target, and where they came from.  Ignored tokens then
 // cost nothing in the three products, and what stands in their rows (NaN too)
 // cannot reach the gradient; their rows of grad_hidden are written as zeros
-// here.  Behind the last row, zeros up to the next tile.
+// here.  Behind the last row, zeros up to the next stage of k.
 __global__ void __launch_bounds__(256)
     compact_kernel(int T, int V, int D, int rows_per_block, const __half *x, size_t xs, const void *y,
                    int wide, const float *lse, __half *xc, float *lsec, int *targetc, int *from,
@@ -160,9 +190,10 @@ __global__ void __launch_bounds__(256)
     const int total = all_sum, vecs = D / 8;
     if(blockIdx.x == 0 && tid == 0)
         *count = total;
-    for(int r = r0; r < min(r0 + rows_per_block, T); r += 32) {
+    const int r1 = min(r0 + rows_per_block, T);
+    for(int r = r0; r < r1; r += 32) {
         if(warp == 0) {
-            const int t = r + lane, id = t < T ? lm_index_at(y, wide, t, V) : -1;
+            const int t = r + lane, id = t < r1 ? lm_index_at(y, wide, t, V) : -1;
             const unsigned mask = __ballot_sync(0xffffffffu, id >= 0);
             const int at = next + __popc(mask & ((1u << lane) - 1));
             place[lane] = id >= 0 ? at : -1;
@@ -178,7 +209,7 @@ __global__ void __launch_bounds__(256)
             seen += place[j] >= 0;
         for(int j = warp; j < 32; j += 8) {
             const int t = r + j, at = place[j];
-            if(t >= T)
+            if(t >= r1)
                 continue;
             if(at >= 0) {
                 const uint4 *s = reinterpret_cast<const uint4 *>(x + (size_t)t * xs);
@@ -194,7 +225,8 @@ __global__ void __launch_bounds__(256)
         next += seen;
         __syncthreads();
     }
-    const int pad = max((total + kTcTile - 1) / kTcTile, 1) * kTcTile;
+    // grad_weight's product runs over whole stages of tokens
+    const int pad = max((total + kTcK - 1) / kTcK, 1) * kTcK;
     for(int r = total + blockIdx.x * 8 + warp; r < pad; r += gridDim.x * 8) {
         uint4 *d = reinterpret_cast<uint4 *>(xc + (size_t)r * D);
         for(int c = lane; c < vecs; c += 32)
@@ -215,18 +247,17 @@ struct DzEpilogue {
         int at;
         bool live;
     };
-    __device__ __forceinline__ State begin(int row, int, int) const
+    __device__ __forceinline__ int common() const { return *count; }
+    __device__ __forceinline__ State begin(int tokens, int row, int, int) const
     {
-        const bool live = row < *count;
+        const bool live = row < tokens;
         return {live ? fmaf(lse[row], kLog2e, -15.0f) : 0.0f, live ? target[row] - first : -1, live};
     }
-    __device__ __forceinline__ void columns(State &s, int row, int col, float (&v)[32]) const
+    __device__ __forceinline__ void columns(int, State &s, int row, int col, float (&v)[32], char *buf) const
     {
         if((size_t)col >= stride)
             return;
         const int at = s.at - col;
-        uint4 out[4];
-        __half2 *h = reinterpret_cast<__half2 *>(out);
 #pragma unroll
         for(int j = 0; j < 32; j++)
             v[j] = s.live ? exp2_fast(fmaf(v[j], kLog2e, -s.c)) : 0.0f;
@@ -235,13 +266,22 @@ struct DzEpilogue {
             for(int j = 0; j < 32; j++)
                 v[j] -= at == j ? kLift : 0.0f;
         }
+        const Turn<4> turn = {buf, (int)(threadIdx.x & 31)};
+        __syncwarp();
 #pragma unroll
-        for(int j = 0; j < 16; j++)
-            h[j] = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
-        uint4 *to = reinterpret_cast<uint4 *>(dz + (size_t)row * stride + col);
+        for(int w = 0; w < 4; w++) {
+            uint4 bits;
+            __half2 *h = reinterpret_cast<__half2 *>(&bits);
 #pragma unroll
-        for(int j = 0; j < 4; j++)
-            to[j] = out[j];
+            for(int i = 0; i < 4; i++)
+                h[i] = __floats2half2_rn(v[8 * w + 2 * i], v[8 * w + 2 * i + 1]);
+            turn.put(w, bits);
+        }
+        __syncwarp();
+        __half *to = dz + (size_t)(row - turn.lane) * stride + col + turn.word() * 8;
+#pragma unroll
+        for(int i = 0; i < turn.kSteps; i++)
+            *reinterpret_cast<uint4 *>(to + turn.row(i) * stride) = turn.get(i);
     }
     __device__ __forceinline__ void end(const State &, int, int) const {}
 };
@@ -271,52 +311,99 @@ struct OutEpilogue {
     int accumulate;
     Factor factor;
     struct State {
-        float *sum;
-        __half *out;
-        float f;
-        bool live;
+        long long row;
+        float *sums;    // of this part
+        int to;         // row of the result; -1: none
     };
-    __device__ __forceinline__ State begin(int row, int, int part) const
+    struct Common {
+        int live;
+        float f;
+    };
+    __device__ __forceinline__ Common common() const
     {
-        State s;
-        s.live = row < (count ? *count : m);
-        s.sum = sum ? sum + part * part_stride + (size_t)row * n : nullptr;
-        s.out = out && s.live ? out + (size_t)(rows ? rows[row] : row) * stride : nullptr;
-        s.f = out ? factor.get() : 0.0f;
-        return s;
+        return {count ? *count : m, out ? factor.get() : 0.0f};
     }
-    __device__ __forceinline__ void columns(State &s, int, int col, float (&v)[32]) const
+    __device__ __forceinline__ State begin(const Common &g, int row, int, int part) const
     {
-        if(!s.live)
+        return {(long long)row, sum ? sum + part * part_stride : nullptr,
+                row < g.live ? (out && rows ? rows[row] : row) : -1};
+    }
+    __device__ __forceinline__ void columns(const Common &g, State &s, int, int col, float (&v)[32], char *buf) const
+    {
+        const int lane = threadIdx.x & 31;
+        if(col >= n)
             return;
+        float *const sums = s.sums;
+        const long long row0 = s.row - lane;
+        if(sums && (add || !out)) {
+            // fp32: what earlier pieces left comes in, or the new sums go out
+            const Turn<8> turn = {buf, lane};
+            const int c = col + turn.word() * 4;
+            __syncwarp();
+            if(add) {
 #pragma unroll
-        for(int j = 0; j < 32; j += 8) {
-            if(col + j >= n)  // n is a multiple of 8
-                return;
-            if(sum && add) {
-                const float4 a = *reinterpret_cast<const float4 *>(s.sum + col + j);
-                const float4 b = *reinterpret_cast<const float4 *>(s.sum + col + j + 4);
-                v[j] += a.x, v[j + 1] += a.y, v[j + 2] += a.z, v[j + 3] += a.w;
-                v[j + 4] += b.x, v[j + 5] += b.y, v[j + 6] += b.z, v[j + 7] += b.w;
+                for(int i = 0; i < turn.kSteps; i++) {
+                    const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i));
+                    if(to >= 0 && c < n)
+                        *turn.at(turn.row(i), turn.word()) =
+                            *reinterpret_cast<const uint4 *>(sums + (row0 + turn.row(i)) * n + c);
+                }
+                __syncwarp();
+#pragma unroll
+                for(int w = 0; w < 8; w++) {
+                    const float4 a = *reinterpret_cast<const float4 *>(turn.at(lane, w));
+                    v[4 * w] += a.x, v[4 * w + 1] += a.y, v[4 * w + 2] += a.z, v[4 * w + 3] += a.w;
+                }
+                __syncwarp();
             }
             if(!out) {
-                float4 *to = reinterpret_cast<float4 *>(s.sum + col + j);
-                to[0] = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
-                to[1] = make_float4(v[j + 4], v[j + 5], v[j + 6], v[j + 7]);
-                continue;
+#pragma unroll
+                for(int w = 0; w < 8; w++)
+                    turn.put(w, make_uint4(__float_as_uint(v[4 * w]), __float_as_uint(v[4 * w + 1]),
+                                           __float_as_uint(v[4 * w + 2]), __float_as_uint(v[4 * w + 3])));
+                __syncwarp();
+#pragma unroll
+                for(int i = 0; i < turn.kSteps; i++) {
+                    const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i));
+                    if(to >= 0 && c < n)
+                        *reinterpret_cast<uint4 *>(sums + (row0 + turn.row(i)) * n + c) = turn.get(i);
+                }
+                return;
             }
-            uint4 *to = reinterpret_cast<uint4 *>(s.out + col + j);
-            uint4 bits = accumulate ? *to : make_uint4(0, 0, 0, 0);
+        }
+        const Turn<4> turn = {buf, lane};
+        __syncwarp();
+        if(accumulate) {
+            // fp32 sums go through a first turn of the old values
+#pragma unroll
+            for(int i = 0; i < turn.kSteps; i++) {
+                const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i)), c = col + turn.word() * 8;
+                if(to >= 0 && c < n)
+                    *turn.at(turn.row(i), turn.word()) =
+                        *reinterpret_cast<const uint4 *>(out + (size_t)to * stride + c);
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for(int w = 0; w < 4; w++) {
+            uint4 bits = accumulate ? *turn.at(lane, w) : make_uint4(0, 0, 0, 0);
             __half2 *h = reinterpret_cast<__half2 *>(&bits);
 #pragma unroll
             for(int i = 0; i < 4; i++) {
                 const float2 old = __half22float2(h[i]);
-                float a = s.f * v[j + 2 * i], b = s.f * v[j + 2 * i + 1];
+                float a = g.f * v[8 * w + 2 * i], b = g.f * v[8 * w + 2 * i + 1];
                 if(accumulate)
                     a += old.x, b += old.y;
                 h[i] = __floats2half2_rn(a, b);
             }
-            *to = bits;
+            turn.put(w, bits);
+        }
+        __syncwarp();
+#pragma unroll
+        for(int i = 0; i < turn.kSteps; i++) {
+            const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i)), c = col + turn.word() * 8;
+            if(to >= 0 && c < n)  // n is a multiple of 8
+                *reinterpret_cast<uint4 *>(out + (size_t)to * stride + c) = turn.get(i);
         }
     }
     __device__ __forceinline__ void end(const State &, int, int) const {}
@@ -413,13 +500,24 @@ int head_sizes(size_t T, size_t V, size_t D)
 {
     if(!V || !D)
         return B200OPT_EINVAL;
-    return T > B200OPT_LM_MAX || V > B200OPT_LM_MAX || D > B200OPT_LM_MAX ? B200OPT_ETOOBIG : B200OPT_OK;
+    if(T > B200OPT_LM_MAX || V > B200OPT_LM_MAX || D > B200OPT_LM_MAX)
+        return B200OPT_ETOOBIG;
+    // the tiles of a product are counted in 31 bits
+    const size_t most = std::max(T, std::max(V, D)), rest = std::max(std::min(std::max(T, V), D), std::min(T, V));
+    return tiles_of(most) * tiles_of(rest) > 0x7fffffff ? B200OPT_ETOOBIG : B200OPT_OK;
 }
 
-size_t fwd_bytes(size_t T, size_t V)
-{
-    return lm_up(T * 4, 256) + (V + kTcHalf - 1) / kTcHalf * T * 8;
-}
+// The forward pass's workspace: target logits, blocks' sums, their count, parts.
+struct FwdPlan {
+    size_t at_sums, at_done, at_part, bytes;
+    FwdPlan(size_t T, size_t V)
+    {
+        at_sums = lm_up(T * 4, 256);
+        at_done = at_sums + lm_up((T + 31) / 32 * 8, 256);
+        at_part = at_done + 256;
+        bytes = at_part + (V + kTcHalf - 1) / kTcHalf * T * 8;
+    }
+};
 
 }  // namespace
 }  // namespace b200
@@ -434,7 +532,7 @@ int b200opt_vocab_loss_fwd_workspace(size_t tokens, size_t vocab, size_t dim, si
         return B200OPT_EINVAL;
     if(const int rc = head_sizes(tokens, vocab, dim))
         return rc;
-    *bytes = fwd_bytes(tokens, vocab);
+    *bytes = tokens ? FwdPlan(tokens, vocab).bytes : 0;
     return B200OPT_OK;
 }
 
@@ -445,7 +543,8 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
 {
     if(const int rc = head_sizes(tokens, vocab, dim))
         return rc;
-    const size_t need = fwd_bytes(tokens, vocab);
+    const FwdPlan p(tokens, vocab);
+    const size_t need = tokens ? p.bytes : 0;
     if(!lm_index(index_bytes) ||
        !lm_head(tokens, vocab, dim, hidden, hidden_stride, weight, weight_stride, targets, index_bytes) ||
        (tokens && (!loss || !lse)) || !lm_aligned(loss, 4) || !lm_aligned(lse, 4) ||
@@ -457,21 +556,24 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
     if(!tokens && !stats)
         return B200OPT_OK;
     if(tokens) {
-        float *zt = (float *)workspace;
-        float2 *part = (float2 *)((char *)workspace + lm_up(tokens * 4, 256));
+        char *ws = (char *)workspace;
+        float *zt = (float *)ws;
+        unsigned *done = (unsigned *)(ws + p.at_done);
+        float2 *part = (float2 *)(ws + p.at_part);
         int sms = 0;
         CUtensorMap mx, mw;
         if(!lm_sms(&sms) || !tc_map(&mx, hidden, tokens, dim, hidden_stride, tc_box(false)) ||
            !tc_map(&mw, weight, vocab, dim, weight_stride, tc_box(false)))
             return B200OPT_ECUDA;
         TcShape s = {T, V, (int)dim, nullptr, 0, 0, 0, 0, 1, 16};
-        if(!tc_launch<false, false>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt}, sms, st))
+        if(!tc_launch<false, false>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt, done}, sms, st))
             return B200OPT_ECUDA;
         loss_kernel<<<(unsigned)((tokens + 31) / 32), 512, 0, st>>>(
-            T, V, (V - 1) / kTcHalf + 1, part, zt, targets, wide, loss, lse);
+            T, V, (V - 1) / kTcHalf + 1, part, zt, targets, wide, loss, lse, (float2 *)(ws + p.at_sums), done,
+            stats);
+    } else {
+        no_stats_kernel<<<1, 1, 0, st>>>(stats);
     }
-    if(stats)
-        stats_kernel<<<1, 1024, 0, st>>>(T, V, loss, targets, wide, stats);
     return lm_launched();
 }
 
@@ -527,7 +629,7 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
     const size_t rows = lm_up(tokens, kTcTile);
     const Factor factor = {grad_scale, loss_scale, stats};
 
-    const int per = (int)std::max<size_t>(32, lm_up((tokens + 4 * sms - 1) / (4 * sms), 32));
+    const int per = (int)lm_up((tokens + 4 * sms - 1) / (4 * sms), 8);  // a row a warp, at least
     compact_kernel<<<(T + per - 1) / per, 256, 0, st>>>(
         T, V, D, per, (const __half *)hidden, hidden_stride, targets, wide, lse, xc, lsec, target, from,
         count, (__half *)grad_hidden, grad_hidden_stride);
