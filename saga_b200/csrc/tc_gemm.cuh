@@ -16,7 +16,7 @@
 // is ever transposed in memory.
 //
 // Warps: 0 issues the TMA loads, 1 (of the even CTA) the MMAs, 2 owns the tensor
-// memory, 4..11 are the epilogue.  Two accumulators alternate, so the epilogue
+// memory, 4..19 are the epilogue.  Two accumulators alternate, so the epilogue
 // of a tile runs beside the main loop of the next one.
 //
 // Every wait is bounded: one that runs out makes the epilogue write NaN for the
@@ -32,11 +32,13 @@ namespace b200 {
 constexpr int kTcTile = 256;    // tile of a CTA pair, both ways
 constexpr int kTcHalf = 128;    // a CTA's rows of A, of B and of the result
 constexpr int kTcK = 64;        // k per stage: 128 bytes, the swizzle's span
-constexpr int kTcStages = 6;
+constexpr int kTcStages = 5;
 constexpr int kTcOperand = kTcHalf * kTcK * 2;  // bytes of one operand of a stage in a CTA
-constexpr int kTcThreads = 384;
+constexpr int kTcEpilogue = 16;  // warps: four for each 32 rows, 64 columns each
+constexpr int kTcColumns = kTcTile / (kTcEpilogue / 4);
+constexpr int kTcThreads = 128 + 32 * kTcEpilogue;
 constexpr int kTcStaging = 4096;  // bytes an epilogue warp turns its columns around in
-constexpr int kTcSmem = kTcStages * 2 * kTcOperand + 8 * kTcStaging + 1024;
+constexpr int kTcSmem = kTcStages * 2 * kTcOperand + kTcEpilogue * kTcStaging + 1024;
 constexpr unsigned long long kTcWaitNs = 2000000000ull;
 
 struct TcShape {
@@ -206,6 +208,14 @@ __device__ __forceinline__ void tmem_wait(float (&v)[32])
         asm volatile("" : "+f"(v[j]));
 }
 
+// A part of the sum without a share of k is 0, a tile whose wait ran out NaN.
+__device__ __forceinline__ void no_result(float (&v)[32], bool ok)
+{
+#pragma unroll
+    for(int j = 0; j < 32; j++)
+        v[j] = ok ? 0.0f : __int_as_float(0x7fffffff);
+}
+
 // ------------------------------------------------------------- epilogue's turn
 //
 // A thread has 32 columns of one row; written straight to memory that would be a
@@ -265,9 +275,10 @@ struct TcTiles {
 };
 
 // Epi: the epilogue.  common() is what all tiles share; begin(common, row, col,
-// part) gives a thread's state for its row of a tile and the 128 columns from col;
-// columns(common, state, row, col, v, staging) gets 32 columns at a time, all lanes
-// of a warp together; end(state, row, col) closes them.  Rows and columns beyond the matrix come too and are for the epilogue to
+// part) gives a thread's state for its row of a tile and the kTcColumns columns from
+// col; columns(common, state, row, col, v, staging) gets 32 columns at a time, all
+// lanes of a warp together; end(state, row, col, acc, shared) closes them, where
+// `shared` is the staging memory of all epilogue warps.  Rows and columns beyond the matrix come too and are for the epilogue to
 // leave out.
 template <bool A_MN, bool B_MN, typename Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
@@ -292,7 +303,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         }
         for(int i = 0; i < 2; i++) {
             mbar_init(smem_u32(&acc_full[i]), 1);
-            mbar_init(smem_u32(&acc_empty[i]), 2 * 8);  // the epilogue warps of both CTAs
+            mbar_init(smem_u32(&acc_empty[i]), 2 * kTcEpilogue);  // the epilogue warps of both CTAs
         }
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
@@ -389,8 +400,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         }
     } else if(warp >= 4) {
         const int quad = warp & 3, side = (warp - 4) >> 2;
-        char *staging = smem_raw + (base - smem_u32(smem_raw)) + kTcStages * 2 * kTcOperand +
-                        (warp - 4) * kTcStaging;
+        char *const shared = smem_raw + (base - smem_u32(smem_raw)) + kTcStages * 2 * kTcOperand;
+        char *const staging = shared + (warp - 4) * kTcStaging;
         const auto common = epi.common();
         int acc = 0;
         uint32_t acc_phase = 0;
@@ -399,31 +410,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             int m, n, part, k0, k1;
             tiles.at(i, m, n, part, k0, k1);
             const int row = m * kTcTile + (int)rank * kTcHalf + quad * 32 + lane;
-            const int col = n * kTcTile + side * kTcHalf;
+            const int col = n * kTcTile + side * kTcColumns;
             const uint32_t from =
-                tmem + ((uint32_t)(quad * 32) << 16) + acc * kTcTile + side * kTcHalf;
+                tmem + ((uint32_t)(quad * 32) << 16) + acc * kTcTile + side * kTcColumns;
             auto state = epi.begin(common, row, col, part);  // its loads run during the wait
             ok = ok && mbar_wait(smem_u32(&acc_full[acc]), acc_phase, dead);
             ok = __all_sync(0xffffffffu, ok);
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            float v[2][32];
-            const bool none = !ok || k1 == k0;  // a wait that ran out, or no share of k
-            if(!none)
-                tmem_load(from, v[0]);
-#pragma unroll
-            for(int c = 0; c < kTcHalf / 32; c++) {  // the next columns load meanwhile
-                if(none) {
-#pragma unroll
-                    for(int j = 0; j < 32; j++)
-                        v[c & 1][j] = ok ? 0.0f : __int_as_float(0x7fffffff);
-                } else {
-                    tmem_wait(v[c & 1]);
-                    if(c + 1 < kTcHalf / 32)
-                        tmem_load(from + (c + 1) * 32, v[(c + 1) & 1]);
-                }
-                epi.columns(common, state, row, col + c * 32, v[c & 1], staging);
+#pragma unroll 1
+            for(int c = 0; c < kTcColumns; c += 32) {
+                float v[32];
+                tmem_load(from + c, v);
+                tmem_wait(v);
+                if(!ok || k1 == k0)
+                    no_result(v, ok);
+                epi.columns(common, state, row, col + c, v, staging);
             }
-            epi.end(state, row, col);
+            epi.end(state, row, col, acc, shared);
             asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
             __syncwarp();
             if(lane == 0)

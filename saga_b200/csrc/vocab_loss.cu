@@ -23,7 +23,7 @@ __device__ __forceinline__ float exp2_fast(float x)
 
 // ------------------------------------------------------------------ forward
 
-// Per row and 128 columns of the vocabulary: the maximum of z log2(e) and the
+// Per row and tile of the vocabulary: the maximum of z log2(e) and the
 // sum of 2^(z log2(e) - maximum), in one pass over the accumulator.  The target's
 // logit goes to zt.
 struct StatsEpilogue {
@@ -76,10 +76,24 @@ struct StatsEpilogue {
         s.top = top;
         s.sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
-    __device__ __forceinline__ void end(const State &s, int row, int col) const
+    // The four warps that share 32 rows meet; two sets of slots, one for each
+    // accumulator, keep a tile's from the next one's.
+    __device__ __forceinline__ void end(const State &s, int row, int col, int acc, char *shared) const
     {
-        if(row < T && col < V)
-            part[(size_t)(col / kTcHalf) * T + row] = make_float2(s.top, s.sum);
+        const int quad = (threadIdx.x >> 5) & 3, side = ((threadIdx.x >> 5) - 4) >> 2;
+        float2 *slots = reinterpret_cast<float2 *>(shared) + acc * 512 + quad * 32 + (threadIdx.x & 31);
+        slots[side * 128] = make_float2(s.top, s.sum);
+        asm volatile("bar.sync %0, 128;" ::"r"(1 + quad) : "memory");
+        if(side || row >= T)
+            return;
+        float top = s.top, sum = 0.0f;
+#pragma unroll
+        for(int i = 1; i < 4; i++)
+            top = fmaxf(top, slots[i * 128].x);
+#pragma unroll
+        for(int i = 0; i < 4; i++)  // a side beyond the vocabulary has -inf and 0
+            sum += slots[i * 128].y * exp2_fast(slots[i * 128].x - top);
+        part[(size_t)(col / kTcTile) * T + row] = make_float2(top, sum);
     }
 };
 
@@ -283,7 +297,7 @@ struct DzEpilogue {
         for(int i = 0; i < turn.kSteps; i++)
             *reinterpret_cast<uint4 *>(to + turn.row(i) * stride) = turn.get(i);
     }
-    __device__ __forceinline__ void end(const State &, int, int) const {}
+    __device__ __forceinline__ void end(const State &, int, int, int, char *) const {}
 };
 
 struct Factor {
@@ -297,56 +311,71 @@ struct Factor {
     }
 };
 
-// One of: sum[part][row] = acc, or += acc; out = factor * (sum + acc) (+ out).
+// What a product's result does, MODE:
+enum {
+    kOut,         // out = factor * acc
+    kAccumulate,  // out += factor * acc
+    kSums,        // sum[part] = acc, or += acc when it holds earlier pieces
+    kLast         // out = factor * (sum + acc): the last piece
+};
+template <int MODE>
 struct OutEpilogue {
     int m;
     const int *count;  // replaces m
     int n;
-    float *sum;        // fp32, row stride n, one matrix per part; may be null
+    float *sum;        // fp32, row stride n, one matrix per part
     size_t part_stride;
     int add;           // sum holds earlier pieces
-    __half *out;       // null: into sum
+    __half *out;
     size_t stride;
     const int *rows;   // where a row of the result goes; null: its own place
-    int accumulate;
     Factor factor;
-    struct State {
-        long long row;
-        float *sums;    // of this part
-        int to;         // row of the result; -1: none
-    };
     struct Common {
         int live;
         float f;
     };
+    struct State {
+        int to;         // row of the result; -1: none
+        float *sums;    // of this warp's first row and part
+        __half *at[4];  // where this thread writes in the four steps of a turn; null: nowhere
+    };
     __device__ __forceinline__ Common common() const
     {
-        return {count ? *count : m, out ? factor.get() : 0.0f};
+        return {count ? *count : m, MODE == kSums ? 0.0f : factor.get()};
     }
     __device__ __forceinline__ State begin(const Common &g, int row, int, int part) const
     {
-        return {(long long)row, sum ? sum + part * part_stride : nullptr,
-                row < g.live ? (out && rows ? rows[row] : row) : -1};
+        State s;
+        const int lane = threadIdx.x & 31;
+        s.to = row < g.live ? (MODE != kSums && rows ? rows[row] : row) : -1;
+        if(MODE == kSums || MODE == kLast)
+            s.sums = sum + part * part_stride + (size_t)(row - lane) * n;
+        if(MODE != kSums) {
+            const Turn<4> turn = {nullptr, lane};
+#pragma unroll
+            for(int i = 0; i < 4; i++) {
+                const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i));
+                s.at[i] = to >= 0 ? out + (size_t)to * stride + turn.word() * 8 : nullptr;
+            }
+        }
+        return s;
     }
     __device__ __forceinline__ void columns(const Common &g, State &s, int, int col, float (&v)[32], char *buf) const
     {
         const int lane = threadIdx.x & 31;
         if(col >= n)
             return;
-        float *const sums = s.sums;
-        const long long row0 = s.row - lane;
-        if(sums && (add || !out)) {
-            // fp32: what earlier pieces left comes in, or the new sums go out
+        if(MODE == kSums || MODE == kLast) {
             const Turn<8> turn = {buf, lane};
             const int c = col + turn.word() * 4;
             __syncwarp();
-            if(add) {
+            if(MODE == kLast || add) {
 #pragma unroll
                 for(int i = 0; i < turn.kSteps; i++) {
                     const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i));
                     if(to >= 0 && c < n)
                         *turn.at(turn.row(i), turn.word()) =
-                            *reinterpret_cast<const uint4 *>(sums + (row0 + turn.row(i)) * n + c);
+                            *reinterpret_cast<const uint4 *>(s.sums + (size_t)turn.row(i) * n + c);
                 }
                 __syncwarp();
 #pragma unroll
@@ -356,7 +385,7 @@ struct OutEpilogue {
                 }
                 __syncwarp();
             }
-            if(!out) {
+            if(MODE == kSums) {
 #pragma unroll
                 for(int w = 0; w < 8; w++)
                     turn.put(w, make_uint4(__float_as_uint(v[4 * w]), __float_as_uint(v[4 * w + 1]),
@@ -366,48 +395,55 @@ struct OutEpilogue {
                 for(int i = 0; i < turn.kSteps; i++) {
                     const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i));
                     if(to >= 0 && c < n)
-                        *reinterpret_cast<uint4 *>(sums + (row0 + turn.row(i)) * n + c) = turn.get(i);
+                        *reinterpret_cast<uint4 *>(s.sums + (size_t)turn.row(i) * n + c) = turn.get(i);
                 }
-                return;
             }
         }
+        if(MODE == kSums)
+            return;
         const Turn<4> turn = {buf, lane};
+        const bool inside = col + turn.word() * 8 < n;  // n is a multiple of 8
         __syncwarp();
-        if(accumulate) {
-            // fp32 sums go through a first turn of the old values
+        if(MODE == kAccumulate) {
 #pragma unroll
-            for(int i = 0; i < turn.kSteps; i++) {
-                const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i)), c = col + turn.word() * 8;
-                if(to >= 0 && c < n)
-                    *turn.at(turn.row(i), turn.word()) =
-                        *reinterpret_cast<const uint4 *>(out + (size_t)to * stride + c);
-            }
+            for(int i = 0; i < 4; i++)
+                if(s.at[i] && inside)
+                    *turn.at(turn.row(i), turn.word()) = *reinterpret_cast<const uint4 *>(s.at[i] + col);
             __syncwarp();
         }
 #pragma unroll
         for(int w = 0; w < 4; w++) {
-            uint4 bits = accumulate ? *turn.at(lane, w) : make_uint4(0, 0, 0, 0);
+            uint4 bits = MODE == kAccumulate ? *turn.at(lane, w) : make_uint4(0, 0, 0, 0);
             __half2 *h = reinterpret_cast<__half2 *>(&bits);
 #pragma unroll
             for(int i = 0; i < 4; i++) {
-                const float2 old = __half22float2(h[i]);
                 float a = g.f * v[8 * w + 2 * i], b = g.f * v[8 * w + 2 * i + 1];
-                if(accumulate)
+                if(MODE == kAccumulate) {
+                    const float2 old = __half22float2(h[i]);
                     a += old.x, b += old.y;
+                }
                 h[i] = __floats2half2_rn(a, b);
             }
             turn.put(w, bits);
         }
         __syncwarp();
 #pragma unroll
-        for(int i = 0; i < turn.kSteps; i++) {
-            const int to = __shfl_sync(0xffffffffu, s.to, turn.row(i)), c = col + turn.word() * 8;
-            if(to >= 0 && c < n)  // n is a multiple of 8
-                *reinterpret_cast<uint4 *>(out + (size_t)to * stride + c) = turn.get(i);
-        }
+        for(int i = 0; i < 4; i++)
+            if(s.at[i] && inside)
+                *reinterpret_cast<uint4 *>(s.at[i] + col) = turn.get(i);
     }
-    __device__ __forceinline__ void end(const State &, int, int) const {}
+    __device__ __forceinline__ void end(const State &, int, int, int, char *) const {}
 };
+
+// A product into its result; false when it could not be launched.
+template <bool A_MN, bool B_MN, int MODE>
+bool product(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, int m, const int *count, int n,
+             float *sum, size_t part_stride, int add, __half *out, size_t stride, const int *rows,
+             const Factor &factor, int sms, cudaStream_t st)
+{
+    const OutEpilogue<MODE> e = {m, count, n, sum, part_stride, add, out, stride, rows, factor};
+    return tc_launch<A_MN, B_MN>(a, b, s, e, sms, st);
+}
 
 // Joins the parts of a product that was cut along k, in their order.
 __global__ void __launch_bounds__(256)
@@ -515,7 +551,7 @@ struct FwdPlan {
         at_sums = lm_up(T * 4, 256);
         at_done = at_sums + lm_up((T + 31) / 32 * 8, 256);
         at_part = at_done + 256;
-        bytes = at_part + (V + kTcHalf - 1) / kTcHalf * T * 8;
+        bytes = at_part + tiles_of(V) * T * 8;
     }
 };
 
@@ -569,7 +605,7 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
         if(!tc_launch<false, false>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt, done}, sms, st))
             return B200OPT_ECUDA;
         loss_kernel<<<(unsigned)((tokens + 31) / 32), 512, 0, st>>>(
-            T, V, (V - 1) / kTcHalf + 1, part, zt, targets, wide, loss, lse, (float2 *)(ws + p.at_sums), done,
+            T, V, (int)tiles_of(vocab), part, zt, targets, wide, loss, lse, (float2 *)(ws + p.at_sums), done,
             stats);
     } else {
         no_stats_kernel<<<1, 1, 0, st>>>(stats);
@@ -654,9 +690,11 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
         if(grad_hidden) {  // += dz W
             const bool direct = p.x_parts == 1 && last;
             s = {T, D, N, count, 1, 0, 0, at, (int)p.x_parts, 8};
-            OutEpilogue e = {T, count, D, xsum, tokens * dim, !begin,
-                             direct ? (__half *)grad_hidden : nullptr, grad_hidden_stride, from, 0, factor};
-            if(!tc_launch<false, true>(dz_k, w_mn, s, e, sms, st))
+            auto *run = !direct ? product<false, true, kSums>
+                        : begin ? product<false, true, kOut>
+                                : product<false, true, kLast>;
+            if(!run(dz_k, w_mn, s, T, count, D, xsum, tokens * dim, !begin, (__half *)grad_hidden,
+                    grad_hidden_stride, from, factor, sms, st))
                 return B200OPT_ECUDA;
             if(last && !direct)
                 join_kernel<<<sms * 4, 256, 0, st>>>(T, count, D, xsum, tokens * dim, (int)p.x_parts,
@@ -666,9 +704,11 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
         if(grad_weight) {  // = dz^T X
             __half *to = (__half *)grad_weight + first * grad_weight_stride;
             s = {N, D, T, count, 0, 1, 0, 0, (int)p.w_parts, 8};
-            OutEpilogue e = {N, nullptr, D, wsum, n * dim, 0, p.w_parts == 1 ? to : nullptr,
-                             grad_weight_stride, nullptr, accumulate, factor};
-            if(!tc_launch<true, true>(dz_mn, x_mn, s, e, sms, st))
+            auto *run = p.w_parts > 1 ? product<true, true, kSums>
+                        : accumulate  ? product<true, true, kAccumulate>
+                                      : product<true, true, kOut>;
+            if(!run(dz_mn, x_mn, s, N, nullptr, D, wsum, n * dim, 0, to, grad_weight_stride, nullptr,
+                    factor, sms, st))
                 return B200OPT_ECUDA;
             if(p.w_parts > 1)
                 join_kernel<<<sms * 4, 256, 0, st>>>(N, nullptr, D, wsum, n * dim, (int)p.w_parts, to,
