@@ -484,9 +484,8 @@ int gradient(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide,
     unsigned char *named = (unsigned char *)(work + w.at_named);
     float *parts = (float *)(work + w.at_parts);
     int sms = 0;
-    if(!lm_sms(&sms) ||
-       cudaFuncSetAttribute(order_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kOrderSmem) !=
-           cudaSuccess)
+    static std::atomic<uint64_t> allowed{0};
+    if(!lm_sms(&sms) || !lm_allow_smem(order_kernel, kOrderSmem, allowed))
         return B200OPT_ECUDA;
     // one block an SM, more where a block would get more rows than it has digits for
     const size_t blocks = std::min(vocab, std::max<size_t>(sms, (vocab + kDigits - 1) / kDigits));

@@ -5,6 +5,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -34,6 +35,24 @@ inline bool lm_matrix(const void *p, size_t rows, size_t cols, size_t stride, si
 inline int lm_launched()
 {
     return cudaGetLastError() == cudaSuccess ? B200OPT_OK : B200OPT_ECUDA;
+}
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device.  The
+// setting stays with the kernel, so it is made once per device; `done` is the
+// kernel's own record of where.
+template <typename Kernel>
+inline bool lm_allow_smem(Kernel *kernel, int bytes, std::atomic<uint64_t> &done)
+{
+    int dev = 0;
+    if(cudaGetDevice(&dev) != cudaSuccess)
+        return false;
+    const uint64_t bit = dev < 64 ? 1ull << dev : 0;
+    if(done.load(std::memory_order_relaxed) & bit)
+        return true;
+    if(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) != cudaSuccess)
+        return false;
+    done.fetch_or(bit, std::memory_order_relaxed);
+    return true;
 }
 
 // The number of SMs of the current device.

@@ -50,7 +50,31 @@ struct TcShape {
     int a_row0, b_row0;  // first row of the tensor maps' outer dimension that is used
     int splits;          // the k range is cut into so many parts
     int group;           // m tiles that are walked through before the next n tile
+    int sum_rows;        // dyn_m and splits > 1: rows that the parts' sums have room for
+    int plan_stages;     // and the stages of k that the parts are planned for
 };
+
+constexpr int kTcPlanPairs = 74;  // CTA pairs that a product is cut for: 148 SMs
+
+// How many parts the k range of a product is cut into: as many as fill the GPU
+// when its tiles alone do not, each with at least 16 stages of k (a part of eight
+// saves 2 us of main loop, which the launch that joins the parts costs again).
+__host__ __device__ inline uint32_t tc_parts(uint32_t tiles, uint32_t stages)
+{
+    const uint32_t fill = kTcPlanPairs / tiles, most = stages / 16;
+    const uint32_t parts = fill < most ? fill : most;
+    return parts ? parts : 1;
+}
+
+// The same on the device, where the number of rows is known: fewer rows than
+// planned leave room for more parts.
+__device__ __forceinline__ uint32_t tc_parts_of(const TcShape &s, int rows)
+{
+    if(s.splits <= 1 || !s.dyn_m)
+        return s.splits;
+    const uint32_t tiles = ((rows + kTcTile - 1) / kTcTile) * ((s.n + kTcTile - 1) / kTcTile);
+    return min(tc_parts(tiles, s.plan_stages), (uint32_t)s.sum_rows / (uint32_t)rows);
+}
 
 // --------------------------------------------------------------- primitives
 
@@ -253,7 +277,7 @@ struct TcTiles {
         nt = (s.n + kTcTile - 1) / kTcTile;
         kblocks = (k + kTcK - 1) / kTcK;
         group = s.group;
-        splits = s.splits;
+        splits = tc_parts_of(s, m);
     }
     __device__ __forceinline__ uint32_t count() const { return mt * nt * splits; }
     __device__ __forceinline__ void at(uint32_t i, int &m, int &n, int &part, int &k0, int &k1) const
@@ -487,9 +511,11 @@ bool tc_launch(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, con
                cudaStream_t st)
 {
     auto *kernel = tc_gemm_kernel<A_MN, B_MN, Epi>;
-    if(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kTcSmem) != cudaSuccess)
+    static std::atomic<uint64_t> allowed{0};
+    if(!lm_allow_smem(kernel, kTcSmem, allowed))
         return false;
-    const long long tiles = (s.m + kTcTile - 1ll) / kTcTile * ((s.n + kTcTile - 1ll) / kTcTile) * s.splits;
+    // (as many pairs as planned for, where the device may find more parts)
+    const long long tiles = s.splits > 1 && s.dyn_m ? kTcPlanPairs : (s.m + kTcTile - 1ll) / kTcTile * ((s.n + kTcTile - 1ll) / kTcTile) * s.splits;
     const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
     if(tiles > 0x7fffffff)
         return false;

@@ -12,7 +12,6 @@ constexpr size_t kPieceBytes = (size_t)256 << 20;  // of p - onehot held at a ti
 constexpr float kLift = 32768.0f;                  // 2^15: see the header
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-constexpr int kPlanPairs = 74;  // CTA pairs that a product is cut for: 148 SMs
 
 __device__ __forceinline__ float exp2_fast(float x)
 {
@@ -323,8 +322,7 @@ struct OutEpilogue {
     int m;
     const int *count;  // replaces m
     int n;
-    float *sum;        // fp32, row stride n, one matrix per part
-    size_t part_stride;
+    float *sum;        // fp32, row stride n, a matrix of the product's rows per part
     int add;           // sum holds earlier pieces
     __half *out;
     size_t stride;
@@ -349,7 +347,7 @@ struct OutEpilogue {
         const int lane = threadIdx.x & 31;
         s.to = row < g.live ? (MODE != kSums && rows ? rows[row] : row) : -1;
         if(MODE == kSums || MODE == kLast)
-            s.sums = sum + part * part_stride + (size_t)(row - lane) * n;
+            s.sums = sum + ((size_t)part * g.live + (row - lane)) * n;
         if(MODE != kSums) {
             const Turn<4> turn = {nullptr, lane};
 #pragma unroll
@@ -438,19 +436,21 @@ struct OutEpilogue {
 // A product into its result; false when it could not be launched.
 template <bool A_MN, bool B_MN, int MODE>
 bool product(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, int m, const int *count, int n,
-             float *sum, size_t part_stride, int add, __half *out, size_t stride, const int *rows,
+             float *sum, int add, __half *out, size_t stride, const int *rows,
              const Factor &factor, int sms, cudaStream_t st)
 {
-    const OutEpilogue<MODE> e = {m, count, n, sum, part_stride, add, out, stride, rows, factor};
+    const OutEpilogue<MODE> e = {m, count, n, sum, add, out, stride, rows, factor};
     return tc_launch<A_MN, B_MN>(a, b, s, e, sms, st);
 }
 
 // Joins the parts of a product that was cut along k, in their order.
 __global__ void __launch_bounds__(256)
-    join_kernel(int m, const int *count, int n, const float *sum, size_t part_stride, int parts,
-                __half *out, size_t stride, const int *rows, int accumulate, Factor factor)
+    join_kernel(TcShape shape, const int *count, int n, const float *sum, __half *out, size_t stride,
+                const int *rows, int accumulate, Factor factor)
 {
-    const int live = count ? *count : m, vecs = n / 8;
+    const int live = count ? *count : shape.m, vecs = n / 8;
+    const int parts = (int)tc_parts_of(shape, max(live, 1));
+    const size_t part_stride = (size_t)live * n;
     const float f = factor.get();
     const long long total = (long long)live * vecs;
     for(long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total;
@@ -482,12 +482,10 @@ __global__ void __launch_bounds__(256)
 
 size_t tiles_of(size_t n) { return (n + kTcTile - 1) / kTcTile; }
 
-// How many parts the k range of a product is cut into: as many as fill the GPU
-// when its tiles alone do not, each with at least eight stages of k.
 size_t parts_of(size_t m, size_t n, size_t k)
 {
-    const size_t tiles = tiles_of(m) * tiles_of(n), stages = (k + kTcK - 1) / kTcK;
-    return std::max<size_t>(1, std::min(kPlanPairs / tiles, stages / 8));
+    const size_t tiles = tiles_of(m) * tiles_of(n);
+    return tiles > kTcPlanPairs ? 1 : tc_parts((uint32_t)tiles, (uint32_t)((k + kTcK - 1) / kTcK));
 }
 
 struct Plan {
@@ -689,17 +687,17 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
             return B200OPT_ECUDA;
         if(grad_hidden) {  // += dz W
             const bool direct = p.x_parts == 1 && last;
-            s = {T, D, N, count, 1, 0, 0, at, (int)p.x_parts, 8};
+            s = {T, D, N, count, 1, 0, 0, at, (int)p.x_parts, 8, (int)(p.x_parts * tokens),
+                 (int)((std::min(p.piece, vocab) + kTcK - 1) / kTcK)};
             auto *run = !direct ? product<false, true, kSums>
                         : begin ? product<false, true, kOut>
                                 : product<false, true, kLast>;
-            if(!run(dz_k, w_mn, s, T, count, D, xsum, tokens * dim, !begin, (__half *)grad_hidden,
+            if(!run(dz_k, w_mn, s, T, count, D, xsum, !begin, (__half *)grad_hidden,
                     grad_hidden_stride, from, factor, sms, st))
                 return B200OPT_ECUDA;
             if(last && !direct)
-                join_kernel<<<sms * 4, 256, 0, st>>>(T, count, D, xsum, tokens * dim, (int)p.x_parts,
-                                                     (__half *)grad_hidden, grad_hidden_stride, from, 0,
-                                                     factor);
+                join_kernel<<<sms * 4, 256, 0, st>>>(s, count, D, xsum, (__half *)grad_hidden,
+                                                     grad_hidden_stride, from, 0, factor);
         }
         if(grad_weight) {  // = dz^T X
             __half *to = (__half *)grad_weight + first * grad_weight_stride;
@@ -707,12 +705,12 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
             auto *run = p.w_parts > 1 ? product<true, true, kSums>
                         : accumulate  ? product<true, true, kAccumulate>
                                       : product<true, true, kOut>;
-            if(!run(dz_mn, x_mn, s, N, nullptr, D, wsum, n * dim, 0, to, grad_weight_stride, nullptr,
+            if(!run(dz_mn, x_mn, s, N, nullptr, D, wsum, 0, to, grad_weight_stride, nullptr,
                     factor, sms, st))
                 return B200OPT_ECUDA;
             if(p.w_parts > 1)
-                join_kernel<<<sms * 4, 256, 0, st>>>(N, nullptr, D, wsum, n * dim, (int)p.w_parts, to,
-                                                     grad_weight_stride, nullptr, accumulate, factor);
+                join_kernel<<<sms * 4, 256, 0, st>>>(s, nullptr, D, wsum, to, grad_weight_stride, nullptr,
+                                                     accumulate, factor);
         }
     }
     return lm_launched();

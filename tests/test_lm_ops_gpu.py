@@ -388,6 +388,17 @@ def test_vocab_loss_several_pieces_of_the_vocabulary():
     check_head(x, w, y, f, b, 4096.0)
 
 
+@pytest.mark.parametrize("tokens,vocab,dim,ignored", [
+    (1000, 6000, 264, 0.5), (1000, 6000, 264, 0.97), (700, 9000, 64, 0.999), (2000, 300, 520, 0.9),
+    (4500, 40000, 64, 0.6)])
+def test_vocab_loss_mostly_ignored(tokens, vocab, dim, ignored):
+    """Few tokens left of many: the gradient's products are cut for those that are left."""
+    x, w, y = head_inputs(tokens, vocab, dim, seed=5, ignored=ignored)
+    f = layers.vocab_loss_forward(x, w, y)
+    b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=256.0)
+    check_head(x, w, y, f, b, 256.0)
+
+
 @pytest.mark.parametrize("std", [0.0, 30.0])
 def test_vocab_loss_flat_and_peaked_distributions(std):
     g = gen(17)
@@ -422,6 +433,15 @@ def test_vocab_loss_non_finite_tokens_stay_in_their_rows():
     """A NaN token spoils its own loss and the table's gradient, which the optimizer's flags then
     report, but no other token's loss or gradient; an ignored NaN token spoils nothing."""
     x, w, y = head_inputs(300, 500, 64, ignored=0)
+    y3, x3 = y.clone(), x.clone()
+    y3[[7, 200, 299]] = -1
+    x3[7], x3[200, 3], x3[299] = float("nan"), float("inf"), float("-inf")
+    good3 = layers.vocab_loss_forward(x, w, y3)
+    f3 = layers.vocab_loss_forward(x3, w, y3)
+    assert torch.equal(f3[0], good3[0]) and torch.equal(f3[2], good3[2])
+    want3 = layers.vocab_loss_backward(x, w, y3, good3[1], stats=good3[2])
+    got3 = layers.vocab_loss_backward(x3, w, y3, f3[1], stats=f3[2])
+    assert all(torch.equal(p, q) for p, q in zip(got3, want3))
     clean = layers.vocab_loss_forward(x, w, y)
     x2 = x.clone()
     x2[7], x2[200, 3] = float("nan"), float("inf")
