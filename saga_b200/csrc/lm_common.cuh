@@ -132,6 +132,56 @@ __device__ __forceinline__ int lm_index_at(const void *ids, int wide, size_t i, 
     return v >= 0 && v < (long long)vocab ? (int)v : -1;
 }
 
+// --------------------------------------------- barriers of asynchronous copies
+
+constexpr unsigned long long kWaitNs = 2000000000ull;  // limit of every wait
+
+__device__ __forceinline__ uint32_t smem_u32(const void *p)
+{
+    return (uint32_t)__cvta_generic_to_shared(p);
+}
+
+__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
+{
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
+}
+
+__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
+{
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n"
+        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
+        " selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+
+__device__ __forceinline__ unsigned long long now_ns()
+{
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Waits for the phase; false when the time ran out here or elsewhere in the CTA.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead)
+{
+    for(int i = 0; i < 64; i++)
+        if(mbar_try(bar, parity))
+            return true;
+    const unsigned long long began = now_ns();
+    while(!mbar_try(bar, parity)) {
+        if(*dead || now_ns() - began > kWaitNs) {
+            *dead = 1;
+            return false;
+        }
+    }
+    return true;
+}
+
 __device__ __forceinline__ float warp_sum(float v)
 {
 #pragma unroll

@@ -39,7 +39,6 @@ constexpr int kTcColumns = kTcTile / (kTcEpilogue / 4);
 constexpr int kTcThreads = 128 + 32 * kTcEpilogue;
 constexpr int kTcStaging = 4096;  // bytes an epilogue warp turns its columns around in
 constexpr int kTcSmem = kTcStages * 2 * kTcOperand + kTcEpilogue * kTcStaging + 1024;
-constexpr unsigned long long kTcWaitNs = 2000000000ull;
 
 struct TcShape {
     // sizes in elements; a dynamic size is read from *count on the device
@@ -77,52 +76,6 @@ __device__ __forceinline__ uint32_t tc_parts_of(const TcShape &s, int rows)
 }
 
 // --------------------------------------------------------------- primitives
-
-__device__ __forceinline__ uint32_t smem_u32(const void *p)
-{
-    return (uint32_t)__cvta_generic_to_shared(p);
-}
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count)
-{
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-
-__device__ __forceinline__ bool mbar_try(uint32_t bar, uint32_t parity)
-{
-    uint32_t ok;
-    asm volatile(
-        "{\n .reg .pred p;\n"
-        " mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n"
-        " selp.u32 %0, 1, 0, p;\n}\n"
-        : "=r"(ok)
-        : "r"(bar), "r"(parity)
-        : "memory");
-    return ok != 0;
-}
-
-__device__ __forceinline__ unsigned long long tc_now()
-{
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Waits for the phase; false when the time ran out here or elsewhere in the CTA.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int *dead)
-{
-    for(int i = 0; i < 64; i++)
-        if(mbar_try(bar, parity))
-            return true;
-    const unsigned long long began = tc_now();
-    while(!mbar_try(bar, parity)) {
-        if(*dead || tc_now() - began > kTcWaitNs) {
-            *dead = 1;
-            return false;
-        }
-    }
-    return true;
-}
 
 __device__ __forceinline__ uint32_t cluster_rank()
 {
