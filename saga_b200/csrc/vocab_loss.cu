@@ -1,7 +1,6 @@
 // Softmax cross entropy over the vocabulary with the classifier's product, and
 // its gradient (b200opt_vocab_loss_* of include/b200opt.h).
 #include <algorithm>
-#include <climits>
 
 #include "tc_gemm.cuh"
 
@@ -649,6 +648,8 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
             return B200OPT_ECUDA;
         return B200OPT_OK;
     }
+    if(!grad_hidden && !grad_weight)
+        return B200OPT_OK;
     int sms = 0;
     if(!lm_sms(&sms))
         return B200OPT_ECUDA;

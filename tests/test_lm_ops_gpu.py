@@ -71,7 +71,7 @@ def strided(t, stride, shift=0):
 
 EMB_SIZES = [  # tokens, vocab, dim
     (1, 1, 1), (1, 1000, 64), (7, 3, 5), (64, 1000, 333), (1000, 17, 40), (1025, 5003, 96),
-    (300, 300, 1032), (2049, 1, 24), (33, 70001, 8), (20011, 211, 16)]
+    (300, 300, 1032), (2049, 1, 24), (33, 70001, 8), (20011, 211, 16), (50, 700, 2304), (40, 20, 70000)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
@@ -246,6 +246,29 @@ def test_layernorm_backward(rows, dim, dtype, params):
         close(ab, db + bb.double(), e_db + U * (db.abs() + bb.double().abs()) + half_step(db + bb.double(), kind))
 
 
+def test_layernorm_outputs_that_are_not_wanted():
+    """Each output alone, through the C entry, equals the one of the full call."""
+    g = gen(6)
+    rows, dim = 70, 264
+    x, dy, gamma = normal(g, rows, dim), normal(g, rows, dim), normal(g, dim, dtype=torch.float32)
+    y, mean, rstd = layers.layernorm_forward(x, gamma)
+    vp = lambda t: C.c_void_p(t.data_ptr() if t is not None else None)
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    alone = torch.empty_like(y)
+    assert capi.lib().b200opt_layernorm_fwd(capi.HALF, capi.FLOAT, rows, dim, vp(x), dim, vp(gamma), None,
+                                            1e-5, vp(alone), dim, None, None, stream) == capi.OK
+    assert torch.equal(alone, y)
+    want = layers.layernorm_backward(dy, x, gamma, mean, rstd)
+    ws = torch.empty(layers.layernorm_workspace(rows, dim), dtype=torch.uint8, device=DEV)
+    for keep in ((0,), (1,), (2,), (0, 2), (1, 2), ()):
+        out = [torch.zeros_like(t) if k in keep else None for k, t in enumerate(want)]
+        assert capi.lib().b200opt_layernorm_bwd(
+            capi.HALF, capi.FLOAT, rows, dim, vp(dy), dim, vp(x), dim, vp(gamma), vp(mean), vp(rstd),
+            vp(out[0]), dim, vp(out[1]), vp(out[2]), 0, vp(ws), ws.numel(), stream) == capi.OK
+        for k in keep:
+            assert torch.equal(out[k], want[k]), (keep, k)
+
+
 def test_layernorm_large_mean_and_non_finite_rows():
     g = gen(5)
     x = normal(g, 6, 777, mean=4096.0, std=1.0, dtype=torch.float32)
@@ -366,7 +389,7 @@ def test_vocab_loss(tokens, vocab, dim):
     assert all(torch.equal(p, q) for p, q in zip(f + b, f2 + b2))
 
 
-@pytest.mark.parametrize("tokens,vocab,dim", [(65, 300, 72), (260, 130, 200), (5, 1001, 64)])
+@pytest.mark.parametrize("tokens,vocab,dim", [(65, 300, 72), (260, 130, 200), (5, 1001, 64), (4100, 300, 72)])
 def test_vocab_loss_strides_sum_accumulate_int32(tokens, vocab, dim):
     x, w, y = head_inputs(tokens, vocab, dim, seed=3)
     xs, _ = strided(x, dim + 8, 8)
@@ -381,8 +404,10 @@ def test_vocab_loss_strides_sum_accumulate_int32(tokens, vocab, dim):
     assert clean_x() and clean_w()
 
 
-def test_vocab_loss_several_pieces_of_the_vocabulary():
-    x, w, y = head_inputs(8200, 20000, 64)
+@pytest.mark.parametrize("tokens,vocab", [(8200, 20000), (9600, 14000)])
+def test_vocab_loss_several_pieces_of_the_vocabulary(tokens, vocab):
+    """With the sums of grad_hidden in parts, and whole."""
+    x, w, y = head_inputs(tokens, vocab, 64)
     f = layers.vocab_loss_forward(x, w, y)
     b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=4096.0)
     check_head(x, w, y, f, b, 4096.0)
@@ -493,6 +518,55 @@ def test_vocab_loss_gradient_against_differences():
     tol += float((r["e_dx"] + half_step(r["dx"], torch.float16)).sum()) / 1024
     diff = float((loss[0] - loss[1]).sum() / (2 * e))
     assert abs(float((dx.double() * s.double()).sum()) / 1024 - diff) <= tol * SLACK
+
+
+# ------------------------------------------------------ offsets over 32 bits
+
+def test_far_offsets():
+    """Tables and activations of more than 2^31 elements: what lies at their ends."""
+    rows, dim = 1_060_000, 2048
+    g = gen(12)
+    big = torch.empty(rows, dim, dtype=torch.float16, device=DEV).normal_(generator=g)
+    ids = torch.tensor([rows - 1, 0, rows - 7, rows, rows - 1, 1_048_576], device=DEV)
+    out = layers.embedding_forward(ids, big)
+    assert torch.equal(out[[0, 1, 2, 5]], big[ids[[0, 1, 2, 5]]]) and (out[3] == 0).all()
+    y, mean, rstd = layers.layernorm_forward(big)
+    tail = slice(rows - 50, rows)
+    ty, tm, tr = layers.layernorm_forward(big[tail].clone())
+    assert torch.equal(y[tail], ty) and torch.equal(mean[tail], tm) and torch.equal(rstd[tail], tr)
+    dx, _, db = layers.layernorm_backward(y, big, None, mean, rstd)
+    tdx, _, _ = layers.layernorm_backward(ty, big[tail].clone(), None, tm, tr)
+    assert torch.equal(dx[tail], tdx)
+    del dx
+    y.fill_(float("nan"))
+    dw = layers.embedding_backward(ids, out, rows, grad_weight=y)
+    assert torch.equal(dw[rows - 7], out[2]) and torch.equal(dw[1_048_576], out[5])
+    two = (out[0].float() * 2).half()
+    assert torch.equal(dw[rows - 1], two)
+    dw[ids[[0, 1, 2, 5]]] = 0
+    assert int(dw.view(torch.int16).count_nonzero()) == 0
+
+
+def test_vocab_loss_far_offsets():
+    tokens, vocab, dim = 70, 530_000, 4096
+    g = gen(13)
+    w = torch.empty(vocab, dim, dtype=torch.float16, device=DEV).normal_(std=0.02, generator=g)
+    x = normal(g, tokens, dim)
+    y = integers(g, tokens, vocab - 300, vocab)
+    loss, lse, stats = layers.vocab_loss_forward(x, w, y)
+    top = torch.full((tokens,), -float("inf"), device=DEV, dtype=torch.float64)
+    for at in range(0, vocab, 53_000):
+        top = torch.logaddexp(top, torch.logsumexp(x.double() @ w[at:at + 53_000].double().t(), 1))
+    e_z = 2 * dim * U * float((x.double().abs().sum(1).max() * 0.12))
+    close(lse, top, e_z + (chain(vocab) + 64) * U + 0 * top)
+    dx, dw = layers.vocab_loss_backward(x, w, y, lse, stats=stats, grad_scale=4096.0)
+    tail = slice(vocab - 400, vocab)
+    p = torch.exp(x.double() @ w[tail].double().t() - top[:, None])
+    p[torch.arange(tokens, device=DEV), y - (vocab - 400)] -= 1
+    f = 4096.0 / tokens
+    want = f * p.t() @ x.double()
+    size = f * p.abs().t() @ x.double().abs()
+    close(dw[tail], want, size * (2.0 ** -11 + 2 * e_z + 2 * tokens * U) + half_step(want, torch.float16))
 
 
 # -------------------------------------------- streams, graphs, several at once
