@@ -95,48 +95,60 @@ struct StatsEpilogue {
     }
 };
 
-// Joins the parts of 32 rows: 16 threads a row, then a tree.  The block that
-// finishes last adds up the blocks' sums of losses, in their order.
+// Joins the parts of kLossRows rows, 64 threads a row.  The block that finishes
+// last adds up the blocks' sums of losses, in their order.
+constexpr int kLossRows = 8;
 __global__ void __launch_bounds__(512)
     loss_kernel(int T, int V, int parts, const float2 *part, const float *zt, const void *y, int wide,
                 float *loss, float *lse, float2 *block_sums, unsigned *done, float *stats)
 {
-    __shared__ float2 red[16][33];
+    __shared__ float2 red[64][kLossRows];
     __shared__ bool last;
-    const int x = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int t = blockIdx.x * 32 + x;
-    float top = -INFINITY, sum = 0.0f;
+    const int x = threadIdx.x % kLossRows, w = threadIdx.x / kLossRows;
+    const int t = blockIdx.x * kLossRows + x;
+    auto add = [](float2 a, float2 b) {  // two (maximum, sum) of disjoint stretches
+        const float m = fmaxf(a.x, b.x);
+        return make_float2(m, (a.y ? a.y * exp2_fast(a.x - m) : 0.0f) + (b.y ? b.y * exp2_fast(b.x - m) : 0.0f));
+    };
+    // asked for now, used at the end
+    const bool valid = t < T && lm_index_at(y, wide, t, V) >= 0;
+    const float target = t < T ? zt[t] : 0.0f;
+    float2 mine = make_float2(-INFINITY, 0.0f);
     if(t < T)
 #pragma unroll 4
-        for(int i = w; i < parts; i += 16) {
-            const float2 p = part[(size_t)i * T + t];
-            const float m = fmaxf(top, p.x);
-            sum = sum * exp2_fast(top - m) + p.y * exp2_fast(p.x - m);
-            top = m;
-        }
-    red[w][x] = make_float2(top, sum);
+        for(int i = w; i < parts; i += 64)
+            mine = add(mine, part[(size_t)i * T + t]);
+    red[w][x] = mine;
     __syncthreads();
-    if(w == 0) {
-        float mine = 0.0f, counted = 0.0f;
-        if(t < T) {
-            const int used = min(16, parts);
-            for(int i = 1; i < used; i++)
-                top = fmaxf(top, red[i][x].x);
-            sum = 0.0f;
-            for(int i = 0; i < used; i++)
-                sum += red[i][x].y * exp2_fast(red[i][x].x - top);
-            const float l = (top + log2f(sum)) * kLn2;
+    if(threadIdx.x < 32) {  // four threads a row, then one
+        float top = mine.x, sum = 0.0f;
+#pragma unroll
+        for(int i = 1; i < 16; i++)
+            top = fmaxf(top, red[w + 4 * i][x].x);
+#pragma unroll
+        for(int i = 0; i < 16; i++) {
+            const float2 p = red[w + 4 * i][x];
+            sum += p.y ? p.y * exp2_fast(p.x - top) : 0.0f;
+        }
+        mine = make_float2(top, sum);
+#pragma unroll
+        for(int o = 16; o >= kLossRows; o >>= 1)
+            mine = add(mine, make_float2(__shfl_xor_sync(0xffffffffu, mine.x, o),
+                                         __shfl_xor_sync(0xffffffffu, mine.y, o)));
+        float own = 0.0f, counted = 0.0f;
+        if(t < T && w == 0) {
+            const float l = (mine.x + log2f(mine.y)) * kLn2;
             lse[t] = l;
-            if(lm_index_at(y, wide, t, V) >= 0) {
-                mine = l - zt[t];
+            if(valid) {
+                own = l - target;
                 counted = 1.0f;
             }
-            loss[t] = mine;
+            loss[t] = own;
         }
-        mine = warp_sum(mine);
+        own = warp_sum(own);
         counted = warp_sum(counted);
-        if(x == 0 && stats) {
-            block_sums[blockIdx.x] = make_float2(mine, counted);
+        if(threadIdx.x == 0 && stats) {
+            block_sums[blockIdx.x] = make_float2(own, counted);
             __threadfence();
             last = atomicAdd(done, 1) == gridDim.x - 1;
         }
@@ -147,21 +159,25 @@ __global__ void __launch_bounds__(512)
     if(!last)
         return;
     __threadfence();
-    float mine = 0.0f;
+    float sum = 0.0f;
     int counted = 0;
     for(int i = threadIdx.x; i < (int)gridDim.x; i += 512) {
         const float2 p = __ldcg(block_sums + i);
-        mine += p.x;
+        sum += p.x;
         counted += (int)p.y;
     }
-    float *slots = &red[0][0].x;
-    mine = block_sum(mine, slots);
-    // whole numbers in two parts, each of which fp32 holds exactly
-    const float hi = block_sum((float)(counted >> 12), slots);
-    const float lo = block_sum((float)(counted & 4095), slots);
+    sum = warp_sum(sum);
+    counted = __reduce_add_sync(0xffffffffu, counted);
+    if((threadIdx.x & 31) == 0)
+        red[threadIdx.x >> 5][0] = make_float2(sum, __int_as_float(counted));
+    __syncthreads();
     if(threadIdx.x == 0) {
-        stats[0] = mine;
-        stats[1] = hi * 4096.0f + lo;
+        for(int i = 1; i < 16; i++) {
+            sum += red[i][0].x;
+            counted += __float_as_int(red[i][0].y);
+        }
+        stats[0] = sum;
+        stats[1] = (float)counted;
     }
 }
 
@@ -546,7 +562,7 @@ struct FwdPlan {
     FwdPlan(size_t T, size_t V)
     {
         at_sums = lm_up(T * 4, 256);
-        at_done = at_sums + lm_up((T + 31) / 32 * 8, 256);
+        at_done = at_sums + lm_up((T + kLossRows - 1) / kLossRows * 8, 256);
         at_part = at_done + 256;
         bytes = at_part + tiles_of(V) * T * 8;
     }
@@ -601,7 +617,7 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
         TcShape s = {T, V, (int)dim, nullptr, 0, 0, 0, 0, 1, 16};
         if(!tc_launch<false, false>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt, done}, sms, st))
             return B200OPT_ECUDA;
-        loss_kernel<<<(unsigned)((tokens + 31) / 32), 512, 0, st>>>(
+        loss_kernel<<<(unsigned)((tokens + kLossRows - 1) / kLossRows), 512, 0, st>>>(
             T, V, (int)tiles_of(vocab), part, zt, targets, wide, loss, lse, (float2 *)(ws + p.at_sums), done,
             stats);
     } else {

@@ -36,10 +36,9 @@ def _dtype(t, what):
 
 def _device(t, what):
     """Index of the CUDA device that the tensor is on."""
-    index = t.get_device() if isinstance(t, torch.Tensor) else -1
-    if index < 0 or not t.is_cuda:
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError(f"{what} must be a CUDA tensor")
-    return index
+    return t.get_device()
 
 
 def _on(index, what, t):
@@ -95,6 +94,14 @@ def _vector(t, what, n, dtype, index):
     if t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{what} must be contiguous with {n} elements")
     return t.data_ptr()
+
+
+def _vector_out(t, what, shape, n, dtype, like, index, stream):
+    """(tensor, address) of a vector that a call fills: the caller's, or a new one."""
+    if t is None:
+        t = _new(like, shape, dtype, what, stream)
+        return t, t.data_ptr()
+    return t, _vector(t, what, n, dtype, index)
 
 
 def _index(t, what, index):
@@ -198,15 +205,11 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None, mean=None, r
         out, ys = _new(x, x.shape, x.dtype, "out", stream), max(dim, 1)
     else:
         ys = _matrix(out, "out", rows, dim, x.dtype, dev)
-    if mean is None:
-        mean = _new(x, x.shape[:-1], torch.float32, "mean", stream)
-    if rstd is None:
-        rstd = _new(x, x.shape[:-1], torch.float32, "rstd", stream)
+    mean, mp = _vector_out(mean, "mean", x.shape[:-1], rows, torch.float32, x, dev, stream)
+    rstd, rp = _vector_out(rstd, "rstd", x.shape[:-1], rows, torch.float32, x, dev, stream)
     _call(lib().b200opt_layernorm_fwd, dev, stream, dtype, _DTYPES.get(params, -1), rows, dim,
           x.data_ptr(), xs, _vector(gamma, "gamma", dim, params, dev),
-          _vector(beta, "beta", dim, params, dev), eps, out.data_ptr(), ys,
-          _vector(mean, "mean", rows, torch.float32, dev),
-          _vector(rstd, "rstd", rows, torch.float32, dev))
+          _vector(beta, "beta", dim, params, dev), eps, out.data_ptr(), ys, mp, rp)
     return out, mean, rstd
 
 
@@ -229,17 +232,14 @@ def layernorm_backward(grad_y, x, gamma, mean, rstd, grad_x=None, grad_gamma=Non
         grad_x, dxs = _new(x, x.shape, x.dtype, "grad_x", stream), max(dim, 1)
     else:
         dxs = _matrix(grad_x, "grad_x", rows, dim, x.dtype, dev)
-    if grad_gamma is None:
-        grad_gamma = _new(x, (dim,), params, "grad_gamma", stream)
-    if grad_beta is None:
-        grad_beta = _new(x, (dim,), params, "grad_beta", stream)
+    grad_gamma, gp = _vector_out(grad_gamma, "grad_gamma", (dim,), dim, params, x, dev, stream)
+    grad_beta, bp = _vector_out(grad_beta, "grad_beta", (dim,), dim, params, x, dev, stream)
     keep, wp, wb = _workspace(workspace, layernorm_workspace(rows, dim), x, dev, stream)
     _call(lib().b200opt_layernorm_bwd, dev, stream, dtype, _DTYPES.get(params, -1), rows, dim,
           grad_y.data_ptr(), ys, x.data_ptr(), xs, _vector(gamma, "gamma", dim, params, dev),
           _vector(mean, "mean", rows, torch.float32, dev),
-          _vector(rstd, "rstd", rows, torch.float32, dev), grad_x.data_ptr(), dxs,
-          _vector(grad_gamma, "grad_gamma", dim, params, dev),
-          _vector(grad_beta, "grad_beta", dim, params, dev), int(accumulate), wp, wb)
+          _vector(rstd, "rstd", rows, torch.float32, dev), grad_x.data_ptr(), dxs, gp, bp,
+          int(accumulate), wp, wb)
     return grad_x, grad_gamma, grad_beta
 
 
@@ -266,18 +266,13 @@ def vocab_loss_forward(hidden, weight, targets, loss=None, lse=None, stats=None,
     stored.  loss and lse: fp32 per token; stats: fp32 {sum of losses, tokens counted}.  Targets
     outside the vocabulary are ignored."""
     dev, sizes, args = _head(hidden, weight, targets)
-    if loss is None:
-        loss = _new(hidden, targets.shape, torch.float32, "loss", stream)
-    if lse is None:
-        lse = _new(hidden, targets.shape, torch.float32, "lse", stream)
-    if stats is None:
-        stats = _new(hidden, (2,), torch.float32, "stats", stream)
+    n, shape, f32 = sizes[0], targets.shape, torch.float32
+    loss, lp = _vector_out(loss, "loss", shape, n, f32, hidden, dev, stream)
+    lse, ep = _vector_out(lse, "lse", shape, n, f32, hidden, dev, stream)
+    stats, sp = _vector_out(stats, "stats", (2,), 2, f32, hidden, dev, stream)
     keep, wp, wb = _workspace(workspace, _bytes("b200opt_vocab_loss_fwd_workspace", *sizes), hidden,
                               dev, stream)
-    _call(lib().b200opt_vocab_loss_fwd, dev, stream, *sizes, *args,
-          _vector(loss, "loss", sizes[0], torch.float32, dev),
-          _vector(lse, "lse", sizes[0], torch.float32, dev),
-          _vector(stats, "stats", 2, torch.float32, dev), wp, wb)
+    _call(lib().b200opt_vocab_loss_fwd, dev, stream, *sizes, *args, lp, ep, sp, wp, wb)
     return loss, lse, stats
 
 
