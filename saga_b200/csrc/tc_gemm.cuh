@@ -7,8 +7,10 @@
 // cta_group::2 instruction stream: each CTA holds 128 rows of A and 128 rows of
 // B in shared memory and 128 rows x 256 columns of the result in its tensor
 // memory.  A single CTA's 128 x 256 tile would fetch 1.5 times as many bytes from
-// L2 for the same arithmetic (85 against 128 flops a byte), which at the measured
-// tensor rate is more than L2 delivers.
+// L2 for the same arithmetic (85 against 128 flops a byte).  At 4096 x 50021 x 2048
+// the product with the losses in its epilogue takes 577 us, 1.45 PFLOP/s or 0.88 of
+// the measured bf16 rate; long runs are bound by the power limit (8192 x 128000 x
+// 4096: 6.7 ms, 1.28 PFLOP/s, 0.90 of the measured sustained rate).
 //
 // Either operand may be "K-major" (k contiguous in memory) or "MN-major" (m or n
 // contiguous): TMA brings boxes of 64 contiguous elements (128 bytes, swizzled)
@@ -17,7 +19,8 @@
 //
 // Warps: 0 issues the TMA loads, 1 (of the even CTA) the MMAs, 2 owns the tensor
 // memory, 4..19 are the epilogue.  Two accumulators alternate, so the epilogue
-// of a tile runs beside the main loop of the next one.
+// of a tile runs beside the main loop of the next one; a wide tile has both, and
+// its halves are skewed to the same end.
 //
 // Every wait is bounded: one that runs out makes the epilogue write NaN for the
 // tiles it did not get, which the loss and the optimizer's overflow flags show.
@@ -29,16 +32,22 @@
 
 namespace b200 {
 
-constexpr int kTcTile = 256;    // tile of a CTA pair, both ways
+constexpr int kTcTile = 256;    // tile of a CTA pair, both ways; a wide one is 256 x 512
 constexpr int kTcHalf = 128;    // a CTA's rows of A, of B and of the result
 constexpr int kTcK = 64;        // k per stage: 128 bytes, the swizzle's span
-constexpr int kTcStages = 5;
 constexpr int kTcOperand = kTcHalf * kTcK * 2;  // bytes of one operand of a stage in a CTA
 constexpr int kTcEpilogue = 16;  // warps: four for each 32 rows, 64 columns each
 constexpr int kTcColumns = kTcTile / (kTcEpilogue / 4);
 constexpr int kTcThreads = 128 + 32 * kTcEpilogue;
-constexpr int kTcStaging = 4096;  // bytes an epilogue warp turns its columns around in
-constexpr int kTcSmem = kTcStages * 2 * kTcOperand + kTcEpilogue * kTcStaging + 1024;
+// Stages of A and of NH times 128 rows of B, the bytes in which each epilogue warp
+// turns its columns around, and the dynamic shared memory of it all.
+__host__ __device__ constexpr int tc_stages(int nh) { return nh == 1 ? 5 : 4; }
+__host__ __device__ constexpr int tc_staging(int nh) { return nh == 1 ? 4096 : 2048; }
+__host__ __device__ constexpr int tc_stage_bytes(int nh) { return (1 + nh) * kTcOperand; }
+constexpr int tc_smem(int nh)
+{
+    return tc_stages(nh) * tc_stage_bytes(nh) + kTcEpilogue * tc_staging(nh) + 1024;
+}
 
 struct TcShape {
     // sizes in elements; a dynamic size is read from *count on the device
@@ -222,12 +231,12 @@ struct Turn {
 // host has made sure that their number fits 31 bits.
 struct TcTiles {
     uint32_t mt, nt, group, splits, kblocks;
-    __device__ __forceinline__ TcTiles(const TcShape &s)
+    __device__ __forceinline__ TcTiles(const TcShape &s, int columns)
     {
         const int c = s.dyn_m || s.dyn_k ? max(*s.count, 1) : 0;
         const int m = s.dyn_m ? c : s.m, k = s.dyn_k ? c : s.k;
         mt = (m + kTcTile - 1) / kTcTile;
-        nt = (s.n + kTcTile - 1) / kTcTile;
+        nt = (s.n + columns - 1) / columns;
         kblocks = (k + kTcK - 1) / kTcK;
         group = s.group;
         splits = tc_parts_of(s, m);
@@ -257,11 +266,12 @@ struct TcTiles {
 // lanes of a warp together; end(state, row, col, acc, shared) closes them, where
 // `shared` is the staging memory of all epilogue warps.  Rows and columns beyond the matrix come too and are for the epilogue to
 // leave out.
-template <bool A_MN, bool B_MN, typename Epi>
+template <bool A_MN, bool B_MN, int NH, typename Epi>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     tc_gemm_kernel(const __grid_constant__ CUtensorMap map_a, const __grid_constant__ CUtensorMap map_b,
                    const TcShape shape, const Epi epi)
 {
+    constexpr int kTcStages = tc_stages(NH), kStageBytes = tc_stage_bytes(NH);
     extern __shared__ char smem_raw[];
     __shared__ __align__(8) uint64_t full[kTcStages], empty[kTcStages], acc_full[2], acc_empty[2];
     __shared__ uint32_t tmem_slot;
@@ -296,7 +306,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
 
-    const TcTiles tiles(shape);
+    const TcTiles tiles(shape, NH * kTcTile);
     const uint32_t total = tiles.count(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
 
     if(warp == 0 && lane == 0) {
@@ -306,16 +316,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         for(uint32_t i = pair; ok && i < total; i += pairs) {
             int m, n, part, k0, k1;
             tiles.at(i, m, n, part, k0, k1);
-            const int am = m * kTcTile + (int)rank * kTcHalf, bn = n * kTcTile + (int)rank * kTcHalf;
+            const int am = m * kTcTile + (int)rank * kTcHalf, bn = n * NH * kTcTile + (int)rank * kTcHalf;
             for(int kb = k0; kb < k1; kb++) {
                 if(!(ok = mbar_wait(smem_u32(&empty[stage]), phase ^ 1, dead)))
                     break;
-                const uint32_t a = base + stage * 2 * kTcOperand, b = a + kTcOperand;
+                const uint32_t a = base + stage * kStageBytes;
                 const uint32_t bar = map_to(smem_u32(&full[stage]), 0);
                 if(rank == 0)
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(
                                      smem_u32(&full[stage])),
-                                 "r"(4 * kTcOperand)
+                                 "r"(2 * kStageBytes)
                                  : "memory");
                 const int k = kb * kTcK;
                 if(A_MN) {
@@ -324,11 +334,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
                 } else {
                     tma_load(a, &map_a, k, shape.a_row0 + am, bar);
                 }
-                if(B_MN) {
-                    tma_load(b, &map_b, bn, shape.b_row0 + k, bar);
-                    tma_load(b + kTcOperand / 2, &map_b, bn + 64, shape.b_row0 + k, bar);
-                } else {
-                    tma_load(b, &map_b, k, shape.b_row0 + bn, bar);
+#pragma unroll
+                for(int h = 0; h < NH; h++) {
+                    const uint32_t b = a + (1 + h) * kTcOperand;
+                    const int at = bn + h * kTcTile;
+                    if(B_MN) {
+                        tma_load(b, &map_b, at, shape.b_row0 + k, bar);
+                        tma_load(b + kTcOperand / 2, &map_b, at + 64, shape.b_row0 + k, bar);
+                    } else {
+                        tma_load(b, &map_b, k, shape.b_row0 + at, bar);
+                    }
                 }
                 if(++stage == kTcStages) {
                     stage = 0;
@@ -344,41 +359,100 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
         int stage = 0, acc = 0;
         uint32_t phase = 0, acc_phase = 0;
         bool ok = true;
+        // one stage's product into accumulator `to`, with B's half h
+        auto multiply = [&](int of, int h, int to, bool add) {
+            const uint32_t a = base + of * kStageBytes;
+            uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + (1 + h) * kTcOperand);
+#pragma unroll
+            for(int s = 0; s < kTcK / 16; s++) {
+                mma(tmem + to * kTcTile, da, db, idesc, add || s);
+                da += k_step<A_MN>();
+                db += k_step<B_MN>();
+            }
+        };
+        auto arrived = [&](int of, uint32_t parity) {
+            const bool got = mbar_wait(smem_u32(&full[of]), parity, dead);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            return got;
+        };
+        auto next = [&](int &of, uint32_t &parity) {
+            if(++of == kTcStages) {
+                of = 0;
+                parity ^= 1;
+            }
+        };
+        auto emptied = [&](int which, uint32_t parity) {
+            const bool got = mbar_wait(smem_u32(&acc_empty[which]), parity, dead);
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            return got;
+        };
         for(uint32_t i = pair; ok && i < total; i += pairs) {
             int m, n, part, k0, k1;
             tiles.at(i, m, n, part, k0, k1);
-            if(!(ok = mbar_wait(smem_u32(&acc_empty[acc]), acc_phase ^ 1, dead)))
-                break;
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-            for(int kb = k0; kb < k1; kb++) {
-                if(!(ok = mbar_wait(smem_u32(&full[stage]), phase, dead)))
+            if constexpr(NH == 1) {
+                if(!(ok = emptied(acc, acc_phase ^ 1)))
                     break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t a = base + stage * 2 * kTcOperand;
-                uint64_t da = operand_desc<A_MN>(a), db = operand_desc<B_MN>(a + kTcOperand);
-#pragma unroll
-                for(int s = 0; s < kTcK / 16; s++) {
-                    mma(tmem + acc * kTcTile, da, db, idesc, kb > k0 || s);
-                    da += k_step<A_MN>();
-                    db += k_step<B_MN>();
+                for(int kb = k0; kb < k1; kb++) {
+                    if(!(ok = arrived(stage, phase)))
+                        break;
+                    multiply(stage, 0, acc, kb > k0);
+                    mma_commit(smem_u32(&empty[stage]));
+                    next(stage, phase);
                 }
-                mma_commit(smem_u32(&empty[stage]));
-                if(++stage == kTcStages) {
-                    stage = 0;
-                    phase ^= 1;
+                if(ok)
+                    mma_commit(smem_u32(&acc_full[acc]));
+                if(++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1;
                 }
-            }
-            if(ok)
-                mma_commit(smem_u32(&acc_full[acc]));
-            if(++acc == 2) {
-                acc = 0;
+            } else {
+                // Both accumulators are one tile's.  At its start and at its end the
+                // first half runs ahead by as many stages as there are: the epilogue of
+                // one half then runs beside the main loop of the other.
+                const int all = k1 - k0, head = min(all, kTcStages), tail = min(all - head, kTcStages);
+                int done = 0;
+                auto skewed = [&](int count, bool first) {
+                    int of = stage;
+                    uint32_t parity = phase;
+                    for(int j = 0; ok && j < count; j++) {
+                        if((ok = arrived(of, parity)))
+                            multiply(of, 0, 0, !first || j);
+                        next(of, parity);
+                    }
+                    if(ok && done + count == all)
+                        mma_commit(smem_u32(&acc_full[0]));
+                    if(first)
+                        ok = ok && emptied(1, acc_phase ^ 1);
+                    for(int j = 0; ok && j < count; j++) {
+                        multiply(stage, 1, 1, !first || j);
+                        mma_commit(smem_u32(&empty[stage]));
+                        next(stage, phase);
+                    }
+                    done += count;
+                    if(ok && done == all)
+                        mma_commit(smem_u32(&acc_full[1]));
+                };
+                if(!(ok = emptied(0, acc_phase ^ 1)))
+                    break;
+                skewed(head, true);
+                for(int j = head; ok && j < all - tail; j++) {
+                    if(!(ok = arrived(stage, phase)))
+                        break;
+                    multiply(stage, 0, 0, true);
+                    multiply(stage, 1, 1, true);
+                    mma_commit(smem_u32(&empty[stage]));
+                    next(stage, phase);
+                    done++;
+                }
+                if(ok && tail)
+                    skewed(tail, false);
                 acc_phase ^= 1;
             }
         }
     } else if(warp >= 4) {
         const int quad = warp & 3, side = (warp - 4) >> 2;
-        char *const shared = smem_raw + (base - smem_u32(smem_raw)) + kTcStages * 2 * kTcOperand;
-        char *const staging = shared + (warp - 4) * kTcStaging;
+        char *const shared = smem_raw + (base - smem_u32(smem_raw)) + kTcStages * kStageBytes;
+        char *const staging = shared + (warp - 4) * tc_staging(NH);
         const auto common = epi.common();
         int acc = 0;
         uint32_t acc_phase = 0;
@@ -387,32 +461,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
             int m, n, part, k0, k1;
             tiles.at(i, m, n, part, k0, k1);
             const int row = m * kTcTile + (int)rank * kTcHalf + quad * 32 + lane;
-            const int col = n * kTcTile + side * kTcColumns;
-            const uint32_t from =
-                tmem + ((uint32_t)(quad * 32) << 16) + acc * kTcTile + side * kTcColumns;
-            auto state = epi.begin(common, row, col, part);  // its loads run during the wait
-            ok = ok && mbar_wait(smem_u32(&acc_full[acc]), acc_phase, dead);
-            ok = __all_sync(0xffffffffu, ok);
-            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
 #pragma unroll 1
-            for(int c = 0; c < kTcColumns; c += 32) {
-                float v[32];
-                tmem_load(from + c, v);
-                tmem_wait(v);
-                if(!ok || k1 == k0)
-                    no_result(v, ok);
-                epi.columns(common, state, row, col + c, v, staging);
-            }
-            epi.end(state, row, col, acc, shared);
-            asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-            __syncwarp();
-            if(lane == 0)
-                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
-                                 map_to(smem_u32(&acc_empty[acc]), 0))
-                             : "memory");
-            if(++acc == 2) {
-                acc = 0;
-                acc_phase ^= 1;
+            for(int h = 0; h < NH; h++) {
+                const int col = (n * NH + h) * kTcTile + side * kTcColumns;
+                const uint32_t from =
+                    tmem + ((uint32_t)(quad * 32) << 16) + acc * kTcTile + side * kTcColumns;
+                auto state = epi.begin(common, row, col, part);  // its loads run during the wait
+                ok = ok && mbar_wait(smem_u32(&acc_full[acc]), acc_phase, dead);
+                ok = __all_sync(0xffffffffu, ok);
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll 1
+                for(int c = 0; c < kTcColumns; c += 32) {
+                    float v[32];
+                    tmem_load(from + c, v);
+                    tmem_wait(v);
+                    if(!ok || k1 == k0)
+                        no_result(v, ok);
+                    epi.columns(common, state, row, col + c, v, staging);
+                }
+                epi.end(state, row, col, acc, shared);
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                if(lane == 0)
+                    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(
+                                     map_to(smem_u32(&acc_empty[acc]), 0))
+                                 : "memory");
+                if(++acc == 2) {
+                    acc = 0;
+                    acc_phase ^= 1;
+                }
             }
         }
     }
@@ -459,20 +536,39 @@ inline bool tc_map(CUtensorMap *map, const void *p, size_t rows, size_t cols, si
 // rows of a box: an operand's 128 rows when k is contiguous, 64 k otherwise
 constexpr unsigned tc_box(bool mn) { return mn ? kTcK : kTcHalf; }
 
-template <bool A_MN, bool B_MN, typename Epi>
+// Whether a product of two MN-major operands is faster in wide tiles, which fetch a
+// quarter less per flop: 9 % in grad_weight's product (16384 x 4096, 8192 tokens:
+// 980 us narrow, 912 wide; 512 columns: 116 and 98), nothing with K-major operands,
+// whose callers keep to narrow ones (losses of 8192 x 128000, 512 columns: 876 us
+// narrow, 982 wide).  There are half as many wide tiles to spread over the pairs, so
+// they are taken where the turns that the pairs make, counted in narrow tiles, grow
+// by less than that gain.
+inline bool tc_wide(long long m, long long n, int sms)
+{
+    const long long mt = (m + kTcTile - 1) / kTcTile, pairs = sms / 2 > 0 ? sms / 2 : 1;
+    const long long narrow = mt * ((n + kTcTile - 1) / kTcTile);
+    const long long wide = mt * ((n + 2 * kTcTile - 1) / (2 * kTcTile));
+    const long long turns = (narrow + pairs - 1) / pairs, turns2 = 2 * ((wide + pairs - 1) / pairs);
+    return 100 * turns2 <= 109 * turns;
+}
+
+template <bool A_MN, bool B_MN, int NH, typename Epi>
 bool tc_launch(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, const Epi &epi, int sms,
                cudaStream_t st)
 {
-    auto *kernel = tc_gemm_kernel<A_MN, B_MN, Epi>;
+    auto *kernel = tc_gemm_kernel<A_MN, B_MN, NH, Epi>;
     static std::atomic<uint64_t> allowed{0};
-    if(!lm_allow_smem(kernel, kTcSmem, allowed))
+    if(!lm_allow_smem(kernel, tc_smem(NH), allowed))
         return false;
     // (as many pairs as planned for, where the device may find more parts)
-    const long long tiles = s.splits > 1 && s.dyn_m ? kTcPlanPairs : (s.m + kTcTile - 1ll) / kTcTile * ((s.n + kTcTile - 1ll) / kTcTile) * s.splits;
+    const long long tiles = s.splits > 1 && s.dyn_m
+                                ? kTcPlanPairs
+                                : (s.m + kTcTile - 1ll) / kTcTile *
+                                      ((s.n + NH * kTcTile - 1ll) / (NH * kTcTile)) * s.splits;
     const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
     if(tiles > 0x7fffffff)
         return false;
-    kernel<<<(unsigned)(2 * pairs), kTcThreads, kTcSmem, st>>>(a, b, s, epi);
+    kernel<<<(unsigned)(2 * pairs), kTcThreads, tc_smem(NH), st>>>(a, b, s, epi);
     return true;
 }
 

@@ -449,13 +449,13 @@ struct OutEpilogue {
 };
 
 // A product into its result; false when it could not be launched.
-template <bool A_MN, bool B_MN, int MODE>
+template <bool A_MN, bool B_MN, int NH, int MODE>
 bool product(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, int m, const int *count, int n,
              float *sum, int add, __half *out, size_t stride, const int *rows,
              const Factor &factor, int sms, cudaStream_t st)
 {
     const OutEpilogue<MODE> e = {m, count, n, sum, add, out, stride, rows, factor};
-    return tc_launch<A_MN, B_MN>(a, b, s, e, sms, st);
+    return tc_launch<A_MN, B_MN, NH>(a, b, s, e, sms, st);
 }
 
 // Joins the parts of a product that was cut along k, in their order.
@@ -615,7 +615,7 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
            !tc_map(&mw, weight, vocab, dim, weight_stride, tc_box(false)))
             return B200OPT_ECUDA;
         TcShape s = {T, V, (int)dim, nullptr, 0, 0, 0, 0, 1, 16};
-        if(!tc_launch<false, false>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt, done}, sms, st))
+        if(!tc_launch<false, false, 1>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt, done}, sms, st))
             return B200OPT_ECUDA;
         loss_kernel<<<(unsigned)((tokens + kLossRows - 1) / kLossRows), 512, 0, st>>>(
             T, V, (int)tiles_of(vocab), part, zt, targets, wide, loss, lse, (float2 *)(ws + p.at_sums), done,
@@ -700,15 +700,15 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
             return B200OPT_ECUDA;
         // dz = p - onehot
         TcShape s = {T, N, D, count, 1, 0, 0, at, 1, 16};
-        if(!tc_launch<false, false>(x_k, w_k, s, DzEpilogue{count, lsec, target, at, dz, p.piece}, sms, st))
+        if(!tc_launch<false, false, 1>(x_k, w_k, s, DzEpilogue{count, lsec, target, at, dz, p.piece}, sms, st))
             return B200OPT_ECUDA;
         if(grad_hidden) {  // += dz W
             const bool direct = p.x_parts == 1 && last;
             s = {T, D, N, count, 1, 0, 0, at, (int)p.x_parts, 8, (int)(p.x_parts * tokens),
                  (int)((std::min(p.piece, vocab) + kTcK - 1) / kTcK)};
-            auto *run = !direct ? product<false, true, kSums>
-                        : begin ? product<false, true, kOut>
-                                : product<false, true, kLast>;
+            auto *run = !direct ? product<false, true, 1, kSums>
+                        : begin ? product<false, true, 1, kOut>
+                                : product<false, true, 1, kLast>;
             if(!run(dz_k, w_mn, s, T, count, D, xsum, !begin, (__half *)grad_hidden,
                     grad_hidden_stride, from, factor, sms, st))
                 return B200OPT_ECUDA;
@@ -719,9 +719,12 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
         if(grad_weight) {  // = dz^T X
             __half *to = (__half *)grad_weight + first * grad_weight_stride;
             s = {N, D, T, count, 0, 1, 0, 0, (int)p.w_parts, 8};
-            auto *run = p.w_parts > 1 ? product<true, true, kSums>
-                        : accumulate  ? product<true, true, kAccumulate>
-                                      : product<true, true, kOut>;
+            const bool wide_tiles = tc_wide(N, D, sms);
+            auto *run = p.w_parts > 1 ? product<true, true, 1, kSums>
+                        : accumulate  ? (wide_tiles ? product<true, true, 2, kAccumulate>
+                                                    : product<true, true, 1, kAccumulate>)
+                                      : (wide_tiles ? product<true, true, 2, kOut>
+                                                    : product<true, true, 1, kOut>);
             if(!run(dz_mn, x_mn, s, N, nullptr, D, wsum, 0, to, grad_weight_stride, nullptr,
                     factor, sms, st))
                 return B200OPT_ECUDA;

@@ -404,6 +404,19 @@ def test_vocab_loss_strides_sum_accumulate_int32(tokens, vocab, dim):
     assert clean_x() and clean_w()
 
 
+@pytest.mark.parametrize("tokens,vocab,dim,accumulate", [
+    (300, 9400, 520, False), (300, 9400, 520, True), (40, 9300, 1024, False), (700, 9400, 1000, True)])
+def test_vocab_loss_wide_tiles(tokens, vocab, dim, accumulate):
+    """Enough of the table's gradient for tiles of 512 columns, the last of them ragged or whole,
+    with fewer and with more stages of tokens than the ring holds."""
+    x, w, y = head_inputs(tokens, vocab, dim, seed=9)
+    base = normal(gen(2), vocab, dim) if accumulate else None
+    f = layers.vocab_loss_forward(x, w, y)
+    b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=512.0, accumulate=accumulate,
+                                   grad_weight=base.clone() if accumulate else None)
+    check_head(x, w, y, f, b, 512.0, base=base)
+
+
 @pytest.mark.parametrize("tokens,vocab", [(8200, 20000), (9600, 14000)])
 def test_vocab_loss_several_pieces_of_the_vocabulary(tokens, vocab):
     """With the sums of grad_hidden in parts, and whole."""
