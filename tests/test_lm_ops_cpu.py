@@ -24,7 +24,7 @@ def _need(name, *sizes):
 
 EMB_FWD = dict(dtype=capi.HALF, tokens=5, vocab=10, dim=16, ids=A, ib=8, w=A, ws=16, scale=1.0,
                out=A, os=16, stream=None)
-EMB_BWD = dict(dtype=capi.HALF, tokens=5, vocab=10, dim=16, ids=A, ib=8, dy=A, ys=16, scale=1.0,
+EMB_BWD = dict(dtype=capi.HALF, tokens=500, vocab=10, dim=16, ids=A, ib=8, dy=A, ys=16, scale=1.0,
                dw=A, ws=16, acc=0, wk=A, wb=1 << 40, stream=None)
 LN_FWD = dict(dtype=capi.HALF, pdtype=capi.HALF, rows=5, dim=16, x=A, xs=16, g=A, b=A, eps=1e-5,
               y=A, ys=16, mean=A, rstd=A, stream=None)

@@ -71,7 +71,8 @@ def strided(t, stride, shift=0):
 
 EMB_SIZES = [  # tokens, vocab, dim
     (1, 1, 1), (1, 1000, 64), (7, 3, 5), (64, 1000, 333), (1000, 17, 40), (1025, 5003, 96),
-    (300, 300, 1032), (2049, 1, 24), (33, 70001, 8), (20011, 211, 16), (50, 700, 2304), (40, 20, 70000)]
+    (300, 300, 1032), (2049, 1, 24), (33, 70001, 8), (20011, 211, 16), (50, 700, 2304), (40, 20, 70000),
+    (128, 1000, 333), (129, 1000, 333), (100, 50021, 520), (120, 5, 2304), (300, 700, 2304)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
@@ -126,8 +127,8 @@ def test_embedding_backward(tokens, vocab, dim, dtype):
     close(got[n > 0], total[n > 0], (tol + total.abs() * U + half_step(total, dtype))[n > 0])
 
 
-@pytest.mark.parametrize("pattern", ["none", "all the same", "sorted", "reversed", "two"])
-@pytest.mark.parametrize("tokens", [31, 32, 33, 4096, 16384, 16385, 40000])
+@pytest.mark.parametrize("pattern", ["none", "all the same", "sorted", "reversed", "two", "one block"])
+@pytest.mark.parametrize("tokens", [31, 32, 33, 127, 128, 129, 4096, 16384, 16385, 40000])
 def test_embedding_backward_orders(tokens, pattern):
     """Orders of ids that leave a sort or a split of a long run nothing to hide behind."""
     g, vocab, dim = gen(tokens), 30011, 24
@@ -136,7 +137,8 @@ def test_embedding_backward_orders(tokens, pattern):
            "all the same": lambda: torch.full((tokens,), vocab - 1, device=DEV),
            "sorted": lambda: integers(g, tokens, 0, vocab).sort().values,
            "reversed": lambda: integers(g, tokens, 0, vocab).sort(descending=True).values,
-           "two": lambda: torch.where(integers(g, tokens, 0, 2) > 0, 29999, 3)}[pattern]()
+           "two": lambda: torch.where(integers(g, tokens, 0, 2) > 0, 29999, 3),
+           "one block": lambda: torch.arange(tokens, device=DEV) % 50 * (593 if tokens <= 128 else 148)}[pattern]()
     exact, tol, n = embedding_exact(ids, dy, vocab, 1.0)
     close(layers.embedding_backward(ids, dy, vocab), exact, tol + half_step(exact, dy.dtype))
 
