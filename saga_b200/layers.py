@@ -97,9 +97,11 @@ def _vector(t, what, n, dtype, index):
 
 
 def _vector_out(t, what, shape, n, dtype, like, index, stream):
-    """(tensor, address) of a vector that a call fills: the caller's, or a new one."""
+    """(tensor, address) of a vector that a call fills: the caller's, or a new one (made after
+    `like` where that is such a vector already, which is cheaper)."""
     if t is None:
-        t = _new(like, shape, dtype, what, stream)
+        t = (_new_like(like, what, stream) if like.dtype == dtype and like.shape == shape
+             else _new(like, shape, dtype, what, stream))
         return t, t.data_ptr()
     return t, _vector(t, what, n, dtype, index)
 
@@ -117,6 +119,13 @@ def _new(like, shape, dtype, what, stream):
     if stream is not None:
         raise ValueError(f"pass {what} when a raw stream is given")
     return like.new_empty(shape, dtype=dtype)
+
+
+def _new_like(t, what, stream):
+    """A contiguous tensor of t's shape and type."""
+    if stream is not None:
+        raise ValueError(f"pass {what} when a raw stream is given")
+    return torch.empty_like(t) if t.is_contiguous() else t.new_empty(t.shape)
 
 
 @functools.lru_cache(maxsize=1024)
@@ -202,11 +211,11 @@ def layernorm_forward(x, gamma=None, beta=None, eps=1e-5, out=None, mean=None, r
     given = gamma if gamma is not None else beta
     params = given.dtype if given is not None else torch.float32
     if out is None:
-        out, ys = _new(x, x.shape, x.dtype, "out", stream), max(dim, 1)
+        out, ys = _new_like(x, "out", stream), max(dim, 1)
     else:
         ys = _matrix(out, "out", rows, dim, x.dtype, dev)
     mean, mp = _vector_out(mean, "mean", x.shape[:-1], rows, torch.float32, x, dev, stream)
-    rstd, rp = _vector_out(rstd, "rstd", x.shape[:-1], rows, torch.float32, x, dev, stream)
+    rstd, rp = _vector_out(rstd, "rstd", x.shape[:-1], rows, torch.float32, mean, dev, stream)
     _call(lib().b200opt_layernorm_fwd, dev, stream, dtype, _DTYPES.get(params, -1), rows, dim,
           x.data_ptr(), xs, _vector(gamma, "gamma", dim, params, dev),
           _vector(beta, "beta", dim, params, dev), eps, out.data_ptr(), ys, mp, rp)
@@ -229,11 +238,11 @@ def layernorm_backward(grad_y, x, gamma, mean, rstd, grad_x=None, grad_gamma=Non
     if accumulate and (grad_gamma is None or grad_beta is None):
         raise ValueError("accumulate needs grad_gamma and grad_beta")
     if grad_x is None:
-        grad_x, dxs = _new(x, x.shape, x.dtype, "grad_x", stream), max(dim, 1)
+        grad_x, dxs = _new_like(x, "grad_x", stream), max(dim, 1)
     else:
         dxs = _matrix(grad_x, "grad_x", rows, dim, x.dtype, dev)
     grad_gamma, gp = _vector_out(grad_gamma, "grad_gamma", (dim,), dim, params, x, dev, stream)
-    grad_beta, bp = _vector_out(grad_beta, "grad_beta", (dim,), dim, params, x, dev, stream)
+    grad_beta, bp = _vector_out(grad_beta, "grad_beta", (dim,), dim, params, grad_gamma, dev, stream)
     keep, wp, wb = _workspace(workspace, layernorm_workspace(rows, dim), x, dev, stream)
     _call(lib().b200opt_layernorm_bwd, dev, stream, dtype, _DTYPES.get(params, -1), rows, dim,
           grad_y.data_ptr(), ys, x.data_ptr(), xs, _vector(gamma, "gamma", dim, params, dev),
@@ -268,7 +277,7 @@ def vocab_loss_forward(hidden, weight, targets, loss=None, lse=None, stats=None,
     dev, sizes, args = _head(hidden, weight, targets)
     n, shape, f32 = sizes[0], targets.shape, torch.float32
     loss, lp = _vector_out(loss, "loss", shape, n, f32, hidden, dev, stream)
-    lse, ep = _vector_out(lse, "lse", shape, n, f32, hidden, dev, stream)
+    lse, ep = _vector_out(lse, "lse", shape, n, f32, loss, dev, stream)
     stats, sp = _vector_out(stats, "stats", (2,), 2, f32, hidden, dev, stream)
     keep, wp, wb = _workspace(workspace, _bytes("b200opt_vocab_loss_fwd_workspace", *sizes), hidden,
                               dev, stream)
@@ -287,12 +296,12 @@ def vocab_loss_backward(hidden, weight, targets, lse, stats=None, grad_scale=1.0
     if accumulate and grad_weight is None:
         raise ValueError("accumulate needs grad_weight")
     if grad_hidden is None:
-        grad_hidden = _new(hidden, hidden.shape, torch.float16, "grad_hidden", stream)
+        grad_hidden = _new_like(hidden, "grad_hidden", stream)
         xs = dim
     else:
         xs = _matrix(grad_hidden, "grad_hidden", tokens, dim, torch.float16, dev)
     if grad_weight is None:
-        grad_weight = _new(weight, weight.shape, torch.float16, "grad_weight", stream)
+        grad_weight = _new_like(weight, "grad_weight", stream)
         ws = dim
     else:
         ws = _matrix(grad_weight, "grad_weight", vocab, dim, torch.float16, dev)
