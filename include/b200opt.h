@@ -552,6 +552,8 @@ B200OPT_API int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim,
  * The logits are recomputed piece by piece; p - onehot, at most 1 in magnitude,
  * is rounded to fp16 after a multiplication by 2^15 (which keeps every
  * probability over 2e-9 at full fp16 precision), for the tensor cores.
+ * The product kernels' waits on their own copies are bounded (10 s); one that
+ * ran out, here or in the forward pass, leaves NaN in what it should have given.
  */
 B200OPT_API int b200opt_vocab_loss_bwd_workspace(size_t tokens, size_t vocab,
                        size_t dim, size_t *bytes);

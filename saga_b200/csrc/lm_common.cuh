@@ -134,7 +134,7 @@ __device__ __forceinline__ int lm_index_at(const void *ids, int wide, size_t i, 
 
 // --------------------------------------------- barriers of asynchronous copies
 
-constexpr unsigned long long kWaitNs = 2000000000ull;  // limit of every wait
+constexpr unsigned long long kWaitNs = 10000000000ull;  // limit of every wait: 10 s, as in the step kernels
 
 __device__ __forceinline__ uint32_t smem_u32(const void *p)
 {

@@ -9,6 +9,10 @@ normal range).  SLACK covers the products of such terms and the few steps of exp
 log, division and square root that a bound does not name one by one.
 """
 import ctypes as C
+import os
+import subprocess
+import sys
+import threading
 
 import pytest
 import torch
@@ -630,6 +634,62 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for _, out in graphs:
             assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+def test_first_call_of_a_process_inside_a_capture():
+    """Nothing has to be called before a capture is open: kernels load and their shared-memory limits
+    are set under it."""
+    code = """
+import torch
+from saga_b200 import layers
+d = 'cuda:0'
+torch.manual_seed(3)
+x, w = torch.randn(300, 72, device=d).half(), torch.randn(700, 72, device=d).half()
+y = torch.randint(0, 700, (300,), device=d)
+def run():
+    a, mean, rstd = layers.layernorm_forward(layers.embedding_forward(y, w))
+    loss, lse, stats = layers.vocab_loss_forward(a, w, y)
+    dh, dw = layers.vocab_loss_backward(a, w, y, lse, stats=stats)
+    dx, dg, db = layers.layernorm_backward(dh, x, None, mean, rstd)
+    layers.embedding_backward(y, dx, 700, grad_weight=dw, accumulate=True)
+    return [loss, dh, dw, dx, dg, db, layers.embedding_backward(y[:20], dx[:20], 700)]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    out = run()
+g.replay()
+want = run()
+torch.cuda.synchronize()
+assert all(torch.equal(p, q) for p, q in zip(out, want))
+print('same')
+"""
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    res = subprocess.run([sys.executable, "-c", code], cwd=root, capture_output=True, text=True, timeout=300)
+    assert res.returncode == 0 and "same" in res.stdout, res.stderr[-2000:]
+
+
+def test_two_host_threads():
+    """Calls from two threads, each on a stream of its own, at the same time."""
+    inputs, run = _calls()
+    want = run()
+    torch.cuda.synchronize()
+    got, errors = [], []
+
+    def work():
+        try:
+            with torch.cuda.stream(torch.cuda.Stream()):
+                for _ in range(10):
+                    got.append(run())
+                torch.cuda.current_stream().synchronize()
+        except Exception as e:      # reported by the test, not lost with the thread
+            errors.append(e)
+    threads = [threading.Thread(target=work) for _ in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors
+    assert len(got) == 20 and all(torch.equal(a, b) for out in got for a, b in zip(out, want))
 
 
 def test_two_streams_at_once_and_a_raw_stream():
