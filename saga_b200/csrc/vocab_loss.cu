@@ -10,20 +10,22 @@ namespace {
 constexpr size_t kPieceBytes = (size_t)256 << 20;  // of p - onehot held at a time
 constexpr float kLift = 32768.0f;                  // 2^15: see the header
 constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kLn2 = 0.6931471805599453f;
 
-__device__ __forceinline__ float exp2_fast(float x)
+// e^x for x <= 0, to about 2^-22 of its size.  The callers subtract first and in
+// full: next to a probability of 1 what is lost in x is all that is left of the
+// gradient.
+__device__ __forceinline__ float exp_fast(float x)
 {
     float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * kLog2e));
     return y;
 }
 
 // ------------------------------------------------------------------ forward
 
-// Per row and tile of the vocabulary: the maximum of z log2(e) and the
-// sum of 2^(z log2(e) - maximum), in one pass over the accumulator.  The target's
-// logit goes to zt.
+// Per row and tile of the vocabulary: the maximum of z and the sum of
+// exp(z - maximum), in one pass over the accumulator.  The target's logit goes to
+// zt.
 struct StatsEpilogue {
     int T, V;
     const void *y;
@@ -66,11 +68,11 @@ struct StatsEpilogue {
 #pragma unroll
         for(int j = 4; j < 32; j++)
             most[j & 3] = fmaxf(most[j & 3], v[j]);
-        const float top = fmaxf(s.top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])) * kLog2e);
-        float sum[4] = {s.sum * exp2_fast(s.top - top), 0.0f, 0.0f, 0.0f};
+        const float top = fmaxf(s.top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
+        float sum[4] = {s.sum * exp_fast(s.top - top), 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for(int j = 0; j < 32; j++)
-            sum[j & 3] += exp2_fast(fmaf(v[j], kLog2e, -top));
+            sum[j & 3] += exp_fast(v[j] - top);
         s.top = top;
         s.sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
@@ -90,7 +92,7 @@ struct StatsEpilogue {
             top = fmaxf(top, slots[i * 128].x);
 #pragma unroll
         for(int i = 0; i < 4; i++)  // a side beyond the vocabulary has -inf and 0
-            sum += slots[i * 128].y * exp2_fast(slots[i * 128].x - top);
+            sum += slots[i * 128].y * exp_fast(slots[i * 128].x - top);
         part[(size_t)(col / kTcTile) * T + row] = make_float2(top, sum);
     }
 };
@@ -108,7 +110,7 @@ __global__ void __launch_bounds__(512)
     const int t = blockIdx.x * kLossRows + x;
     auto add = [](float2 a, float2 b) {  // two (maximum, sum) of disjoint stretches
         const float m = fmaxf(a.x, b.x);
-        return make_float2(m, (a.y ? a.y * exp2_fast(a.x - m) : 0.0f) + (b.y ? b.y * exp2_fast(b.x - m) : 0.0f));
+        return make_float2(m, (a.y ? a.y * exp_fast(a.x - m) : 0.0f) + (b.y ? b.y * exp_fast(b.x - m) : 0.0f));
     };
     // asked for now, used at the end
     const bool valid = t < T && lm_index_at(y, wide, t, V) >= 0;
@@ -128,7 +130,7 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
         for(int i = 0; i < 16; i++) {
             const float2 p = red[w + 4 * i][x];
-            sum += p.y ? p.y * exp2_fast(p.x - top) : 0.0f;
+            sum += p.y ? p.y * exp_fast(p.x - top) : 0.0f;
         }
         mine = make_float2(top, sum);
 #pragma unroll
@@ -137,7 +139,7 @@ __global__ void __launch_bounds__(512)
                                          __shfl_xor_sync(0xffffffffu, mine.y, o)));
         float own = 0.0f, counted = 0.0f;
         if(t < T && w == 0) {
-            const float l = (mine.x + log2f(mine.y)) * kLn2;
+            const float l = mine.x + logf(mine.y);
             lse[t] = l;
             if(valid) {
                 own = l - target;
@@ -271,7 +273,7 @@ struct DzEpilogue {
     __half *dz;
     size_t stride;  // a multiple of 256: whole tiles may be written
     struct State {
-        float c;
+        float lse;
         int at;
         bool live;
     };
@@ -279,7 +281,7 @@ struct DzEpilogue {
     __device__ __forceinline__ State begin(int tokens, int row, int, int) const
     {
         const bool live = row < tokens;
-        return {live ? fmaf(lse[row], kLog2e, -15.0f) : 0.0f, live ? target[row] - first : -1, live};
+        return {live ? lse[row] : 0.0f, live ? target[row] - first : -1, live};
     }
     __device__ __forceinline__ void columns(int, State &s, int row, int col, float (&v)[32], char *buf) const
     {
@@ -288,7 +290,7 @@ struct DzEpilogue {
         const int at = s.at - col;
 #pragma unroll
         for(int j = 0; j < 32; j++)
-            v[j] = s.live ? exp2_fast(fmaf(v[j], kLog2e, -s.c)) : 0.0f;
+            v[j] = s.live ? exp_fast(v[j] - s.lse) * kLift : 0.0f;
         if(at >= 0 && at < 32) {
 #pragma unroll
             for(int j = 0; j < 32; j++)

@@ -453,6 +453,34 @@ def test_vocab_loss_flat_and_peaked_distributions(std):
     check_head(x, w, y, f, b, 8.0)
 
 
+def test_vocab_loss_next_to_certainty():
+    """Targets with probabilities up to 1 - 1e-5, and a vocabulary of one: p - 1 keeps what the
+    rounding of lse leaves of it.  Values on a grid make the logits exact; then p is off by the
+    rounding of lse (a step of it or two) and of one exponential."""
+    tokens, vocab, dim = 64, 40, 8
+    x = torch.zeros(tokens, dim, dtype=torch.float16, device=DEV)
+    x[:, 0] = torch.linspace(0, 1, tokens, device=DEV).mul(64).round().div(64).half()
+    w = torch.zeros(vocab, dim, dtype=torch.float16, device=DEV)
+    w[3, 0] = 16.0
+    y = torch.full((tokens,), 3, device=DEV)
+    _, lse, _ = layers.vocab_loss_forward(x, w, y)
+    dx, dw = layers.vocab_loss_backward(x, w, y, lse, grad_scale=2.0 ** 14)
+    z = x.double() @ w.double().t()
+    exact = torch.logsumexp(z, 1)
+    close(lse, exact, exact.abs() * 2 * U + 8 * U)
+    dz = torch.exp(z[:, 3] - exact) - 1
+    want = 2.0 ** 14 * 16.0 * dz
+    e_p = 2 * U * exact.abs() + 16 * U
+    tol = 2.0 ** 14 * 16.0 * (e_p + dz.abs() * 2.0 ** -11) + half_step(want, torch.float16)
+    fits = want.abs() + tol < 65504          # beyond fp16's range the result is infinite
+    close(dx[fits, 0].double(), want[fits], tol[fits])
+    assert (dx[want.abs() - tol > 65520, 0] == -float("inf")).all()
+    one = layers.vocab_loss_forward(x, w[3:4], y * 0)
+    assert (one[0] == 0).all()
+    dx, dw = layers.vocab_loss_backward(x, w[3:4], y * 0, one[1])
+    assert (dx == 0).all() and (dw == 0).all()
+
+
 def test_vocab_loss_all_ignored():
     x, w, y = head_inputs(40, 100, 64)
     y[:] = -1
