@@ -156,6 +156,24 @@ def test_embedding_non_finite_values_stay_in_their_rows():
     assert (dw[5] == 2).all() and (dw[9, :7] == 1).all() and dw[[0, 1, 2, 3, 4, 7, 8, 10, 11]].abs().sum() == 0
 
 
+@pytest.mark.parametrize("tokens", [100, 1000, 20000])
+def test_embedding_padding_may_hold_anything(tokens):
+    """NaN in the rows of padding ids, first, last and in between, reaches nothing."""
+    g, vocab, dim = gen(tokens), 500, 40
+    ids = integers(g, tokens, 0, vocab)
+    pad = torch.rand(tokens, generator=g, device=DEV) < 0.4
+    pad[0] = pad[-1] = True
+    ids[pad] = torch.where(integers(g, int(pad.sum()), 0, 2) > 0, -1, 2 ** 40)
+    dy = normal(g, tokens, dim)
+    clean = dy.clone()
+    dy[pad] = float("nan")
+    clean[pad] = 0
+    got = layers.embedding_backward(ids, dy, vocab)
+    assert torch.equal(got, layers.embedding_backward(ids, clean, vocab))
+    exact, tol, _ = embedding_exact(ids, clean, vocab, 1.0)
+    close(got, exact, tol + half_step(exact, dy.dtype))
+
+
 # ---------------------------------------------------------------- layer norm
 
 LN_SIZES = [  # rows, dim
