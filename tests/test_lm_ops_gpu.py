@@ -76,7 +76,8 @@ def strided(t, stride, shift=0):
 EMB_SIZES = [  # tokens, vocab, dim
     (1, 1, 1), (1, 1000, 64), (7, 3, 5), (64, 1000, 333), (1000, 17, 40), (1025, 5003, 96),
     (300, 300, 1032), (2049, 1, 24), (33, 70001, 8), (20011, 211, 16), (50, 700, 2304), (40, 20, 70000),
-    (128, 1000, 333), (129, 1000, 333), (100, 50021, 520), (120, 5, 2304), (300, 700, 2304)]
+    (128, 1000, 333), (129, 1000, 333), (100, 50021, 520), (120, 5, 2304), (300, 700, 2304),
+    (2048, 3000, 1032), (1500, 40, 4104), (129, 64000, 600)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
