@@ -10,7 +10,7 @@ namespace {
 // threads of a block: eight rows of a warp each, or one row of WARPS warps
 __host__ __device__ constexpr int threads_of(int warps) { return warps == 1 ? 256 : 32 * warps; }
 __host__ __device__ constexpr int rows_of(int warps) { return warps == 1 ? 8 : 1; }
-constexpr int kMaxParts = 296;  // blocks of the gradient kernel: two on each of 148 SMs
+constexpr int kMaxParts = 444;  // blocks of the gradient kernel at most: three on each of 148 SMs
 
 // Sums over the threads that share a row: a warp, or the block.  `turn` alternates
 // between two sets of slots, so that one barrier a sum is enough.
@@ -37,11 +37,12 @@ __device__ __forceinline__ void row_sums(float (&v)[K], float (*slots)[16][K], i
     turn ^= 1;
 }
 
-// Two sums at once: the halves of a warp exchange, then each carries one of them.
-template <int WARPS>
+// Two sums at once over the WARPS warps of a group that shares a row, of a block of
+// BLOCK warps: the halves of a warp exchange, then each carries one of the sums.
+template <int WARPS, int BLOCK>
 __device__ __forceinline__ float2 row_pair(float a, float b, float (*slots)[2][16], int &turn)
 {
-    const int lane = threadIdx.x & 31;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, group = warp / WARPS;
     const bool low = lane < 16;
     float v = (low ? a : b) + __shfl_xor_sync(0xffffffffu, low ? b : a, 16);
 #pragma unroll
@@ -50,12 +51,15 @@ __device__ __forceinline__ float2 row_pair(float a, float b, float (*slots)[2][1
     if(WARPS == 1)
         return make_float2(__shfl_sync(0xffffffffu, v, 0), __shfl_sync(0xffffffffu, v, 16));
     if((lane & 15) == 0)
-        slots[turn][lane >> 4][threadIdx.x >> 5] = v;
-    __syncthreads();
+        slots[turn][lane >> 4][warp] = v;
+    if(WARPS == BLOCK)
+        __syncthreads();
+    else
+        asm volatile("bar.sync %0, %1;" ::"r"(1 + group), "n"(32 * WARPS) : "memory");
     float2 s = make_float2(0.0f, 0.0f);
 #pragma unroll
     for(int w = 0; w < WARPS; w++)
-        s.x += slots[turn][0][w], s.y += slots[turn][1][w];
+        s.x += slots[turn][0][group * WARPS + w], s.y += slots[turn][1][group * WARPS + w];
     turn ^= 1;
     return s;
 }
@@ -200,18 +204,24 @@ __global__ void __launch_bounds__(1024)
 // thread keeps the parameters' sums of its own columns in registers and leaves
 // them in `parts` at the end, for params_kernel to join in a fixed order.  The
 // next row's vectors are loaded before the present row's sums are waited for.
-__host__ __device__ constexpr int bwd_blocks(int columns) { return columns <= 16 ? 2 : 1; }
+// Blocks of the gradient kernel: 256 threads, several groups of WARPS warps with a
+// row each, or 512; and how many an SM is to hold, by the columns a thread has.
+__host__ __device__ constexpr int bwd_warps(int warps) { return warps > 8 ? warps : 8; }
+__host__ __device__ constexpr int bwd_blocks(int columns, bool halves)
+{
+    return columns <= 8 && halves ? 3 : columns <= 16 ? 2 : 1;
+}
 
 template <typename T, typename P, int N, int NV, int WARPS>
-__global__ void __launch_bounds__(threads_of(WARPS), bwd_blocks(N * NV))
+__global__ void __launch_bounds__(32 * bwd_warps(WARPS), bwd_blocks(N * NV, N == 8))
     layernorm_bwd_kernel(size_t rows, size_t dim, const T *dy, size_t ys, const T *x, size_t xs,
                          const P *gamma, const float *mean, const float *rstd, T *dx, size_t dxs,
                          float *parts)
 {
+    constexpr int BLOCK = bwd_warps(WARPS), R = BLOCK / WARPS, L = 32 * WARPS, THREADS = 32 * BLOCK;
     __shared__ __align__(16) float slots[2][2][16];
-    __shared__ float joined[WARPS == 1 ? 2 * 32 * NV * N : 1];
+    __shared__ float joined[R > 1 ? 2 * L * NV * N : 1];
     int turn = 0;
-    constexpr int L = 32 * WARPS, R = rows_of(WARPS);
     const int l = threadIdx.x % L, vecs = (int)(dim / N);
     const size_t step = (size_t)gridDim.x * R;
     const float inverse = 1.0f / (float)dim;
@@ -225,7 +235,7 @@ __global__ void __launch_bounds__(threads_of(WARPS), bwd_blocks(N * NV))
     size_t r = (size_t)blockIdx.x * R + threadIdx.x / L;
     Vec<T, N> vx[NV], vy[NV];
     float mu = 0.0f, rs = 0.0f;
-    auto fetch = [&](size_t row, Vec<T, N> (&a)[NV], Vec<T, N> (&b)[NV], float &m, float &q) {
+    auto fetch = [&](size_t row, Vec<T, N> *a, Vec<T, N> *b, float &m, float &q) {
         if(row >= rows)
             return;
         m = mean[row];
@@ -239,78 +249,98 @@ __global__ void __launch_bounds__(threads_of(WARPS), bwd_blocks(N * NV))
                 b[i] = py[l + i * L];
             }
     };
+    // registers for the next row's vectors, and for xh and d between the two passes: not
+    // with 512 threads
+    constexpr bool kRoom = BLOCK == 8;
     fetch(r, vx, vy, mu, rs);
-    // the rows of a block are consecutive steps, so with WARPS 8 all threads agree
+    // the threads of a group agree on r
     for(; r < rows; r += step) {
         if(N > 1 && l == 0 && r + 2 * step < rows) {  // two rows ahead, as far as L2
             prefetch_row(x + (r + 2 * step) * xs, (uint32_t)(dim * sizeof(T)));
             prefetch_row(dy + (r + 2 * step) * ys, (uint32_t)(dim * sizeof(T)));
         }
-        Vec<T, N> nx[NV], ny[NV];
+        Vec<T, N> nx[kRoom ? NV : 1], ny[kRoom ? NV : 1];
         float nmu = 0.0f, nrs = 0.0f;
-        fetch(r + step, nx, ny, nmu, nrs);
-        float s[2] = {0.0f, 0.0f}, xh[NV][N], d[NV][N];
+        if constexpr(kRoom)
+            fetch(r + step, nx, ny, nmu, nrs);
+        float s[2] = {0.0f, 0.0f}, xh[kRoom ? NV : 1][N], d[kRoom ? NV : 1][N];
 #pragma unroll
         for(int i = 0; i < NV; i++)
             if(l + i * L < vecs) {
                 float fx[N], fy[N], g[N];
+                const int k = kRoom ? i : 0;
                 vx[i].get(fx);
                 vy[i].get(fy);
                 load_param<P, N>(gamma, l + i * L, 1.0f, g);
 #pragma unroll
                 for(int j = 0; j < N; j++) {
-                    xh[i][j] = (fx[j] - mu) * rs;
-                    d[i][j] = fy[j] * g[j];
-                    sg[i][j] = fmaf(fy[j], xh[i][j], sg[i][j]);
+                    xh[k][j] = (fx[j] - mu) * rs;
+                    d[k][j] = fy[j] * g[j];
+                    sg[i][j] = fmaf(fy[j], xh[k][j], sg[i][j]);
                     sb[i][j] += fy[j];
-                    s[0] += d[i][j];
-                    s[1] = fmaf(d[i][j], xh[i][j], s[1]);
+                    s[0] += d[k][j];
+                    s[1] = fmaf(d[k][j], xh[k][j], s[1]);
                 }
             }
         if(dx) {
-            const float2 t = row_pair<WARPS>(s[0], s[1], slots, turn);
+            const float2 t = row_pair<WARPS, BLOCK>(s[0], s[1], slots, turn);
             const float a = t.x * inverse, b = t.y * inverse;
             Vec<T, N> *to = reinterpret_cast<Vec<T, N> *>(dx + r * dxs);
 #pragma unroll
             for(int i = 0; i < NV; i++)
                 if(l + i * L < vecs) {
                     float f[N];
+                    const int k = kRoom ? i : 0;
+                    if constexpr(!kRoom) {
+                        vx[i].get(xh[0]);
+                        vy[i].get(d[0]);
+                        load_param<P, N>(gamma, l + i * L, 1.0f, f);
+#pragma unroll
+                        for(int j = 0; j < N; j++) {
+                            xh[0][j] = (xh[0][j] - mu) * rs;
+                            d[0][j] *= f[j];
+                        }
+                    }
 #pragma unroll
                     for(int j = 0; j < N; j++)
-                        f[j] = rs * fmaf(-b, xh[i][j], d[i][j] - a);
+                        f[j] = rs * fmaf(-b, xh[k][j], d[k][j] - a);
                     Vec<T, N> o;
                     o.set(f);
                     to[l + i * L] = o;
                 }
         }
+        if constexpr(kRoom) {
 #pragma unroll
-        for(int i = 0; i < NV; i++) {
-            vx[i] = nx[i];
-            vy[i] = ny[i];
+            for(int i = 0; i < NV; i++) {
+                vx[i] = nx[i];
+                vy[i] = ny[i];
+            }
+            mu = nmu;
+            rs = nrs;
+        } else {
+            fetch(r + step, vx, vy, mu, rs);
         }
-        mu = nmu;
-        rs = nrs;
     }
     if(!parts)
         return;
     float *pg = parts + (size_t)blockIdx.x * 2 * dim, *pb = pg + dim;
-    if(WARPS == 1) {  // the block's warps have the same columns: joined one after the other
-        for(int w = 0; w < 8; w++) {
-            if(threadIdx.x / 32 == w)
+    if(R > 1) {  // the block's groups have the same columns: joined one after the other
+        for(int w = 0; w < R; w++) {
+            if(threadIdx.x / L == w)
 #pragma unroll
                 for(int i = 0; i < NV; i++)
                     if(l + i * L < vecs)
 #pragma unroll
                         for(int j = 0; j < N; j++) {
-                            float *g = joined + (i * L + l) * N + j, *b = g + 32 * NV * N;
+                            float *g = joined + (i * L + l) * N + j, *b = g + L * NV * N;
                             *g = w ? *g + sg[i][j] : sg[i][j];
                             *b = w ? *b + sb[i][j] : sb[i][j];
                         }
             __syncthreads();
         }
-        for(int d = threadIdx.x; d < (int)dim; d += 256) {
+        for(int d = threadIdx.x; d < (int)dim; d += THREADS) {
             pg[d] = joined[d];
-            pb[d] = joined[32 * NV * N + d];
+            pb[d] = joined[L * NV * N + d];
         }
     } else {
 #pragma unroll
@@ -428,14 +458,24 @@ int fwd_with(const Args &a)
 {
     auto launch = [&](auto nv, auto warps) {
         constexpr int NV = decltype(nv)::value, W = decltype(warps)::value;
-        constexpr int ROWS = W == 1 || NV > 4 || N == 1 ? 1 : 2;
-        const size_t blocks = (a.rows + rows_of(W) * ROWS - 1) / (rows_of(W) * ROWS);
-        layernorm_fwd_kernel<T, P, N, NV, W, ROWS><<<(unsigned)blocks, threads_of(W), 0, a.st>>>(
-            a.rows, a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y,
-            a.ys, a.mean, a.rstd);
+        // several rows at a time where that leaves blocks enough
+        constexpr int MANY = N == 1 || NV > 4 ? 1 : W > 1 || NV == 4 ? 2 : 4;
+        auto go = [&](auto count) {
+            constexpr int ROWS = decltype(count)::value;
+            const size_t blocks = (a.rows + rows_of(W) * ROWS - 1) / (rows_of(W) * ROWS);
+            layernorm_fwd_kernel<T, P, N, NV, W, ROWS><<<(unsigned)blocks, threads_of(W), 0, a.st>>>(
+                a.rows, a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps,
+                (T *)a.y, a.ys, a.mean, a.rstd);
+        };
+        if(a.rows >= (size_t)592 * rows_of(W) * MANY)
+            go(std::integral_constant<int, MANY>());
+        else
+            go(std::integral_constant<int, 1>());
     };
     const size_t vecs = a.dim / N;
-    if(!pick<1, 1, 4>(vecs, launch) && !pick<4, 2, 16>(vecs, launch) && !pick<16, 8, 16>(vecs, launch))
+    constexpr int MOST = N == 1 ? 16 : 4;
+    if(!pick<1, 1, 4>(vecs, launch) && !pick<4, 2, MOST>(vecs, launch) &&
+       !pick<8, MOST, MOST>(vecs, launch) && !pick<16, MOST, 16>(vecs, launch))
         layernorm_fwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
             a.dim, (const T *)a.x, a.xs, (const P *)a.gamma, (const P *)a.beta, a.eps, (T *)a.y, a.ys,
             a.mean, a.rstd);
@@ -450,16 +490,22 @@ int bwd_with(const Args &a)
     size_t blocks = 0;
     auto launch = [&](auto nv, auto warps) {
         constexpr int NV = decltype(nv)::value, W = decltype(warps)::value;
-        blocks = std::min<size_t>((a.rows + rows_of(W) - 1) / rows_of(W),
-                                  std::min(148 * bwd_blocks(N * NV), kMaxParts));
+        constexpr int R = bwd_warps(W) / W;
+        blocks = std::min<size_t>((a.rows + R - 1) / R, std::min(148 * bwd_blocks(N * NV, N == 8), kMaxParts));
         if(blocks)
-            layernorm_bwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, threads_of(W), 0, a.st>>>(
+            layernorm_bwd_kernel<T, P, N, NV, W><<<(unsigned)blocks, 32 * bwd_warps(W), 0, a.st>>>(
                 a.rows, a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma,
                 a.mean_in, a.rstd_in, (T *)a.dx, a.dxs, parts);
     };
     const size_t vecs = a.dim / N;
-    constexpr int kWarp = N == 1 ? 16 : 16 / N * 2, kBlock = 32 / N;
-    if(!pick<1, 1, kWarp>(vecs, launch) && !pick<8, kWarp / 4, kBlock>(vecs, launch)) {
+    // few columns a thread as long as warps can be added, then more.  Two vectors in
+    // fp16, where a row's fixed cost weighs more (16384 x 2048: 45 us, with one vector
+    // 55; x 1024: 29 and 31), eight columns otherwise (fp32 x 1024: 39 us; a warp a
+    // row with 32 columns 53).
+    constexpr int FEW = N == 8 ? 2 : 8 / N, MOST = 32 / N;
+    if(!pick<1, 1, FEW>(vecs, launch) && !pick<2, FEW, FEW>(vecs, launch) &&
+       !pick<4, FEW, FEW>(vecs, launch) && !pick<8, FEW, MOST>(vecs, launch) &&
+       !(N == 8 && pick<16, 4, 4>(vecs, launch))) {
         if(a.dx && a.rows)
             layernorm_bwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
                 a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma, a.mean_in,

@@ -179,7 +179,10 @@ def test_embedding_padding_may_hold_anything(tokens):
 
 LN_SIZES = [  # rows, dim
     (1, 1), (1, 2), (3, 7), (64, 512), (5, 1001), (33, 1024), (9, 4096), (2, 8193), (300, 40),
-    (1030, 264), (4, 16384), (3, 40001), (2000, 8)]
+    (1030, 264), (4, 16384), (3, 40001), (2000, 8),
+    # several rows a pass, and each width of a group in the gradient
+    (4740, 256), (9500, 72), (2370, 1024), (1200, 2048), (1190, 4096), (300, 4100), (40, 12288), (600, 600),
+    (5, 65544)]
 KINDS = [(torch.float16, torch.float16), (torch.float16, torch.float32), (torch.float32, torch.float32)]
 
 
