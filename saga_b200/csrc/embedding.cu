@@ -64,18 +64,147 @@ constexpr int kOrderWarps = kOrderThreads / 32;
 constexpr int kStretch = 512;                             // consecutive tokens of a warp
 constexpr int kOrderChunk = kOrderWarps * kStretch;       // tokens at a time
 constexpr int kDigits = 512;                              // rows a block can have
+constexpr size_t kOrderBlocks = 148;
 constexpr int kOrderSmem = kOrderChunk * 4 + kOrderWarps * kDigits * 2;
+
+// Many tokens: that every block looks at all of them would be most of the work
+// (65536 tokens: 42 us, 262144: 153 us).  They are then first dealt out by remainder, three
+// launches of a stable counting pass, and a block looks at its own alone: 23 and 52 us
+// together.  At 32768 tokens both ways take 22 us.
+
+constexpr size_t kSplitTokens = 32768;
+constexpr int kDealTokens = 2048;  // of a block: 32 warps, 64 each (8192: the move takes 23 us, not 7.5)
+
+__device__ __forceinline__ int remainder_of(const void *ids, int wide, size_t t, size_t tokens,
+                                            size_t vocab, uint32_t blocks, int &id)
+{
+    id = t < tokens ? lm_index_at(ids, wide, t, vocab) : -1;
+    return id < 0 ? -1 : (int)((uint32_t)id % blocks);
+}
+
+// How many ids of each remainder a chunk has; counts[remainder][chunk].
+__global__ void __launch_bounds__(1024)
+    deal_count_kernel(size_t tokens, size_t vocab, const void *ids, int wide, uint32_t blocks, int *counts)
+{
+    __shared__ int count[kDigits];
+    for(int i = threadIdx.x; i < kDigits; i += 1024)
+        count[i] = 0;
+    __syncthreads();
+#pragma unroll
+    for(int i = 0; i < kDealTokens / 1024; i++) {
+        int id;
+        const int r = remainder_of(ids, wide, (size_t)blockIdx.x * kDealTokens + i * 1024 + threadIdx.x,
+                                   tokens, vocab, blocks, id);
+        if(r >= 0)
+            atomicAdd(&count[r], 1);  // whole numbers: any order gives the same
+    }
+    __syncthreads();
+    for(int i = threadIdx.x; i < (int)blocks; i += 1024)
+        counts[(size_t)i * gridDim.x + blockIdx.x] = count[i];
+}
+
+// n numbers to the sums of those before them; counts[n] gets the sum of all.  It has
+// room for kEach more behind that, since numbers are read and written four at a time.
+constexpr int kEach = 8;  // of a thread, in a row
+
+__global__ void __launch_bounds__(1024) deal_sums_kernel(int *counts, size_t n)
+{
+    __shared__ int warp_sums[32];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int base = 0;
+    for(size_t i0 = 0; i0 < n; i0 += 1024 * kEach) {
+        const size_t i = i0 + threadIdx.x * kEach;
+        int4 *mine = reinterpret_cast<int4 *>(counts + i);
+        int c[kEach], sum = 0;
+#pragma unroll
+        for(int j = 0; j < kEach; j += 4) {
+            const int4 v = i < n ? mine[j / 4] : int4{0, 0, 0, 0};
+            c[j] = v.x, c[j + 1] = v.y, c[j + 2] = v.z, c[j + 3] = v.w;
+        }
+#pragma unroll
+        for(int j = 0; j < kEach; j++)
+            sum += c[j] = i + j < n ? c[j] : 0;
+        int run = sum;
+#pragma unroll
+        for(int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, run, o);
+            run += lane >= o ? v : 0;
+        }
+        if(lane == 31)
+            warp_sums[warp] = run;
+        __syncthreads();
+        const int w = warp_sums[lane];
+        int at = base + __reduce_add_sync(0xffffffffu, lane < warp ? w : 0) + run - sum;
+#pragma unroll
+        for(int j = 0; j < kEach; j += 4) {
+            const int4 v = {at, at + c[j], at + c[j] + c[j + 1], at + c[j] + c[j + 1] + c[j + 2]};
+            if(i < n)
+                mine[j / 4] = v;
+            at = v.w + c[j + 3];
+        }
+        base += __reduce_add_sync(0xffffffffu, w);
+        __syncthreads();
+    }
+    if(threadIdx.x == 0)
+        counts[n] = base;
+}
+
+__global__ void __launch_bounds__(1024)
+    deal_move_kernel(size_t tokens, size_t vocab, const void *ids, int wide, uint32_t blocks,
+                     const int *counts, int *dealt, int *dealt_token)
+{
+    constexpr int kTrips = kDealTokens / 1024;
+    __shared__ uint16_t count[32][kDigits];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for(int i = lane; i < kDigits / 2; i += 32)
+        reinterpret_cast<uint32_t *>(count[warp])[i] = 0;
+    __syncwarp();
+    const size_t first = (size_t)blockIdx.x * kDealTokens + warp * (32 * kTrips) + lane;
+    int id[kTrips], r[kTrips], rank[kTrips];
+#pragma unroll
+    for(int i = 0; i < kTrips; i++)
+        r[i] = remainder_of(ids, wide, first + 32 * i, tokens, vocab, blocks, id[i]);
+#pragma unroll
+    for(int i = 0; i < kTrips; i++) {  // as in order_kernel
+        const unsigned same = __match_any_sync(0xffffffffu, r[i]);
+        const int lower = __popc(same & ((1u << lane) - 1));
+        rank[i] = r[i] >= 0 ? count[warp][r[i]] + lower : 0;
+        __syncwarp();
+        if(r[i] >= 0 && lower == 0)
+            count[warp][r[i]] += (uint16_t)__popc(same);
+        __syncwarp();
+    }
+    __syncthreads();
+    for(int d = threadIdx.x; d < (int)blocks; d += 1024) {
+        int total = 0;
+        for(int w = 0; w < 32; w++) {
+            const int c = count[w][d];
+            count[w][d] = (uint16_t)total;
+            total += c;
+        }
+    }
+    __syncthreads();
+#pragma unroll
+    for(int i = 0; i < kTrips; i++)
+        if(r[i] >= 0) {
+            const int at = counts[(size_t)r[i] * gridDim.x + blockIdx.x] + count[warp][r[i]] + rank[i];
+            dealt[at] = id[i];
+            dealt_token[at] = (int)(first + 32 * i);
+        }
+}
 
 // keys: the ids in their new order, `vocab` behind the last; order: the tokens;
 // ends: where a run of equal ids ends (at its first kChunk tokens).  named: for
-// each row, whether it has a token.
+// each row, whether it has a token.  DEALT: ids (and dealt_token) are dealt
+// out, block b's from starts[b * pitch].
 //
 // The loops stay rolled: the code runs once per block, so its length, fetched cold,
 // would cost more than the branches (unrolled over the ids of a thread it took 9 us
 // for 64 tokens).
+template <bool DEALT>
 __global__ void __launch_bounds__(kOrderThreads, 1)
-    order_kernel(size_t tokens, size_t vocab, const void *ids, int wide, uint32_t *keys, int *order,
-                 int *ends, unsigned char *named)
+    order_kernel(size_t tokens, size_t vocab, const void *ids, int wide, const int *starts, size_t pitch,
+                 const int *dealt_token, uint32_t *keys, int *order, int *ends, unsigned char *named)
 {
     extern __shared__ __align__(16) char order_smem[];
     // this block's tokens, in order, for each warp: place in its stretch << 20 | rank << 9 | digit
@@ -88,24 +217,27 @@ __global__ void __launch_bounds__(kOrderThreads, 1)
     const uint32_t inverse = 0xffffffffu / blocks;
     const int digits = (int)((vocab - me + blocks - 1) / blocks);  // this block's rows
     uint16_t *count = counts + warp * kDigits;
+    const size_t t0 = DEALT ? starts[me * pitch] : 0, t1 = DEALT ? starts[(me + 1) * pitch] : tokens;
     // a warp's stretch: shorter where there are few tokens, so that all warps have some
     const int stretch =
-        (int)min((tokens + kOrderThreads - 1) / kOrderThreads * 32, (size_t)kStretch);
+        (int)min((t1 - t0 + kOrderThreads - 1) / kOrderThreads * 32, (size_t)kStretch);
     const size_t step = (size_t)stretch * kOrderWarps;
     if(tid < kDigits)
         base[tid] = 0;
-    if(tid == 0)
-        before_sum = valid_sum = 0;
+    if(tid == 0) {
+        before_sum = (int)t0;
+        valid_sum = DEALT ? starts[blocks * pitch] : 0;
+    }
     __syncthreads();
 
     int n = 0, before = 0, valid = 0, my_start = 0, my_end = 0;
     for(int pass = 0; pass < 2; pass++) {
-        for(size_t c0 = 0; c0 < tokens; c0 += step) {
+        for(size_t c0 = t0; c0 < t1; c0 += step) {
             const size_t first = c0 + warp * stretch;
-            if(pass == 0 || tokens > step) {
+            if(pass == 0 || t1 - t0 > step) {
                 n = 0;
                 // the stretch's ids, many loads in flight; the block's own replace them
-                const int here = (int)min((size_t)stretch, tokens > first ? tokens - first : 0);
+                const int here = (int)min((size_t)stretch, t1 > first ? t1 - first : 0);
                 __syncwarp();
 #pragma unroll 16
                 for(int i = lane; i < here; i += 32)
@@ -119,7 +251,7 @@ __global__ void __launch_bounds__(kOrderThreads, 1)
                     const bool mine = id >= 0 && r == me;
                     if(pass == 0) {
                         before += id >= 0 && r < me;
-                        valid += id >= 0;
+                        valid += id >= 0 && !DEALT;
                         if(mine)
                             atomicAdd(&base[q], 1);  // whole numbers: any order gives the same
                     }
@@ -166,7 +298,8 @@ __global__ void __launch_bounds__(kOrderThreads, 1)
                 const uint32_t e = list[i], d = e & (kDigits - 1);
                 const int at = base[d] + count[d] + (int)(e >> 9 & 0x7ff);
                 keys[at] = d * blocks + me;
-                order[at] = (int)(first + (e >> 20));
+                const size_t from = first + (e >> 20);
+                order[at] = DEALT ? dealt_token[from] : (int)from;
             }
             __syncthreads();
             if(tid < kDigits)
@@ -677,7 +810,9 @@ bool few_tokens(size_t tokens, size_t vocab)
 }
 
 struct Work {
-    size_t at_keys, at_order, at_ends, at_named, at_parts, bytes;
+    bool split;
+    size_t blocks, deals;  // of order_kernel; of the dealing
+    size_t at_keys, at_order, at_ends, at_named, at_parts, at_dealt, at_token, at_counts, bytes;
     Work(size_t tokens, size_t vocab, size_t dim)
     {
         size_t at = 0;
@@ -691,6 +826,13 @@ struct Work {
         at_ends = take(lm_up(tokens, kChunk) * 4);
         at_named = take(vocab);
         at_parts = take((tokens + kChunk - 1) / kChunk * 2 * dim * 4);
+        // one block an SM, more where a block would get more rows than it has digits for
+        blocks = std::min(vocab, std::max<size_t>(kOrderBlocks, (vocab + kDigits - 1) / kDigits));
+        split = tokens > kSplitTokens && blocks <= kDigits;
+        deals = (tokens + kDealTokens - 1) / kDealTokens;
+        at_dealt = take(split ? tokens * 4 : 0);
+        at_token = take(split ? tokens * 4 : 0);
+        at_counts = take(split ? (blocks * deals + 1 + kEach) * 4 : 0);
         bytes = at;
     }
 };
@@ -710,12 +852,11 @@ int gradient(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide,
     int *order = (int *)(work + w.at_order), *ends = (int *)(work + w.at_ends);
     unsigned char *named = (unsigned char *)(work + w.at_named);
     float *parts = (float *)(work + w.at_parts);
-    int sms = 0;
     static std::atomic<uint64_t> allowed{0};
-    if(!lm_sms(&sms) || !lm_allow_smem(order_kernel, kOrderSmem, allowed))
+    static std::atomic<uint64_t> allowed_dealt{0};
+    if(!lm_allow_smem(order_kernel<false>, kOrderSmem, allowed) ||
+       !lm_allow_smem(order_kernel<true>, kOrderSmem, allowed_dealt))
         return B200OPT_ECUDA;
-    // one block an SM, more where a block would get more rows than it has digits for
-    const size_t blocks = std::min(vocab, std::max<size_t>(sms, (vocab + kDigits - 1) / kDigits));
     const int lanes = lanes_of(vecs, 1);
     const size_t chunks = (tokens + kChunk - 1) / kChunk, per = 256 / lanes;
     const size_t groups = (chunks + per - 1) / per, slices = (vecs + lanes - 1) / lanes;
@@ -727,8 +868,20 @@ int gradient(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide,
     const size_t cuts = (vecs + 31) / 32, joins = (chunks + 7) / 8 * cuts;
     if(groups * slices + fills > 0x7fffffff || joins > 0x7fffffff)
         return B200OPT_ETOOBIG;
-    order_kernel<<<(unsigned)blocks, kOrderThreads, kOrderSmem, st>>>(tokens, vocab, ids, wide, keys, order,
-                                                                      ends, named);
+    const uint32_t blocks = (uint32_t)w.blocks;
+    if(w.split) {
+        int *dealt = (int *)(work + w.at_dealt), *token = (int *)(work + w.at_token);
+        int *counts = (int *)(work + w.at_counts);
+        deal_count_kernel<<<(unsigned)w.deals, 1024, 0, st>>>(tokens, vocab, ids, wide, blocks, counts);
+        deal_sums_kernel<<<1, 1024, 0, st>>>(counts, w.blocks * w.deals);
+        deal_move_kernel<<<(unsigned)w.deals, 1024, 0, st>>>(tokens, vocab, ids, wide, blocks, counts, dealt,
+                                                             token);
+        order_kernel<true><<<blocks, kOrderThreads, kOrderSmem, st>>>(
+            tokens, vocab, dealt, 0, counts, w.deals, token, keys, order, ends, named);
+    } else {
+        order_kernel<false><<<blocks, kOrderThreads, kOrderSmem, st>>>(
+            tokens, vocab, ids, wide, nullptr, 0, nullptr, keys, order, ends, named);
+    }
     sum_kernel<T, N><<<(unsigned)(groups * slices + fills), 256, 0, st>>>(
         tokens, vocab, vecs, lanes, groups * slices, slices, keys, order, named, (const T *)dy, ys, scale,
         (T *)dw, ws, accumulate, parts);

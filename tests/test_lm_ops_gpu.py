@@ -77,7 +77,7 @@ EMB_SIZES = [  # tokens, vocab, dim
     (1, 1, 1), (1, 1000, 64), (7, 3, 5), (64, 1000, 333), (1000, 17, 40), (1025, 5003, 96),
     (300, 300, 1032), (2049, 1, 24), (33, 70001, 8), (20011, 211, 16), (50, 700, 2304), (40, 20, 70000),
     (128, 1000, 333), (129, 1000, 333), (100, 50021, 520), (120, 5, 2304), (300, 700, 2304),
-    (2048, 3000, 1032), (1500, 40, 4104), (129, 64000, 600)]
+    (2048, 3000, 1032), (1500, 40, 4104), (129, 64000, 600), (40961, 90001, 16), (70000, 3, 8), (33000, 300000, 8)]
 
 
 @pytest.mark.parametrize("dtype", [torch.float16, torch.float32])
@@ -133,7 +133,7 @@ def test_embedding_backward(tokens, vocab, dim, dtype):
 
 
 @pytest.mark.parametrize("pattern", ["none", "all the same", "sorted", "reversed", "two", "one block"])
-@pytest.mark.parametrize("tokens", [31, 32, 33, 127, 128, 129, 4096, 16384, 16385, 40000])
+@pytest.mark.parametrize("tokens", [31, 32, 33, 127, 128, 129, 4096, 16384, 16385, 32769, 40000])
 def test_embedding_backward_orders(tokens, pattern):
     """Orders of ids that leave a sort or a split of a long run nothing to hide behind."""
     g, vocab, dim = gen(tokens), 30011, 24
