@@ -685,6 +685,34 @@ def test_captured_and_replayed():
         for _, out in graphs:
             assert all(torch.equal(a, b) for a, b in zip(out, want))
 
+@pytest.mark.parametrize("tokens,vocab,dim", [(1, 3, 8), (129, 700, 72), (513, 1009, 264),
+                                              (1001, 2100, 520), (33001, 500, 24)])
+def test_workspaces_may_hold_anything(tokens, vocab, dim):
+    gen = torch.Generator(device=DEV).manual_seed(tokens)
+    x = torch.randn(tokens, dim, generator=gen, device=DEV).half()
+    dy = torch.randn(tokens, dim, generator=gen, device=DEV).half()
+    w = (torch.randn(vocab, dim, generator=gen, device=DEV) * 0.1).half()
+    ids = torch.randint(-1, vocab, (tokens,), generator=gen, device=DEV)
+    gamma = torch.randn(dim, generator=gen, device=DEV).half()
+    _, mean, rstd = layers.layernorm_forward(x, gamma)
+
+    def run(byte):
+        def ws(n):
+            return torch.full((n,), byte, dtype=torch.uint8, device=DEV)
+        fwd, bwd = layers.vocab_loss_workspace(tokens, vocab, dim)
+        out = [layers.embedding_backward(ids, dy, vocab,
+                                         workspace=ws(layers.embedding_workspace(tokens, vocab, dim)))]
+        out += layers.layernorm_backward(dy, x, gamma, mean, rstd,
+                                         workspace=ws(layers.layernorm_workspace(tokens, dim)))
+        head = layers.vocab_loss_forward(x, w, ids, workspace=ws(fwd))
+        out += head
+        out += layers.vocab_loss_backward(x, w, ids, head[1], head[2], workspace=ws(bwd))
+        return out
+
+    for a, b in zip(run(0), run(255)):      # 255: NaN in either type, -1 as a whole number
+        assert torch.equal(a, b) and a.isfinite().all()
+
+
 
 def test_first_call_of_a_process_inside_a_capture():
     """Nothing has to be called before a capture is open: kernels load and their shared-memory limits
