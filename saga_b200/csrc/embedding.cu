@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(1024)
     deal_count_kernel(size_t tokens, size_t vocab, const void *ids, int wide, uint32_t blocks, int *counts)
 {
     __shared__ int count[kDigits];
+    lm_let_next();
     for(int i = threadIdx.x; i < kDigits; i += 1024)
         count[i] = 0;
     __syncthreads();
@@ -112,6 +113,8 @@ __global__ void __launch_bounds__(1024) deal_sums_kernel(int *counts, size_t n)
     __shared__ int warp_sums[32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int base = 0;
+    lm_let_next();
+    lm_after_previous();
     for(size_t i0 = 0; i0 < n; i0 += 1024 * kEach) {
         const size_t i = i0 + threadIdx.x * kEach;
         int4 *mine = reinterpret_cast<int4 *>(counts + i);
@@ -155,6 +158,8 @@ __global__ void __launch_bounds__(1024)
 {
     constexpr int kTrips = kDealTokens / 1024;
     __shared__ uint16_t count[32][kDigits];
+    lm_let_next();
+    lm_after_previous();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     for(int i = lane; i < kDigits / 2; i += 32)
         reinterpret_cast<uint32_t *>(count[warp])[i] = 0;
@@ -217,6 +222,9 @@ __global__ void __launch_bounds__(kOrderThreads, 1)
     const uint32_t inverse = 0xffffffffu / blocks;
     const int digits = (int)((vocab - me + blocks - 1) / blocks);  // this block's rows
     uint16_t *count = counts + warp * kDigits;
+    lm_let_next();
+    if(DEALT)
+        lm_after_previous();
     const size_t t0 = DEALT ? starts[me * pitch] : 0, t1 = DEALT ? starts[(me + 1) * pitch] : tokens;
     // a warp's stretch: shorter where there are few tokens, so that all warps have some
     const int stretch =
@@ -467,6 +475,8 @@ __global__ void __launch_bounds__(256, 2)
                const uint32_t *keys, const int *order, const unsigned char *named, const T *dy,
                size_t ys, float scale, T *dw, size_t ws, int accumulate, float *parts)
 {
+    lm_let_next();
+    lm_after_previous();
     const size_t block = blockIdx.x * sums / gridDim.x;  // sum blocks before this one
     if((blockIdx.x + 1) * sums / gridDim.x == block) {
         fill_rows<T, N>(blockIdx.x - block, vocab, vecs, named, dw, ws);
@@ -541,6 +551,7 @@ __global__ void __launch_bounds__(256, 4)
                      const int *ends, float scale, T *dw, size_t ws, int accumulate,
                      const float *parts)
 {
+    lm_after_previous();
     __shared__ size_t last_of[8];
     __shared__ Vec<float, N> joined[8][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -873,21 +884,21 @@ int gradient(size_t tokens, size_t vocab, size_t dim, const void *ids, int wide,
         int *dealt = (int *)(work + w.at_dealt), *token = (int *)(work + w.at_token);
         int *counts = (int *)(work + w.at_counts);
         deal_count_kernel<<<(unsigned)w.deals, 1024, 0, st>>>(tokens, vocab, ids, wide, blocks, counts);
-        deal_sums_kernel<<<1, 1024, 0, st>>>(counts, w.blocks * w.deals);
-        deal_move_kernel<<<(unsigned)w.deals, 1024, 0, st>>>(tokens, vocab, ids, wide, blocks, counts, dealt,
-                                                             token);
-        order_kernel<true><<<blocks, kOrderThreads, kOrderSmem, st>>>(
-            tokens, vocab, dealt, 0, counts, w.deals, token, keys, order, ends, named);
+        lm_launch_next(deal_sums_kernel, 1, 1024, 0, st, counts, w.blocks * w.deals);
+        lm_launch_next(deal_move_kernel, (unsigned)w.deals, 1024, 0, st, tokens, vocab, ids, wide, blocks,
+                       counts, dealt, token);
+        lm_launch_next(order_kernel<true>, blocks, kOrderThreads, kOrderSmem, st, tokens, vocab, dealt, 0,
+                       counts, w.deals, token, keys, order, ends, named);
     } else {
         order_kernel<false><<<blocks, kOrderThreads, kOrderSmem, st>>>(
             tokens, vocab, ids, wide, nullptr, 0, nullptr, keys, order, ends, named);
     }
-    sum_kernel<T, N><<<(unsigned)(groups * slices + fills), 256, 0, st>>>(
-        tokens, vocab, vecs, lanes, groups * slices, slices, keys, order, named, (const T *)dy, ys, scale,
-        (T *)dw, ws, accumulate, parts);
+    lm_launch_next(sum_kernel<T, N>, (unsigned)(groups * slices + fills), 256, 0, st, tokens, vocab, vecs, lanes,
+                   groups * slices, slices, keys, order, named, (const T *)dy, ys, scale, (T *)dw, ws, accumulate,
+                   parts);
     if(chunks > 1)
-        join_rows_kernel<T, N><<<(unsigned)joins, 256, 0, st>>>(tokens, vocab, vecs, cuts, keys, ends, scale,
-                                                                (T *)dw, ws, accumulate, parts);
+        lm_launch_next(join_rows_kernel<T, N>, (unsigned)joins, 256, 0, st, tokens, vocab, vecs, cuts, keys, ends,
+                       scale, (T *)dw, ws, accumulate, parts);
     return lm_launched();
 }
 

@@ -359,6 +359,7 @@ template <typename P>
 __global__ void __launch_bounds__(256)
     params_kernel(size_t dim, int blocks, const float *parts, P *dgamma, P *dbeta, int accumulate)
 {
+    lm_after_previous();
     __shared__ float red[8][33];
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const size_t d = (size_t)blockIdx.x * 32 + lane;
@@ -518,8 +519,8 @@ int bwd_with(const Args &a)
                     parts);
     }
     if(want)
-        params_kernel<P><<<dim3((unsigned)((a.dim + 31) / 32), 2), 256, 0, a.st>>>(
-            a.dim, (int)blocks, parts, (P *)a.dgamma, (P *)a.dbeta, a.accumulate);
+        lm_launch_next(params_kernel<P>, dim3((unsigned)((a.dim + 31) / 32), 2), 256, 0, a.st, a.dim, (int)blocks,
+                       parts, (P *)a.dgamma, (P *)a.dbeta, a.accumulate);
     return lm_launched();
 }
 

@@ -37,6 +37,29 @@ inline int lm_launched()
     return cudaGetLastError() == cudaSuccess ? B200OPT_OK : B200OPT_ECUDA;
 }
 
+// Launches a kernel that may be brought onto the GPU while the kernel before it in the
+// stream still runs: it begins with lm_after_previous, which waits until that one has
+// ended and all that it wrote can be read.  The kernel before it can say with lm_let_next
+// from when on (its end, if it does not); that counts once all of its blocks have said
+// it, so they are all running and the next ones take no place that they need.  The three
+// kernels of an embedding gradient of 1999 x 333 called one after the other: 19.3 us
+// without, 17.1 with.
+template <typename... P, typename... A>
+inline void lm_launch_next(void (*kernel)(P...), dim3 grid, unsigned threads, size_t smem, cudaStream_t st,
+                           const A &...args)
+{
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t c = {};
+    c.gridDim = grid, c.blockDim = dim3(threads), c.dynamicSmemBytes = smem, c.stream = st;
+    c.attrs = &early, c.numAttrs = 1;
+    cudaLaunchKernelEx(&c, kernel, static_cast<P>(args)...);  // an error stays for lm_launched
+}
+
+__device__ __forceinline__ void lm_after_previous() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void lm_let_next() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // Lets a kernel use `bytes` of dynamic shared memory on the current device.  The
 // setting stays with the kernel, so it is made once per device; `done` is the
 // kernel's own record of where.
