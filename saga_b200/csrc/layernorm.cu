@@ -518,9 +518,12 @@ int bwd_with(const Args &a)
                     a.rows, a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, a.mean_in, a.rstd_in,
                     parts);
     }
-    if(want)
-        lm_launch_next(params_kernel<P>, dim3((unsigned)((a.dim + 31) / 32), 2), 256, 0, a.st, a.dim, (int)blocks,
-                       parts, (P *)a.dgamma, (P *)a.dbeta, a.accumulate);
+    const dim3 grid((unsigned)((a.dim + 31) / 32), 2);
+    if(want && blocks)
+        lm_launch_next(params_kernel<P>, grid, 256, 0, a.st, a.dim, (int)blocks, parts, (P *)a.dgamma,
+                       (P *)a.dbeta, a.accumulate);
+    else if(want)
+        params_kernel<P><<<grid, 256, 0, a.st>>>(a.dim, 0, parts, (P *)a.dgamma, (P *)a.dbeta, a.accumulate);
     return lm_launched();
 }
 

@@ -305,6 +305,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kTcThreads, 1)
     cluster_sync();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = *(volatile uint32_t *)&tmem_slot;
+    lm_after_previous();
 
     const TcTiles tiles(shape, NH * kTcTile);
     const uint32_t total = tiles.count(), pair = blockIdx.x >> 1, pairs = gridDim.x >> 1;
@@ -554,7 +555,7 @@ inline bool tc_wide(long long m, long long n, int sms)
 
 template <bool A_MN, bool B_MN, int NH, typename Epi>
 bool tc_launch(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, const Epi &epi, int sms,
-               cudaStream_t st)
+               cudaStream_t st, bool next)
 {
     auto *kernel = tc_gemm_kernel<A_MN, B_MN, NH, Epi>;
     static std::atomic<uint64_t> allowed{0};
@@ -568,7 +569,10 @@ bool tc_launch(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, con
     const long long pairs = tiles < sms / 2 ? tiles : sms / 2;
     if(tiles > 0x7fffffff)
         return false;
-    kernel<<<(unsigned)(2 * pairs), kTcThreads, tc_smem(NH), st>>>(a, b, s, epi);
+    if(next)
+        lm_launch_next(kernel, (unsigned)(2 * pairs), kTcThreads, tc_smem(NH), st, a, b, s, epi);
+    else
+        kernel<<<(unsigned)(2 * pairs), kTcThreads, tc_smem(NH), st>>>(a, b, s, epi);
     return true;
 }
 

@@ -106,6 +106,7 @@ __global__ void __launch_bounds__(512)
 {
     __shared__ float2 red[64][kLossRows];
     __shared__ bool last;
+    lm_after_previous();
     const int x = threadIdx.x % kLossRows, w = threadIdx.x / kLossRows;
     const int t = blockIdx.x * kLossRows + x;
     auto add = [](float2 a, float2 b) {  // two (maximum, sum) of disjoint stretches
@@ -200,6 +201,7 @@ __global__ void __launch_bounds__(256)
     __shared__ int before_sum, all_sum, place[32];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int r0 = blockIdx.x * rows_per_block;
+    lm_let_next();
     if(tid == 0)
         before_sum = all_sum = 0;
     __syncthreads();
@@ -457,7 +459,7 @@ bool product(const CUtensorMap &a, const CUtensorMap &b, const TcShape &s, int m
              const Factor &factor, int sms, cudaStream_t st)
 {
     const OutEpilogue<MODE> e = {m, count, n, sum, add, out, stride, rows, factor};
-    return tc_launch<A_MN, B_MN, NH>(a, b, s, e, sms, st);
+    return tc_launch<A_MN, B_MN, NH>(a, b, s, e, sms, st, true);
 }
 
 // Joins the parts of a product that was cut along k, in their order.
@@ -465,6 +467,7 @@ __global__ void __launch_bounds__(256)
     join_kernel(TcShape shape, const int *count, int n, const float *sum, __half *out, size_t stride,
                 const int *rows, int accumulate, Factor factor)
 {
+    lm_after_previous();
     const int live = count ? *count : shape.m, vecs = n / 8;
     const int parts = (int)tc_parts_of(shape, max(live, 1));
     const size_t part_stride = (size_t)live * n;
@@ -617,11 +620,12 @@ int b200opt_vocab_loss_fwd(size_t tokens, size_t vocab, size_t dim, const void *
            !tc_map(&mw, weight, vocab, dim, weight_stride, tc_box(false)))
             return B200OPT_ECUDA;
         TcShape s = {T, V, (int)dim, nullptr, 0, 0, 0, 0, 1, 16};
-        if(!tc_launch<false, false, 1>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt, done}, sms, st))
+        if(!tc_launch<false, false, 1>(mx, mw, s, StatsEpilogue{T, V, targets, wide, part, zt, done}, sms, st,
+                                        false))
             return B200OPT_ECUDA;
-        loss_kernel<<<(unsigned)((tokens + kLossRows - 1) / kLossRows), 512, 0, st>>>(
-            T, V, (int)tiles_of(vocab), part, zt, targets, wide, loss, lse, (float2 *)(ws + p.at_sums), done,
-            stats);
+        lm_launch_next(loss_kernel, (unsigned)((tokens + kLossRows - 1) / kLossRows), 512, 0, st, T, V,
+                       (int)tiles_of(vocab), part, zt, targets, wide, loss, lse, (float2 *)(ws + p.at_sums),
+                       done, stats);
     } else {
         no_stats_kernel<<<1, 1, 0, st>>>(stats);
     }
@@ -702,7 +706,8 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
             return B200OPT_ECUDA;
         // dz = p - onehot
         TcShape s = {T, N, D, count, 1, 0, 0, at, 1, 16};
-        if(!tc_launch<false, false, 1>(x_k, w_k, s, DzEpilogue{count, lsec, target, at, dz, p.piece}, sms, st))
+        if(!tc_launch<false, false, 1>(x_k, w_k, s, DzEpilogue{count, lsec, target, at, dz, p.piece}, sms, st,
+                                        true))
             return B200OPT_ECUDA;
         if(grad_hidden) {  // += dz W
             const bool direct = p.x_parts == 1 && last;
@@ -715,8 +720,8 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
                     grad_hidden_stride, from, factor, sms, st))
                 return B200OPT_ECUDA;
             if(last && !direct)
-                join_kernel<<<sms * 4, 256, 0, st>>>(s, count, D, xsum, (__half *)grad_hidden,
-                                                     grad_hidden_stride, from, 0, factor);
+                lm_launch_next(join_kernel, sms * 4, 256, 0, st, s, count, D, xsum, (__half *)grad_hidden,
+                               grad_hidden_stride, from, 0, factor);
         }
         if(grad_weight) {  // = dz^T X
             __half *to = (__half *)grad_weight + first * grad_weight_stride;
@@ -731,8 +736,8 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
                     factor, sms, st))
                 return B200OPT_ECUDA;
             if(p.w_parts > 1)
-                join_kernel<<<sms * 4, 256, 0, st>>>(s, nullptr, D, wsum, to, grad_weight_stride, nullptr,
-                                                     accumulate, factor);
+                lm_launch_next(join_kernel, sms * 4, 256, 0, st, s, nullptr, D, wsum, to, grad_weight_stride,
+                               nullptr, accumulate, factor);
         }
     }
     return lm_launched();
