@@ -67,6 +67,10 @@ constexpr int kDigits = 512;                              // rows a block can ha
 constexpr size_t kOrderBlocks = 148;
 constexpr int kOrderSmem = kOrderChunk * 4 + kOrderWarps * kDigits * 2;
 
+// Threads of all blocks together, which is how far a thread steps: 2^32 for the
+// largest table, so not a 32-bit number.
+__host__ __device__ constexpr size_t order_step(uint32_t blocks) { return (size_t)blocks * kOrderThreads; }
+
 // Many tokens: that every block looks at all of them would be most of the work
 // (65536 tokens: 42 us, 262144: 153 us).  They are then first dealt out by remainder, three
 // launches of a stable counting pass, and a block looks at its own alone: 23 and 52 us
@@ -345,7 +349,7 @@ __global__ void __launch_bounds__(kOrderThreads, 1)
     if(tid < kDigits)
         for(int i = my_start; i < min(my_end, my_start + kChunk); i++)
             ends[i] = my_end;
-    for(size_t i = (size_t)valid_sum + me * kOrderThreads + tid; i < tokens; i += blocks * kOrderThreads)
+    for(size_t i = (size_t)valid_sum + order_step(me) + tid; i < tokens; i += order_step(blocks))
         keys[i] = (uint32_t)vocab;
 }
 

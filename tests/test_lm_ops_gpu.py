@@ -616,6 +616,23 @@ def test_far_offsets():
     assert int(dw.view(torch.int16).count_nonzero()) == 0
 
 
+def test_embedding_gradient_of_the_largest_table():
+    """As many rows as are allowed, and ids outside the table behind the others."""
+    vocab, tokens = capi.LM_MAX, 300
+    ids = torch.tensor([vocab - 1, 0, vocab - 1, vocab // 2], device=DEV).repeat(tokens // 4)
+    ids[100:150] = -1
+    ids[200] = vocab
+    dy = normal(gen(14), tokens, 1)
+    dw = layers.embedding_backward(ids, dy, vocab)
+    for row in (vocab - 1, 0, vocab // 2):
+        mine = dy[ids == row].double()
+        exact = mine.sum()
+        tol = mine.abs().sum() * U * len(mine) + half_step(exact, dy.dtype)
+        assert abs(float(dw[row, 0]) - float(exact)) <= float(tol) * SLACK
+        dw[row] = 0
+    assert all(int(part.count_nonzero()) == 0 for part in dw.view(-1).view(torch.int16).split(1 << 28))
+
+
 def test_vocab_loss_far_offsets():
     tokens, vocab, dim = 70, 530_000, 4096
     g = gen(13)
