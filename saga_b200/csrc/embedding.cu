@@ -279,12 +279,12 @@ __global__ void __launch_bounds__(kOrderThreads, 1)
                 reinterpret_cast<uint32_t *>(count)[i] = 0;
             __syncwarp();
             for(int i = 0; i < n; i += 32) {  // ranks among the warp's tokens of the same digit
-                if(i + lane < n) {
-                    const unsigned here = __activemask();
-                    const uint32_t e = list[i + lane], d = e & (kDigits - 1);
-                    const unsigned same = __match_any_sync(here, d);
-                    const int lower = __popc(same & ((1u << lane) - 1)), seen = count[d];
-                    __syncwarp(here);
+                const bool have = i + lane < n;  // the others' digit is like no token's
+                const uint32_t e = have ? list[i + lane] : 0, d = have ? e & (kDigits - 1) : kDigits;
+                const unsigned same = __match_any_sync(0xffffffffu, d);
+                const int lower = __popc(same & ((1u << lane) - 1)), seen = have ? count[d] : 0;
+                __syncwarp();
+                if(have) {
                     if(lower == 0)
                         count[d] = (uint16_t)(seen + __popc(same));
                     list[i + lane] = e | (uint32_t)(seen + lower) << 9;

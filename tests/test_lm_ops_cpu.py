@@ -1,5 +1,6 @@
 """Refusals of the language-model operators: decided on the host, before any CUDA call."""
 import ctypes as C
+import os
 
 import pytest
 import torch
@@ -129,3 +130,12 @@ def test_tensor_checks():
                 torch.zeros(())):
         with pytest.raises(ValueError):
             layers._rows(bad, "t")
+
+
+def test_no_kernel_takes_its_lanes_from_what_happens_to_run():
+    """__activemask is whatever lanes arrived together, which CUDA does not promise to be all that took
+    a branch: ranks and counts made from it could split a warp's tokens."""
+    csrc = os.path.join(os.path.dirname(capi.LIB_PATH), "csrc")
+    for name in sorted(os.listdir(csrc)):
+        with open(os.path.join(csrc, name)) as f:
+            assert "__activemask" not in f.read(), name
