@@ -524,6 +524,8 @@ B200OPT_API int b200opt_layernorm_bwd(int dtype, int param_dtype, size_t rows,
  * product, fp16: logits z = hidden weight^T with hidden [tokens][dim] and weight
  * [vocab][dim], lse[t] = log sum_v exp z[t][v], loss[t] = lse[t] - z[t][target].
  * The logits are formed in pieces of the vocabulary in fp32 and never stored.
+ * Logits of -inf (a masked part of the vocabulary) add nothing to lse; a token
+ * whose logits are all -inf has lse -inf, one with a logit of +inf lse +inf.
  *   loss, lse  fp32, one per token (an ignored token has loss 0, its lse is
  *              written as well)
  *   stats      two floats: the sum of the losses and the number of tokens that

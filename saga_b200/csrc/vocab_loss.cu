@@ -23,8 +23,13 @@ __device__ __forceinline__ float exp_fast(float x)
 
 // ------------------------------------------------------------------ forward
 
+// What the exponentials of a stretch are taken from: its maximum, and 0 where that is
+// infinite.  A stretch of -inf alone (a masked part of the vocabulary) then adds 0, where
+// -inf - -inf would make the row NaN, and one with +inf adds +inf.
+__device__ __forceinline__ float base_of(float top) { return fabsf(top) == INFINITY ? 0.0f : top; }
+
 // Per row and tile of the vocabulary: the maximum of z and the sum of
-// exp(z - maximum), in one pass over the accumulator.  The target's logit goes to
+// exp(z - base_of(maximum)), in one pass over the accumulator.  The target's logit goes to
 // zt.
 struct StatsEpilogue {
     int T, V;
@@ -69,10 +74,11 @@ struct StatsEpilogue {
         for(int j = 4; j < 32; j++)
             most[j & 3] = fmaxf(most[j & 3], v[j]);
         const float top = fmaxf(s.top, fmaxf(fmaxf(most[0], most[1]), fmaxf(most[2], most[3])));
-        float sum[4] = {s.sum * exp_fast(s.top - top), 0.0f, 0.0f, 0.0f};
+        const float base = base_of(top);
+        float sum[4] = {s.sum * exp_fast(s.top - base), 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for(int j = 0; j < 32; j++)
-            sum[j & 3] += exp_fast(v[j] - top);
+            sum[j & 3] += exp_fast(v[j] - base);
         s.top = top;
         s.sum = (sum[0] + sum[1]) + (sum[2] + sum[3]);
     }
@@ -90,9 +96,10 @@ struct StatsEpilogue {
 #pragma unroll
         for(int i = 1; i < 4; i++)
             top = fmaxf(top, slots[i * 128].x);
+        const float base = base_of(top);
 #pragma unroll
         for(int i = 0; i < 4; i++)  // a side beyond the vocabulary has -inf and 0
-            sum += slots[i * 128].y * exp_fast(slots[i * 128].x - top);
+            sum += slots[i * 128].y * exp_fast(slots[i * 128].x - base);
         part[(size_t)(col / kTcTile) * T + row] = make_float2(top, sum);
     }
 };
@@ -110,8 +117,8 @@ __global__ void __launch_bounds__(512)
     const int x = threadIdx.x % kLossRows, w = threadIdx.x / kLossRows;
     const int t = blockIdx.x * kLossRows + x;
     auto add = [](float2 a, float2 b) {  // two (maximum, sum) of disjoint stretches
-        const float m = fmaxf(a.x, b.x);
-        return make_float2(m, (a.y ? a.y * exp_fast(a.x - m) : 0.0f) + (b.y ? b.y * exp_fast(b.x - m) : 0.0f));
+        const float m = fmaxf(a.x, b.x), base = base_of(m);
+        return make_float2(m, a.y * exp_fast(a.x - base) + b.y * exp_fast(b.x - base));
     };
     // asked for now, used at the end
     const bool valid = t < T && lm_index_at(y, wide, t, V) >= 0;
@@ -128,10 +135,11 @@ __global__ void __launch_bounds__(512)
 #pragma unroll
         for(int i = 1; i < 16; i++)
             top = fmaxf(top, red[w + 4 * i][x].x);
+        const float base = base_of(top);
 #pragma unroll
         for(int i = 0; i < 16; i++) {
             const float2 p = red[w + 4 * i][x];
-            sum += p.y ? p.y * exp_fast(p.x - top) : 0.0f;
+            sum += p.y * exp_fast(p.x - base);
         }
         mine = make_float2(top, sum);
 #pragma unroll

@@ -465,6 +465,46 @@ def test_vocab_loss_mostly_ignored(tokens, vocab, dim, ignored):
     check_head(x, w, y, f, b, 256.0)
 
 
+@pytest.mark.parametrize("vocab,masked", [
+    (1000, [(0, 32)]), (1000, [(64, 96), (200, 300)]), (1000, [(0, 256)]), (1000, [(0, 1), (2, 1000)]),
+    (1000, [(0, 999)]), (1001, [(960, 1001)]), (1030, [(256, 1024)]), (40000, [(5, 39000)])])
+def test_vocab_loss_masked_vocabulary(vocab, masked):
+    """Whole stretches of logits of -inf, from a column of the table that holds -inf in masked rows
+    and 0 in the others: they count for nothing, in the losses and in both gradients."""
+    tokens, dim = 70, 72
+    x, w, y = head_inputs(tokens, vocab, dim, seed=6)
+    keep = torch.ones(vocab, dtype=torch.bool, device=DEV)
+    for a, b in masked:
+        keep[a:b] = False
+    left = keep.nonzero()[:, 0]
+    x[:, -1], w[:, -1] = 1.0, 0.0
+    ok = (y >= 0) & (y < vocab)
+    y = torch.where(ok, left[y.clamp(0, vocab - 1) % len(left)], y)      # targets that are not masked
+    small = torch.where(ok, torch.searchsorted(left, y), -1)
+    w[~keep, -1] = -float("inf")
+    f = layers.vocab_loss_forward(x, w, y)
+    dx, dw = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=32.0)
+    assert (dw[~keep] == 0).all()
+    assert dx[ok, -1].isnan().all() and (dx[~ok, -1] == 0).all()        # 0 * -inf, as the formula has it
+    dx[:, -1] = layers.vocab_loss_backward(x, w[keep], small, f[1], stats=f[2], grad_scale=32.0)[0][:, -1]
+    check_head(x, w[keep], small, f, (dx, dw[keep]), 32.0)
+
+
+def test_vocab_loss_infinite_logits():
+    """A token whose logits are all -inf, then one of them +inf, beside ordinary tokens."""
+    x, w, y = head_inputs(40, 700, 64, ignored=0)
+    x[:, 0], w[:, 0], x[7] = 0.0, -1.0, 0.0
+    x[7, 0] = float("inf")
+    y[y == 300] = 299
+    others = [t for t in range(40) if t != 7]
+    for at_300, lse, loss in ((-1.0, -float("inf"), None), (1.0, float("inf"), float("inf"))):
+        w[300, 0] = at_300
+        got = layers.vocab_loss_forward(x, w, y)
+        assert got[1][7] == lse and (got[0][7].isnan() if loss is None else got[0][7] == loss)
+        check_head(x[others], w, y[others], (got[0][others], got[1][others],
+                                             layers.vocab_loss_forward(x[others], w, y[others])[2]), None, 1.0)
+
+
 @pytest.mark.parametrize("std", [0.0, 30.0])
 def test_vocab_loss_flat_and_peaked_distributions(std):
     g = gen(17)
