@@ -102,6 +102,11 @@ SIGNATURES = {
 _lib = None
 
 
+class DeviceAddress(int):
+    """An address in device memory, told apart from a number: what a call reads there is checked by
+    nobody, so only a value that was made as an address is taken as one."""
+
+
 class B200OptError(RuntimeError):
     def __init__(self, status, detail=""):
         self.status = status

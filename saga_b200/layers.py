@@ -285,13 +285,25 @@ def vocab_loss_forward(hidden, weight, targets, loss=None, lse=None, stats=None,
     return loss, lse, stats
 
 
+def _scale_address(t, index):
+    """Device address of the loss scale; None where there is none."""
+    if t is None or isinstance(t, capi.DeviceAddress):
+        return t
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"loss_scale is a {type(t).__name__}: a one-element CUDA tensor or a "
+                        "capi.DeviceAddress expected (give a number as grad_scale)")
+    return _vector(t, "loss_scale", 1, torch.float32, index)
+
+
 def vocab_loss_backward(hidden, weight, targets, lse, stats=None, grad_scale=1.0, loss_scale=None,
                         grad_hidden=None, grad_weight=None, accumulate=False, workspace=None,
                         stream=None):
     """(grad_hidden, grad_weight) of the losses' mean (``stats`` of the forward pass given) or sum,
-    times grad_scale and times the loss scale: a one-element fp32 tensor, or a device address such
-    as ``AdamGroup.device_scale_ptr()`` returns."""
+    times grad_scale and times the loss scale: a one-element fp32 tensor, or a
+    ``capi.DeviceAddress`` such as ``AdamGroup.device_scale_ptr()`` returns.  A scale that the host
+    knows, a plain number, is part of grad_scale."""
     dev, sizes, args = _head(hidden, weight, targets)
+    scale_ptr = _scale_address(loss_scale, dev)
     tokens, vocab, dim = sizes
     if accumulate and grad_weight is None:
         raise ValueError("accumulate needs grad_weight")
@@ -305,12 +317,10 @@ def vocab_loss_backward(hidden, weight, targets, lse, stats=None, grad_scale=1.0
         ws = dim
     else:
         ws = _matrix(grad_weight, "grad_weight", vocab, dim, torch.float16, dev)
-    if loss_scale is not None and not isinstance(loss_scale, int):
-        loss_scale = _vector(loss_scale, "loss_scale", 1, torch.float32, dev)
     keep, wp, wb = _workspace(workspace, _bytes("b200opt_vocab_loss_bwd_workspace", *sizes), hidden,
                               dev, stream)
     _call(lib().b200opt_vocab_loss_bwd, dev, stream, *sizes, *args,
           _vector(lse, "lse", tokens, torch.float32, dev),
-          _vector(stats, "stats", 2, torch.float32, dev), grad_scale, loss_scale,
+          _vector(stats, "stats", 2, torch.float32, dev), grad_scale, scale_ptr,
           grad_hidden.data_ptr(), xs, grad_weight.data_ptr(), ws, int(accumulate), wp, wb)
     return grad_hidden, grad_weight

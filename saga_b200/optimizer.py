@@ -224,9 +224,10 @@ class AdamGroup:
                                                 log_capacity), self._h)
 
     def device_scale_ptr(self):
+        """The live scale's address, as vocab_loss_backward takes it for loss_scale."""
         p = C.c_void_p()
         check(lib().b200opt_device_scale_ptr(self._h, C.byref(p)), self._h)
-        return p.value
+        return capi.DeviceAddress(p.value)
 
     def exec_device_scale(self, lr, l2_lambda, stream=0):
         """Like exec, with 1/scale read from and the policy applied on the device."""

@@ -132,6 +132,17 @@ def test_tensor_checks():
             layers._rows(bad, "t")
 
 
+def test_loss_scale_that_is_a_number_is_refused():
+    """A number is not an address: only a tensor, or a value that says it is one, is read from."""
+    for number in (1024, 0, True, 1024.0, C.c_float(1.0)):
+        with pytest.raises(TypeError, match="grad_scale"):
+            layers._scale_address(number, 0)
+    with pytest.raises(ValueError):
+        layers._scale_address(torch.ones(1), 0)          # not on a GPU
+    assert layers._scale_address(None, 0) is None
+    assert layers._scale_address(capi.DeviceAddress(A), 0) == A
+
+
 def test_no_kernel_takes_its_lanes_from_what_happens_to_run():
     """__activemask is whatever lanes arrived together, which CUDA does not promise to be all that took
     a branch: ranks and counts made from it could split a warp's tokens."""

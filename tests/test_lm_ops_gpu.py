@@ -870,6 +870,19 @@ def test_tensor_refusals():
             call()
 
 
+def test_loss_scale_is_a_tensor_or_a_device_address():
+    x, w, y = head_inputs(20, 100, 64)
+    f = layers.vocab_loss_forward(x, w, y)
+    scale = torch.full((1,), 1024.0, device=DEV)
+    want = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=1024.0)
+    for given in (scale, capi.DeviceAddress(scale.data_ptr())):
+        got = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], loss_scale=given)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    for number in (1024, 1024.0, True):
+        with pytest.raises(TypeError):
+            layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], loss_scale=number)
+
+
 # -------------------------------------------------- together with the optimizer
 
 def test_training_step_of_a_tied_model_through_the_optimizer():
