@@ -148,10 +148,11 @@ __global__ void __launch_bounds__(512)
                                          __shfl_xor_sync(0xffffffffu, mine.y, o)));
         float own = 0.0f, counted = 0.0f;
         if(t < T && w == 0) {
-            const float l = mine.x + logf(mine.y);
-            lse[t] = l;
+            const float l = logf(mine.y);
+            lse[t] = mine.x + l;
             if(valid) {
-                own = l - target;
+                // not from lse: its rounding, at a large logit, would be all of a small loss
+                own = (mine.x - target) + l;
                 counted = 1.0f;
             }
             loss[t] = own;

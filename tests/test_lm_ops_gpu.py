@@ -543,6 +543,27 @@ def test_vocab_loss_next_to_certainty():
     assert (dx == 0).all() and (dw == 0).all()
 
 
+@pytest.mark.parametrize("vocab,top,gap", [(2, 24.0, 13.75), (2, 1000.0, 14.0), (40, 1000.0, 14.0),
+                                           (2, -500.0, 12.0), (300, 30000.0, 16.0), (1, 24.0, 0.0)])
+def test_vocab_loss_small_losses_under_large_logits(vocab, top, gap):
+    """Logits that are exact: `top` for the target, `top - gap` for the others.  The loss is
+    log(1 + (vocab - 1) exp(-gap)): vocab - 1 additions to a sum near 1, a half step each, and a few
+    steps of exp and log; nothing of the size of the logits."""
+    x = torch.zeros(40, 8, dtype=torch.float16, device=DEV)
+    x[:, 0] = 1.0
+    w = torch.zeros(vocab, 8, dtype=torch.float16, device=DEV)
+    w[:, 0] = top - gap
+    w[vocab // 2, 0] = top
+    assert float(w[0, 0]) == (top - gap if vocab > 1 else top) and float(w[vocab // 2, 0]) == top
+    y = torch.full((40,), vocab // 2, device=DEV)
+    loss, lse, stats = layers.vocab_loss_forward(x, w, y)
+    exact = torch.log1p((vocab - 1) * torch.exp(torch.full((40,), -gap, device=DEV, dtype=torch.float64)))
+    tol = exact * 32 * U + (vocab - 1) * U
+    close(loss, exact, tol)
+    close(stats[0], exact.sum(), tol.sum() + 40 * U * exact.sum())
+    close(lse, exact + top, tol + abs(top) * U)
+
+
 def test_vocab_loss_all_ignored():
     x, w, y = head_inputs(40, 100, 64)
     y[:] = -1
