@@ -494,7 +494,8 @@ B200OPT_API int b200opt_embedding_bwd(int dtype, size_t tokens, size_t vocab,
  * Layer norm over the last dimension: y = (x - mean) * rstd * gamma + beta with
  * rstd = 1/sqrt(variance + eps), the variance taken around the mean.  gamma and
  * beta are vectors of dtype param_dtype; either may be NULL (1 and 0).  mean and
- * rstd (fp32, one per row) may be NULL when no gradient will be asked for.
+ * rstd (fp32, one per row) may be NULL when no gradient will be asked for; they
+ * are NaN for rows of no elements (dim 0).
  * param_dtype B200OPT_HALF needs dtype B200OPT_HALF.
  */
 B200OPT_API int b200opt_layernorm_fwd(int dtype, int param_dtype, size_t rows,

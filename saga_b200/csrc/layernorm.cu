@@ -566,7 +566,7 @@ int b200opt_layernorm_fwd(int dtype, int param_dtype, size_t rows, size_t dim, c
         return B200OPT_EINVAL;
     if(rows > B200OPT_LM_MAX || dim > B200OPT_LM_MAX)
         return B200OPT_ETOOBIG;
-    if(!rows || !dim)
+    if(!rows || (!dim && !mean && !rstd))
         return B200OPT_OK;
     const size_t e = lm_size(dtype), p = lm_size(param_dtype);
     if(!lm_matrix(x, rows, dim, x_stride, e) || !lm_matrix(y, rows, dim, y_stride, e) ||

@@ -308,6 +308,17 @@ def test_layernorm_large_mean_and_non_finite_rows():
     assert got[2].isnan().any() and got[4].isnan().all()
 
 
+@pytest.mark.parametrize("dtype,params", KINDS)
+def test_layernorm_rows_without_elements(dtype, params):
+    """A mean over nothing is NaN, as the formula has it, and not what the memory held."""
+    x, none = torch.zeros(700, 0, device=DEV, dtype=dtype), torch.zeros(0, device=DEV, dtype=params)
+    mean, rstd = torch.full((700,), 3.0, device=DEV), torch.full((700,), 4.0, device=DEV)
+    y, m, r = layers.layernorm_forward(x, none, none, mean=mean, rstd=rstd)
+    assert y.shape == (700, 0) and m.isnan().all() and r.isnan().all()
+    gx, gg, gb = layers.layernorm_backward(x, x, none, m, r)
+    assert gx.shape == (700, 0) and gg.shape == gb.shape == (0,)
+
+
 def test_layernorm_no_rows_gives_zero_parameter_gradients():
     x = torch.zeros(0, 96, device=DEV)
     s = torch.zeros(0, device=DEV)
