@@ -727,6 +727,93 @@ def test_vocab_loss_far_offsets():
     close(dw[tail], want, size * (2.0 ** -11 + 2 * e_z + 2 * tokens * U) + half_step(want, torch.float16))
 
 
+def grid(g, *shape, steps, unit):
+    """Whole multiples of `unit`, up to `steps` of them either way: products and sums of such values
+    are exact in fp32 as long as they stay under 2^24 units, in any order."""
+    return torch.randint(-steps, steps + 1, shape, generator=g, device=DEV, dtype=torch.int8).half().mul_(unit)
+
+
+def exact_logits_dz(z, lse, e_lse, y):
+    """p - onehot from exact logits, and what the fp16 value that the products read may be off by."""
+    p = torch.exp(z - lse[:, None])
+    dz = p.clone()
+    dz[torch.arange(len(y), device=DEV), y] -= 1
+    return dz, p * (e_lse[:, None] + 4 * U * (1 + (z - lse[:, None]).abs())) + (2.0 ** -11 + U) * dz.abs() + 2.0 ** -40
+
+
+@pytest.mark.parametrize("tokens,vocab,dim", [(300, 5003, 512), (129, 20011, 1032), (1000, 999, 64)])
+def test_vocab_loss_with_exact_logits(tokens, vocab, dim):
+    """Logits without any error leave nothing but the exponentials, the sums and the logarithm to the
+    losses: bounds hundreds of times closer than those of rounded products."""
+    g = gen(tokens)
+    x, w = grid(g, tokens, dim, steps=4, unit=0.25), grid(g, vocab, dim, steps=8, unit=2.0 ** -6)
+    y = integers(g, tokens, 0, vocab)
+    assert dim * 4 * 8 < 2 ** 24
+    loss, lse, stats = layers.vocab_loss_forward(x, w, y)
+    z = x.double() @ w.double().t()
+    want = torch.logsumexp(z, 1)
+    e_lse = (chain(vocab) + 16) * U + 2 * U * want.abs() + 4 * U * (z.amax(1) - z.amin(1))
+    close(lse, want, e_lse + half_step(want, torch.float32))
+    exact = want - z.gather(1, y[:, None])[:, 0]
+    e_loss = e_lse + 2 * U * exact
+    close(loss, exact, e_loss)
+    close(stats[0], exact.sum(), e_loss.sum() + chain(tokens) * U * exact.sum())
+    dx, dw = layers.vocab_loss_backward(x, w, y, lse, stats=stats, grad_scale=1024.0)
+    f = 1024.0 / tokens
+    dz, e_dz = exact_logits_dz(z, want, e_lse + half_step(want, torch.float32), y)
+    for got, ref, size, e, n in ((dx, dz @ w.double(), dz.abs() @ w.double().abs(), e_dz @ w.double().abs(), vocab),
+                                 (dw, dz.t() @ x.double(), dz.t().abs() @ x.double().abs(),
+                                  e_dz.t() @ x.double().abs(), tokens)):
+        ref = f * ref
+        close(got, ref, f * (e + 2 * n * U * size) + 4 * U * ref.abs() + half_step(ref, torch.float16))
+
+
+def test_vocab_loss_far_rows_decide():
+    """The rows of the table beyond 2^31 elements hold the targets and nearly all of the probability:
+    losses and both gradients are theirs.  Exact logits, as above.  Left out, they would move lse by
+    more than 10; what the other rows add to a gradient is rounded relative to their own small sums."""
+    tokens, vocab, dim = 70, 530_000, 4096
+    far = 2 ** 31 // dim
+    g = gen(15)
+    w = torch.empty(vocab, dim, dtype=torch.float16, device=DEV)
+    for at in range(0, vocab, 53_000):
+        w[at:at + 53_000] = grid(g, 53_000, dim, steps=2, unit=2.0 ** -6)
+    w[far:] *= 16
+    x = grid(g, tokens, dim, steps=4, unit=0.25)
+    y = integers(g, tokens, far + 500, vocab)
+    assert dim * 4 * 2 * 16 < 2 ** 24
+    loss, lse, stats = layers.vocab_loss_forward(x, w, y)
+    dx, dw = layers.vocab_loss_backward(x, w, y, lse, stats=stats, grad_scale=4096.0)
+    xd, parts = x.double(), [(a, min(a + 53_000, far)) for a in range(0, far, 53_000)] + [(far, vocab)]
+    logits = lambda a, b: xd @ w[a:b].double().t()
+    near = torch.full((tokens,), -float("inf"), device=DEV, dtype=torch.float64)
+    low = -near
+    for a, b in parts[:-1]:
+        z = logits(a, b)
+        near, low = torch.logaddexp(near, torch.logsumexp(z, 1)), torch.minimum(low, z.amin(1))
+    z = logits(far, vocab)
+    want = torch.logaddexp(near, torch.logsumexp(z, 1))
+    assert (want - near > 10).all()
+    e_lse = (chain(vocab) + 16) * U + 2 * U * want + 4 * U * (z.amax(1) - torch.minimum(low, z.amin(1)))
+    close(lse, want, e_lse + half_step(want, torch.float32))
+    exact = want - z.gather(1, (y - far)[:, None])[:, 0]
+    close(loss, exact, e_lse + 2 * U * exact)
+    f = 4096.0 / tokens
+    e_lse += half_step(want, torch.float32)
+    dz, e_dz = exact_logits_dz(z, want, e_lse, y - far)
+    ref, size = f * dz.t() @ xd, f * dz.t().abs() @ xd.abs()
+    close(dw[far:], ref, f * e_dz.t() @ xd.abs() + 2 * tokens * U * size + 4 * U * ref.abs() + half_step(ref, torch.float16))
+    ref = dz @ w[far:].double()
+    tol = e_dz @ w[far:].double().abs() + 2 * (vocab - far + 128) * U * (dz.abs() @ w[far:].double().abs())
+    for a, b in parts[:-1]:
+        z, wd = logits(a, b), w[a:b].double()
+        p = torch.exp(z - want[:, None])
+        ref += p @ wd
+        tol += (p * (e_lse[:, None] + 4 * U * (1 + (z - want[:, None]).abs()) + 2.0 ** -11 + 2 * vocab * U) + 2.0 ** -40) @ wd.abs()
+    ref, tol = f * ref, f * tol
+    close(dx, ref, tol + 4 * U * ref.abs() + half_step(ref, torch.float16))
+
+
 # -------------------------------------------- streams, graphs, several at once
 
 def _calls():
