@@ -504,9 +504,11 @@ int bwd_with(const Args &a)
     // 55; x 1024: 29 and 31), eight columns otherwise (fp32 x 1024: 39 us; a warp a
     // row with 32 columns 53).
     constexpr int FEW = N == 8 ? 2 : 8 / N, MOST = 32 / N;
-    if(!pick<1, 1, FEW>(vecs, launch) && !pick<2, FEW, FEW>(vecs, launch) &&
-       !pick<4, FEW, FEW>(vecs, launch) && !pick<8, FEW, MOST>(vecs, launch) &&
-       !(N == 8 && pick<16, 4, 4>(vecs, launch))) {
+    bool held = pick<1, 1, FEW>(vecs, launch) || pick<2, FEW, FEW>(vecs, launch) ||
+                pick<4, FEW, FEW>(vecs, launch) || pick<8, FEW, MOST>(vecs, launch);
+    if constexpr(N == 8)
+        held = held || pick<16, 4, 4>(vecs, launch);
+    if(!held) {
         if(a.dx && a.rows)
             layernorm_bwd_long_kernel<<<(unsigned)a.rows, 1024, 0, a.st>>>(
                 a.dim, (const T *)a.dy, a.ys, (const T *)a.x, a.xs, (const P *)a.gamma, a.mean_in,
