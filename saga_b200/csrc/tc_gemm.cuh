@@ -538,19 +538,25 @@ inline bool tc_map(CUtensorMap *map, const void *p, size_t rows, size_t cols, si
 constexpr unsigned tc_box(bool mn) { return mn ? kTcK : kTcHalf; }
 
 // Whether a product of two MN-major operands is faster in wide tiles, which fetch a
-// quarter less per flop: 9 % in grad_weight's product (16384 x 4096, 8192 tokens:
-// 980 us narrow, 912 wide; 512 columns: 116 and 98), nothing with K-major operands,
-// whose callers keep to narrow ones (losses of 8192 x 128000, 512 columns: 876 us
-// narrow, 982 wide).  There are half as many wide tiles to spread over the pairs, so
-// they are taken where the turns that the pairs make, counted in narrow tiles, grow
-// by less than that gain.
-inline bool tc_wide(long long m, long long n, int sms)
+// quarter less per flop but have four stages of k instead of five, and both
+// accumulators, so that a tile's epilogue overlaps less of the next one.  That pays for
+// itself with a long k (grad_weight's product, m = 16384, n = 4096, as many turns both ways;
+// us narrow and wide: k = 512 63 and 76, 1024 110 and 113, 1280 125 and 125, 1536 146 and
+// 143, 2048 202 and 194, 8192 803 and 717).  There are half as many wide tiles to spread
+// over the pairs, so the turns that the pairs make, counted in narrow tiles, can grow:
+// by 5 % is as much as a k of 2048 allows (48640 x 2048: 305 and 303), by 9 % from 4096 on
+// (15360 x 4096, 8 % more turns: k = 2048 188 and 191, 4096 360 and 356, 8192 747 and 708).
+// K-major operands gain nothing, and their callers keep to narrow tiles (losses of 8192 x
+// 128000, 512 columns: 876 us narrow, 982 wide).
+inline bool tc_wide(long long m, long long n, long long k, int sms)
 {
+    if(k < 1536)
+        return false;
     const long long mt = (m + kTcTile - 1) / kTcTile, pairs = sms / 2 > 0 ? sms / 2 : 1;
     const long long narrow = mt * ((n + kTcTile - 1) / kTcTile);
     const long long wide = mt * ((n + 2 * kTcTile - 1) / (2 * kTcTile));
     const long long turns = (narrow + pairs - 1) / pairs, turns2 = 2 * ((wide + pairs - 1) / pairs);
-    return 100 * turns2 <= 109 * turns;
+    return 100 * turns2 <= (k < 4096 ? 105 : 109) * turns;
 }
 
 template <bool A_MN, bool B_MN, int NH, typename Epi>

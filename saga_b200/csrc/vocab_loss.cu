@@ -735,7 +735,8 @@ int b200opt_vocab_loss_bwd(size_t tokens, size_t vocab, size_t dim, const void *
         if(grad_weight) {  // = dz^T X
             __half *to = (__half *)grad_weight + first * grad_weight_stride;
             s = {N, D, T, count, 0, 1, 0, 0, (int)p.w_parts, 8};
-            const bool wide_tiles = tc_wide(N, D, sms);
+            // (by all tokens: how many are ignored is known on the device alone)
+            const bool wide_tiles = tc_wide(N, D, T, sms);
             auto *run = p.w_parts > 1 ? product<true, true, 1, kSums>
                         : accumulate  ? (wide_tiles ? product<true, true, 2, kAccumulate>
                                                     : product<true, true, 1, kAccumulate>)

@@ -456,6 +456,21 @@ def test_vocab_loss_wide_tiles(tokens, vocab, dim, accumulate):
     check_head(x, w, y, f, b, 512.0, base=base)
 
 
+@pytest.mark.parametrize("tokens,vocab,dim,ignored,accumulate", [
+    (1600, 9400, 520, 0.2, False), (1600, 9400, 520, 0.2, True), (1600, 9300, 1024, 0.98, False),
+    (1537, 9400, 1000, 0.9, True), (1700, 9400, 520, 0.999, False), (4100, 9400, 512, 0.5, True)])
+def test_vocab_loss_wide_tiles_of_many_tokens(tokens, vocab, dim, ignored, accumulate):
+    """Tokens enough for tiles of 512 columns; those that are left of them fill many stages of the
+    ring, a few or one."""
+    x, w, y = head_inputs(tokens, vocab, dim, seed=10, ignored=ignored)
+    y[7] = 5
+    base = normal(gen(2), vocab, dim) if accumulate else None
+    f = layers.vocab_loss_forward(x, w, y)
+    b = layers.vocab_loss_backward(x, w, y, f[1], stats=f[2], grad_scale=512.0, accumulate=accumulate,
+                                   grad_weight=base.clone() if accumulate else None)
+    check_head(x, w, y, f, b, 512.0, base=base)
+
+
 @pytest.mark.parametrize("tokens,vocab", [(8200, 20000), (9600, 14000)])
 def test_vocab_loss_several_pieces_of_the_vocabulary(tokens, vocab):
     """With the sums of grad_hidden in parts, and whole."""
