@@ -475,8 +475,9 @@ B200OPT_API int b200opt_embedding_fwd(int dtype, size_t tokens, size_t vocab,
                        void *out, size_t out_stride, void *stream);
 
 /*
- * grad_weight[v] = scale * sum over the tokens t with ids[t] == v, in
- * ascending t, of grad_out[t].  All vocab rows are written (rows that no token
+ * grad_weight[v] = scale * sum over the tokens t with ids[t] == v of
+ * grad_out[t], added in an order that the ids and sizes fix (the tokens of a
+ * frequent id in parts).  All vocab rows are written (rows that no token
  * names become zero), so that grad_weight can be a tensor of the flat gradient
  * buffer; with `accumulate` the sum is added to the rows that tokens name and
  * the others are not touched.

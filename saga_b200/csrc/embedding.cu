@@ -74,7 +74,11 @@ __host__ __device__ constexpr size_t order_step(uint32_t blocks) { return (size_
 // Many tokens: that every block looks at all of them would be most of the work
 // (65536 tokens: 42 us, 262144: 153 us).  They are then first dealt out by remainder, three
 // launches of a stable counting pass, and a block looks at its own alone: 23 and 52 us
-// together.  At 32768 tokens both ways take 22 us.
+// together.  At 32768 tokens both ways take 22 us.  The dealing has counters for kDigits
+// blocks, so it ends where kDigits rows a block need more of them, at kDigits * kDigits =
+// 262144 rows.  Beyond, all blocks (one for every 512 rows, several turns of the GPU) look
+// at all ids: the whole gradient of 65536 tokens x 16 takes 47 us with 262144 rows and
+// 163 us with 262145, of 262144 tokens 73 and 573 us.
 
 constexpr size_t kSplitTokens = 32768;
 constexpr int kDealTokens = 2048;  // of a block: 32 warps, 64 each (8192: the move takes 23 us, not 7.5)
