@@ -287,7 +287,11 @@ def vocab_loss_forward(hidden, weight, targets, loss=None, lse=None, stats=None,
 
 def _scale_address(t, index):
     """Device address of the loss scale; None where there is none."""
-    if t is None or isinstance(t, capi.DeviceAddress):
+    if t is None:
+        return None
+    if isinstance(t, capi.DeviceAddress):
+        if not t:
+            raise ValueError("loss_scale is the null address: None stands for no loss scale")
         return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"loss_scale is a {type(t).__name__}: a one-element CUDA tensor or a "

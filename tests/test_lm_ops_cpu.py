@@ -139,6 +139,8 @@ def test_loss_scale_that_is_a_number_is_refused():
             layers._scale_address(number, 0)
     with pytest.raises(ValueError):
         layers._scale_address(torch.ones(1), 0)          # not on a GPU
+    with pytest.raises(ValueError, match="null"):
+        layers._scale_address(capi.DeviceAddress(0), 0)
     assert layers._scale_address(None, 0) is None
     assert layers._scale_address(capi.DeviceAddress(A), 0) == A
 
